@@ -1,0 +1,536 @@
+"""Cases of the learned-filter operators (short causal convolution, selective state-space scan) and of the AdamW step over many
+tensors: what is timed, on which inputs, with the operators' plain forms and their values in 64 bits.
+
+Axes are the framework's: [trial (batch), time, channel].  Activations are slices of one projection's output, as a model hands them
+on: their time stride is wider than their channel count."""
+import torch
+
+own = False
+
+F8_MAX = 448.0            # largest e4m3 value
+BLOCK = 256               # elements that share one scale in the 8-bit states
+TINY = 1e-30              # a block whose largest magnitude is below this is held as zeros
+TYPES = {"f32": torch.float32, "f64": torch.float64, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def listed():
+    return [
+        # a batch of prompts through the convolution in front of the scan, its last rows kept for the single-step form
+        dict(name="conv prompt bf16", op="conv", mode="forward", B=4, T=2048, D=4096, W=4, dtype="bf16", silu=True, bias=True,
+             state=False, ragged=False),
+        # a training pass over tracking trials: odd width, a warm start, trials of different lengths
+        dict(name="conv train f32 ragged", op="conv", mode="train", B=20, T=1067, D=771, W=3, dtype="f32", silu=False, bias=True,
+             state=True, ragged=True),
+        # one new sample for each of 64 running sequences
+        dict(name="conv step bf16", op="conv", mode="step", B=64, T=1, D=4096, W=4, dtype="bf16", silu=True, bias=True,
+             state=True, ragged=False),
+        # a batch of prompts through the scan
+        dict(name="scan prompt bf16", op="scan", mode="forward", B=8, T=2048, D=2048, N=16, G=1, dtype="bf16", gate=True,
+             state=False, ragged=False),
+        # one long sequence, few channels: only the time axis can fill the card
+        dict(name="scan long bf16", op="scan", mode="forward", B=1, T=16384, D=1024, N=16, G=1, dtype="bf16", gate=True,
+             state=True, ragged=False),
+        # a training pass of the same model
+        dict(name="scan train bf16", op="scan", mode="train", B=4, T=2048, D=2048, N=16, G=1, dtype="bf16", gate=True,
+             state=False, ragged=False),
+        # a training pass over trials of the tracking horizon: six states, three groups, odd width, ragged lengths
+        dict(name="scan train f32 ragged", op="scan", mode="train", B=20, T=500, D=771, N=6, G=3, dtype="f32", gate=False,
+             state=True, ragged=True),
+        # one new sample of one sequence: latency
+        dict(name="scan step one", op="scan", mode="step", B=1, T=1, D=2048, N=16, G=1, dtype="bf16", gate=True, state=True,
+             ragged=False),
+        # one new sample for each of 256 running sequences
+        dict(name="scan step batch", op="scan", mode="step", B=256, T=1, D=4096, N=16, G=1, dtype="bf16", gate=True, state=True,
+             ragged=False),
+        # four parameters of 4096 candidates, in the precision of the inference drivers: latency
+        dict(name="adamw population f64", op="adamw", layers=0, width=4096, tensors=4, dtype="f64", bits=32),
+        # the weights of a stack of learned filters
+        dict(name="adamw stack f32", op="adamw", layers=10, width=1024, tensors=0, dtype="f32", bits=32),
+        # the same with moments in 8 bits and weights in bfloat16
+        dict(name="adamw stack bf16 8bit", op="adamw", layers=10, width=1024, tensors=0, dtype="bf16", bits=8),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(lo * (hi / lo) ** rng.random()))
+
+
+def draw(rng):
+    op = rng.choice(("conv", "scan", "adamw"))
+    if op == "adamw":
+        bits = rng.choice((32, 8))
+        dtype = rng.choice(("f32", "bf16", "f16") if bits == 8 else ("f32", "f64", "bf16", "f16"))
+        if rng.random() < 0.4:
+            return dict(op=op, layers=0, width=_log(rng, 1, 1 << 18), tensors=_log(rng, 1, 48), dtype=dtype, bits=bits)
+        return dict(op=op, layers=rng.randint(1, 6), width=_log(rng, 65, 1024), tensors=0, dtype=dtype, bits=bits)
+    mode = rng.choice(("forward", "train", "step"))
+    case = dict(op=op, mode=mode, dtype=rng.choice(("f32", "bf16", "f16")), state=mode == "step" or rng.random() < 0.5,
+                ragged=mode != "step" and rng.random() < 0.5)
+    if mode == "step":
+        case.update(B=_log(rng, 1, 256), T=1, D=_log(rng, 60, 4096))
+    else:
+        T, D = _log(rng, 1, 8192), _log(rng, 60, 4096)
+        most = (1 << 25 if op == "conv" else 1 << 23) // (T * D)
+        case.update(B=_log(rng, 1, max(1, min(64, most))), T=T, D=D if most else max(60, D // 4))
+    if op == "conv":
+        case.update(W=rng.randint(1, 4), silu=rng.random() < 0.5, bias=rng.random() < 0.5)
+    else:
+        G = rng.choice((1, 1, 2, 3))
+        case.update(D=case["D"] // G * G, N=rng.choice((1, 6, 8, 13, 16, 16, 16)), G=G, gate=rng.random() < 0.5)
+    return case
+
+
+def _sizes(case):
+    """Shapes of the parameter tensors of an AdamW case."""
+    if not case["layers"]:
+        return [(case["width"],)] * case["tensors"]
+    w, e, r, n = case["width"], 2 * case["width"], max(1, case["width"] // 16), 16
+    return [(2 * e, w), (e, 4), (e,), (r + 2 * n, e), (e, r), (e,), (e, n), (e,), (w, e), (w,)] * case["layers"]
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    dt = TYPES[case["dtype"]]
+
+    def normal(*shape, scale=1.0, dtype=dt):
+        return (torch.randn(*shape, generator=gen, device=dev) * scale).to(dtype)
+
+    if case["op"] == "adamw":
+        shapes = _sizes(case)
+        numels = [int(torch.Size(s).numel()) for s in shapes]
+        starts, total = [], 0
+        for n in numels:                     # each tensor begins at a multiple of BLOCK in one array
+            starts.append(total)
+            total += -(-n // BLOCK) * BLOCK
+        live = torch.zeros(total, dtype=torch.bool, device=dev)
+        for s, n in zip(starts, numels):
+            live[s:s + n] = True
+        st = torch.float64 if dt == torch.float64 else torch.float32
+        spread = torch.exp(1.5 * torch.randn(total, generator=gen, device=dev))         # gradients' scales differ by element
+        p = torch.where(live, normal(total, scale=0.1).to(st), 0).to(dt)
+        g = torch.where(live, normal(total, scale=0.01).to(st) * spread, 0).to(dt)
+        m = torch.where(live, normal(total, scale=0.003).to(st) * spread, 0)
+        v = torch.where(live, (normal(total, scale=0.01).to(st) * spread) ** 2 + 1e-8, 0)
+        state = dict(case=case, p=p, g=g, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, step=100)
+        if case["bits"] == 8:
+            state["m"], state["m_scale"] = _pack(m)
+            state["r"], state["r_scale"] = _pack(torch.sqrt(v))
+        else:
+            state["m"], state["v"] = m, v
+        if own:                              # the optimiser a program keeps, over views of the same arrays
+            from lqg_amd.optim import AdamW
+            params = []
+            for s, n, shape in zip(starts, numels, shapes):
+                t = p[s:s + n].view(shape).requires_grad_(True)
+                t.grad = g[s:s + n].view(shape)
+                params.append(t)
+            opt = AdamW(params, lr=state["lr"], betas=state["betas"], eps=state["eps"], weight_decay=state["weight_decay"],
+                        state_bits=case["bits"])
+            saved = dict(step=state["step"] - 1, exp_avg=state["m"])
+            if case["bits"] == 8:
+                saved.update(exp_avg_scale=state["m_scale"], exp_rms=state["r"], exp_rms_scale=state["r_scale"])
+            else:
+                saved.update(exp_avg_sq=state["v"])
+            opt.load_state_dict(saved)
+            state["opt"] = opt
+        return state
+    B, T, D = case["B"], case["T"], case["D"]
+    state = dict(case=case)
+    train, step = case["mode"] == "train", case["mode"] == "step"
+    if case["ragged"]:
+        state["lengths"] = torch.randint(0, T + 1, (B,), generator=gen, device=dev, dtype=torch.int32)
+    if case["op"] == "conv":
+        W = case["W"]
+        both = normal(B, T, 2 * D)           # the convolution's half of a projection
+        state["x"] = both[..., :D]
+        state["w"] = normal(D, W, scale=0.5)
+        state["bias"] = normal(D, scale=0.1) if case["bias"] else None
+        state["state"] = normal(B, W - 1, D) if case["state"] else None
+        if train:
+            state["dy"] = normal(B, T, D)
+    else:
+        N, G = case["N"], case["G"]
+        both = normal(B, T, 2 * D)
+        state["u"] = both[..., :D]
+        state["z"] = both[..., D:] if case["gate"] else None
+        proj = normal(B, T, 2 * G * N)
+        state["Bm"], state["Cm"] = proj[..., :G * N].unflatten(-1, (G, N)), proj[..., G * N:].unflatten(-1, (G, N))
+        state["delta"] = normal(B, T, D, scale=0.5)
+        # a time constant of 1 .. 1000 steps for each channel, decay rates -1 .. -N for its states
+        state["delta_bias"] = torch.log(torch.expm1(torch.exp(torch.rand(D, generator=gen, device=dev) * 4.6 - 6.9)))
+        rates = torch.arange(1, N + 1, device=dev, dtype=torch.float32)
+        state["A"] = -rates * torch.exp(0.1 * torch.randn(D, N, generator=gen, device=dev))
+        state["D"] = torch.ones(D, device=dev) + normal(D, scale=0.1, dtype=torch.float32)
+        state["state"] = normal(B, D, N, dtype=torch.float32) if case["state"] else None
+        if train:
+            state["dy"] = normal(B, T, D)
+    if step:
+        for k in ("x", "u", "z", "delta", "Bm", "Cm"):
+            if state.get(k) is not None:
+                state[k] = state[k][:, 0]
+    return state
+
+
+def _pack(x):
+    """Blocks of BLOCK elements -> (e4m3 codes, a float scale for each block)."""
+    x = x.view(-1, BLOCK)
+    top = x.abs().amax(1)
+    held = top >= TINY
+    code = (x * torch.where(held, F8_MAX / top, 0)[:, None]).to(torch.float8_e4m3fn)
+    return code.view(-1), torch.where(held, top / F8_MAX, 0)
+
+
+# ------------------------------------------------------------------------------------------------- one pass
+
+def run(state):
+    case = state["case"]
+    if case["op"] == "adamw":
+        return _adamw_own(state) if own else _adamw_plain(state)
+    if case["op"] == "conv":
+        return _conv_own(state) if own else _conv_plain(state)
+    return _scan_own(state) if own else _scan_plain(state)
+
+
+def _leaves(state, names):
+    return {k: (state[k].detach().requires_grad_(True) if state[k] is not None else None) for k in names}
+
+
+def _conv_own(s):
+    from lqg_amd.belief import ssm
+    case = s["case"]
+    if case["mode"] == "step":
+        return ssm.causal_conv_step(s["x"], s["state"], s["w"], s["bias"], silu=case["silu"]), s["state"]
+    if case["mode"] == "forward":
+        return ssm.causal_conv(s["x"], s["w"], s["bias"], state=s["state"], lengths=s.get("lengths"), silu=case["silu"],
+                               return_state=True)
+    v = _leaves(s, ("x", "w", "bias", "state"))
+    y = ssm.causal_conv(v["x"], v["w"], v["bias"], state=v["state"], lengths=s.get("lengths"), silu=case["silu"])
+    asked = {k: t for k, t in v.items() if t is not None}
+    return y.detach(), dict(zip(asked, torch.autograd.grad(y, list(asked.values()), s["dy"])))
+
+
+def _scan_own(s):
+    from lqg_amd.belief import ssm
+    case = s["case"]
+    if case["mode"] == "step":
+        return ssm.selective_scan_step(s["u"], s["delta"], s["state"], s["A"], s["Bm"], s["Cm"], s["D"], z=s["z"],
+                                       delta_bias=s["delta_bias"], softplus=True), s["state"]
+    if case["mode"] == "forward":
+        return ssm.selective_scan(s["u"], s["delta"], s["A"], s["Bm"], s["Cm"], s["D"], z=s["z"], delta_bias=s["delta_bias"],
+                                  softplus=True, state=s["state"], lengths=s.get("lengths"), return_state=True)
+    v = _leaves(s, ("u", "delta", "A", "Bm", "Cm", "D", "z", "delta_bias", "state"))
+    y = ssm.selective_scan(v["u"], v["delta"], v["A"], v["Bm"], v["Cm"], v["D"], z=v["z"], delta_bias=v["delta_bias"],
+                           softplus=True, state=v["state"], lengths=s.get("lengths"))
+    asked = {k: t for k, t in v.items() if t is not None}
+    return y.detach(), dict(zip(asked, torch.autograd.grad(y, list(asked.values()), s["dy"])))
+
+
+def _adamw_own(s):
+    """(8 bits: what is held is a block's float scale and, as float8 tensors, its elements' values in that scale; both come back.)"""
+    s["opt"].step()
+    held = s["opt"].state_dict()
+    if s["case"]["bits"] == 8:
+        return s["p"].detach(), held["exp_avg"], held["exp_avg_scale"], held["exp_rms"], held["exp_rms_scale"]
+    return s["p"].detach(), held["exp_avg"], held["exp_avg_sq"]
+
+
+# ------------------------------------------------------------------------------------------------- plain forms
+
+def _live(s, B, T):
+    """[B, T, 1] truth values: the steps before each sequence's end."""
+    if s.get("lengths") is None:
+        return torch.ones(1, 1, 1, dtype=torch.bool, device="cuda")
+    return (torch.arange(T, device="cuda") < s["lengths"][:, None])[..., None]
+
+
+def _conv_plain(s):
+    case = s["case"]
+    W, dt = case["W"], TYPES[case["dtype"]]
+    w = s["w"].float()
+    if case["mode"] == "step":
+        rows = torch.cat((s["state"], s["x"][:, None]), 1)
+        v = (rows.float() * w.t()).sum(1)
+        v = v if s["bias"] is None else v + s["bias"].float()
+        s["state"].copy_(rows[:, 1:])
+        return (v * torch.sigmoid(v) if case["silu"] else v).to(dt), s["state"]
+    B, T, D = s["x"].shape
+    live = _live(s, B, T)
+    before = s["state"].float() if s["state"] is not None else torch.zeros(B, W - 1, D, device="cuda")
+    rows = torch.cat((before, torch.where(live, s["x"].float(), 0)), 1)                   # [B, W-1+T, D]
+    v = (rows.unfold(1, W, 1) * w[:, :]).sum(-1)
+    v = v if s["bias"] is None else v + s["bias"].float()
+    sig = torch.sigmoid(v)
+    y = torch.where(live, v * sig if case["silu"] else v, 0).to(dt)
+    if case["mode"] == "forward":
+        if s.get("lengths") is None:
+            return y, rows[:, T:].to(dt)
+        at = s["lengths"].long()[:, None] + torch.arange(W - 1, device="cuda")
+        return y, rows.gather(1, at[..., None].expand(-1, -1, D)).to(dt)
+    e = s["dy"].float() * (sig * (1 + v * (1 - sig)) if case["silu"] else 1)
+    e = torch.where(live, e, 0)
+    ahead = torch.cat((torch.zeros(B, W - 1, D, device="cuda"), e, torch.zeros(B, W - 1, D, device="cuda")), 1)
+    drows = (ahead.unfold(1, W, 1) * w.flip(1)).sum(-1)                                   # [B, W-1+T, D]
+    grads = dict(x=torch.where(live, drows[:, W - 1:], 0).to(dt),
+                 w=(rows.unfold(1, W, 1) * e[..., None]).sum((0, 1), dtype=torch.float64).to(dt))
+    if s["bias"] is not None:
+        grads["bias"] = e.sum((0, 1), dtype=torch.float64).to(dt)
+    if s["state"] is not None:
+        grads["state"] = drows[:, :W - 1].to(dt)
+    return y, grads
+
+
+def _linear_scan(a, b):
+    """h_t = a_t h_{t-1} + b_t from h_{-1} = 0 along axis 1: after each round a and b span twice as many steps."""
+    span, T = 1, a.shape[1]
+    while span < T:
+        b = torch.cat((b[:, :span], b[:, span:] + a[:, span:] * b[:, :-span]), 1)
+        a = torch.cat((a[:, :span], a[:, span:] * a[:, :-span]), 1)
+        span *= 2
+    return b
+
+
+def _softplus(x):
+    return torch.clamp(x, min=0) + torch.log1p(torch.exp(-x.abs()))
+
+
+def _channels(x, D):
+    """[.., G, N] -> [.., D, N]: each group's rows for its channels."""
+    return x.float().repeat_interleave(D // x.shape[-2], -2)
+
+
+def _scan_plain(s):
+    case = s["case"]
+    dt = TYPES[case["dtype"]]
+    u, raw = s["u"].float(), s["delta"].float() + s["delta_bias"]
+    delta, A = _softplus(raw), s["A"]
+    D = A.shape[0]
+    Bm, Cm = _channels(s["Bm"], D), _channels(s["Cm"], D)
+    if case["mode"] == "step":
+        s["state"].copy_(torch.exp(delta[..., None] * A) * s["state"] + (delta * u)[..., None] * Bm)
+        y = (s["state"] * Cm).sum(-1) + s["D"] * u
+        if s["z"] is not None:
+            z = s["z"].float()
+            y = y * z * torch.sigmoid(z)
+        return y.to(dt), s["state"]
+    nB, T, _ = u.shape
+    live = _live(s, nB, T)
+    delta, u = torch.where(live, delta, 0), torch.where(live, u, 0)
+    a = torch.exp(delta[..., None] * A)
+    b = (delta * u)[..., None] * Bm
+    if s["state"] is not None:
+        b[:, 0] += a[:, 0] * s["state"]
+    h = _linear_scan(a, b)
+    y = (h * Cm).sum(-1) + s["D"] * u
+    z = s["z"].float() if s["z"] is not None else None
+    sig = torch.sigmoid(z) if z is not None else None
+    out = torch.where(live, y * z * sig if z is not None else y, 0).to(dt)
+    if case["mode"] == "forward":
+        return out, h[:, -1].contiguous()
+    dy = torch.where(live, s["dy"].float(), 0)
+    grads = dict()
+    if z is not None:
+        grads["z"] = torch.where(live, dy * y * sig * (1 + z * (1 - sig)), 0).to(dt)
+        dy = dy * z * sig
+    # g_t = C_t dy_t + a_{t+1} g_{t+1}
+    later = torch.cat((a[:, 1:], torch.zeros_like(a[:, :1])), 1)
+    g = _linear_scan(later.flip(1), (Cm * dy[..., None]).flip(1)).flip(1)
+    first = s["state"] if s["state"] is not None else torch.zeros_like(h[:, 0])
+    q = g * a * torch.cat((first[:, None], h[:, :-1]), 1)
+    G = s["Bm"].shape[-2]
+    inner = (g * Bm).sum(-1)
+    ddelta = (q * A).sum(-1) + inner * u
+    ddelta = torch.where(live, ddelta * torch.sigmoid(raw), 0)
+    grads.update(u=(inner * delta + dy * s["D"]).to(dt), delta=ddelta.to(dt), A=(q * delta[..., None]).sum((0, 1), dtype=torch.float64).float(),
+                 Bm=(g * (delta * u)[..., None]).unflatten(2, (G, D // G)).sum(3).to(dt),
+                 Cm=(h * dy[..., None]).unflatten(2, (G, D // G)).sum(3).to(dt),
+                 D=(dy * u).sum((0, 1), dtype=torch.float64).float(), delta_bias=ddelta.sum((0, 1), dtype=torch.float64).float())
+    if s["state"] is not None:
+        grads["state"] = a[:, 0] * g[:, 0]
+    return out, grads
+
+
+def _adamw_plain(s):
+    b1, b2 = s["betas"]
+    wide = s["p"].dtype == torch.float64
+    p, g = (s["p"], s["g"]) if wide else (s["p"].float(), s["g"].float())
+    eight = s["case"]["bits"] == 8
+    if eight:
+        m = (s["m"].float().view(-1, BLOCK) * s["m_scale"][:, None]).view(-1)
+        root = (s["r"].float().view(-1, BLOCK) * s["r_scale"][:, None]).view(-1)
+        v = root * root
+    else:
+        m, v = s["m"], s["v"]
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    # (the passes of a state count on from its step, as a program's do)
+    near, far = m / (1 - b1 ** s["step"]), v / (1 - b2 ** s["step"])
+    s["step"] += 1
+    p = p * (1 - s["lr"] * s["weight_decay"]) - s["lr"] * (near / (torch.sqrt(far) + s["eps"]))
+    s["p"].copy_(p)
+    if not eight:
+        s["m"].copy_(m)
+        s["v"].copy_(v)
+        return s["p"], s["m"], s["v"]
+    root = torch.sqrt(v)
+    code, scale = _pack(m)
+    s["m"].copy_(code)
+    s["m_scale"].copy_(scale)
+    code, scale = _pack(root)
+    least = (code.float() == 0) & (root > 0) & (scale > 0).repeat_interleave(BLOCK)
+    s["r"].copy_(torch.where(least, 2.0 ** -9, code.float()).to(torch.float8_e4m3fn))
+    s["r_scale"].copy_(scale)
+    return s["p"], s["m"], s["m_scale"], s["r"], s["r_scale"]
+
+
+# ------------------------------------------------------------------------------------------------- work, and values in 64 bits
+
+def work(case):
+    size = torch.empty((), dtype=TYPES[case["dtype"]]).element_size()
+    if case["op"] == "adamw":
+        n = sum(int(torch.Size(x).numel()) for x in _sizes(case))
+        moment = 8 if case["dtype"] == "f64" else 4
+        held = 2 * moment if case["bits"] == 32 else 2 + 8 / BLOCK
+        return dict(bytes=n * (3 * size + 2 * held), flops=14 * n)
+    B, T, D = case["B"], case["T"], case["D"]
+    if case["op"] == "conv":
+        W = case["W"]
+        passes = {"forward": 2, "step": 2, "train": 4}[case["mode"]]      # train: x, dy in, y, dx out
+        kept = {"forward": 1, "step": 2, "train": 2}[case["mode"]]        # rows of the state read and written
+        flops = B * T * D * (2 * W + 4) * (3 if case["mode"] == "train" else 1)
+        return dict(bytes=size * (passes * B * T * D + kept * B * (W - 1) * D + D * (W + 1)), flops=flops)
+    N, G = case["N"], case["G"]
+    # reads u, delta (and z), writes y; a training pass reads dy and writes their gradients too
+    act = 3 + case["gate"]
+    groups = 2 * B * T * G * N
+    if case["mode"] == "train":
+        act, groups = 2 * (2 + case["gate"]) + 2, 2 * groups
+    kept = (1 + (case["state"] or case["mode"] == "step")) * B * D * N
+    flops = B * T * D * (N * (25 if case["mode"] == "train" else 7) + 10)
+    return dict(bytes=size * (act * B * T * D + groups) + 4 * (kept + D * (N + 2)), flops=flops)
+
+
+def exact(case, seed):
+    """The definitions step by step in float64."""
+    s = prepare(case, seed)
+    up = {k: (x.double() if isinstance(x, torch.Tensor) and x.is_floating_point() else x) for k, x in s.items()}
+    return {"conv": _conv_exact, "scan": _scan_exact, "adamw": _adamw_exact}[case["op"]](case, up)
+
+
+def _ends(case, s):
+    n = s.get("lengths")
+    return [case["T"]] * case["B"] if n is None else n.tolist()
+
+
+def _conv_exact(case, s):
+    W, mode = case["W"], case["mode"]
+    x = s["x"][:, None] if mode == "step" else s["x"]
+    B, T, D = x.shape
+    bias = 0 if s["bias"] is None else s["bias"]
+    past = x.new_zeros(B, W - 1, D) if s["state"] is None else s["state"]
+    y, last = torch.zeros_like(x), torch.empty_like(past)
+    dx, dw, db, dpast = torch.zeros_like(x), torch.zeros_like(s["w"]), x.new_zeros(D), torch.zeros_like(past)
+    for b, n in enumerate(_ends(case, s)):
+        line = torch.cat((past[b], x[b, :n]))
+        v = bias + sum(line[k:k + n] * s["w"][:, k] for k in range(W))
+        y[b, :n] = torch.nn.functional.silu(v) if case["silu"] else v
+        last[b] = line[n:]
+        if mode == "train":
+            e = s["dy"][b, :n]
+            if case["silu"]:
+                sg = 1 / (1 + torch.exp(-v))
+                e = e * (sg + v * sg * (1 - sg))
+            back = torch.zeros_like(line)
+            for k in range(W):
+                back[k:k + n] += e * s["w"][:, k]
+                dw[:, k] += (line[k:k + n] * e).sum(0)
+            db += e.sum(0)
+            dx[b, :n], dpast[b] = back[W - 1:], back[:W - 1]
+    if mode == "step":
+        return y[:, 0], last
+    if mode == "forward":
+        return y, last
+    grads = dict(x=dx, w=dw)
+    if s["bias"] is not None:
+        grads["bias"] = db
+    if s["state"] is not None:
+        grads["state"] = dpast
+    return y, grads
+
+
+def _scan_exact(case, s):
+    mode, G, N = case["mode"], case["G"], case["N"]
+    seq = lambda t: None if t is None else (t[:, None] if mode == "step" else t)  # noqa: E731
+    u, raw, z, Bg, Cg = seq(s["u"]), seq(s["delta"]) + s["delta_bias"], seq(s["z"]), seq(s["Bm"]), seq(s["Cm"])
+    B, T, D = u.shape
+    group = torch.arange(D, device=u.device) // (D // G)
+    dl = torch.logaddexp(raw, torch.zeros_like(raw))
+    live = torch.arange(T, device=u.device)[None] < torch.tensor(_ends(case, s), device=u.device)[:, None]
+    h = u.new_zeros(B, D, N) if s["state"] is None else s["state"]
+    gate = torch.ones_like(u) if z is None else torch.nn.functional.silu(z)
+    y, kept = torch.zeros_like(u), []
+    for t in range(T):
+        on = live[:, t, None]
+        kept.append(h) if mode == "train" else None
+        new = torch.exp(dl[:, t, :, None] * s["A"]) * h + (dl[:, t] * u[:, t])[..., None] * Bg[:, t, group]
+        h = torch.where(on[..., None], new, h)
+        y[:, t] = torch.where(on, (h * Cg[:, t, group]).sum(-1) + s["D"] * u[:, t], 0)
+    out = y * gate
+    if mode == "step":
+        return out[:, 0], h
+    if mode == "forward":
+        return out, h
+    dy = torch.where(live[..., None], s["dy"], 0)
+    du, ddl, dB, dC = torch.zeros_like(u), torch.zeros_like(u), torch.zeros_like(Bg), torch.zeros_like(Cg)
+    dA, lam = torch.zeros_like(s["A"]), u.new_zeros(B, D, N)
+    core = dy * gate
+    for t in reversed(range(T)):
+        on = live[:, t, None]
+        a = torch.exp(dl[:, t, :, None] * s["A"])
+        now = torch.where(on[..., None], a * kept[t] + (dl[:, t] * u[:, t])[..., None] * Bg[:, t, group], 0)
+        lam = lam + core[:, t, :, None] * Cg[:, t, group]
+        dC[:, t] = (now * core[:, t, :, None]).view(B, G, D // G, N).sum(2)
+        hold = torch.where(on[..., None], lam, 0)
+        dB[:, t] = (hold * (dl[:, t] * u[:, t])[..., None]).view(B, G, D // G, N).sum(2)
+        through = (hold * Bg[:, t, group]).sum(-1)
+        slope = hold * a * kept[t]
+        dA += (slope * dl[:, t, :, None]).sum(0)
+        du[:, t] = through * dl[:, t] + core[:, t] * s["D"]
+        ddl[:, t] = (slope * s["A"]).sum(-1) + through * u[:, t]
+        lam = torch.where(on[..., None], lam * a, lam)
+    ddl = ddl / (1 + torch.exp(-raw))
+    grads = dict(u=du, delta=ddl, A=dA, Bm=dB, Cm=dC, D=(core * u).sum((0, 1)), delta_bias=ddl.sum((0, 1)))
+    if z is not None:
+        sg = 1 / (1 + torch.exp(-z))
+        grads["z"] = dy * y * (sg + z * sg * (1 - sg))
+    if s["state"] is not None:
+        grads["state"] = lam
+    return out, grads
+
+
+def _adamw_exact(case, s):
+    b1, b2 = s["betas"]
+    eight = case["bits"] == 8
+    if eight:
+        m = s["m"] * s["m_scale"].repeat_interleave(BLOCK)
+        v = (s["r"] * s["r_scale"].repeat_interleave(BLOCK)).square()
+    else:
+        m, v = s["m"], s["v"]
+    m = m + (1 - b1) * (s["g"] - m)
+    v = v + (1 - b2) * (s["g"].square() - v)
+    p = s["p"] - s["lr"] * s["weight_decay"] * s["p"]
+    p = p - s["lr"] * (m / (1 - b1 ** s["step"])) / ((v / (1 - b2 ** s["step"])).sqrt() + s["eps"])
+    if not eight:
+        return p, m, v
+    held = []
+    for x in (m, v.sqrt()):
+        x = x.view(-1, BLOCK)
+        top = x.abs().amax(1, keepdim=True)
+        unit = torch.where(top > 0, top / F8_MAX, 1)
+        r = (x / unit).view(-1)
+        # three bits after the leading one, and steps of 2^-9 below 2^-6
+        step = torch.exp2(torch.floor(torch.log2(r.abs().clamp(min=2.0 ** -6))) - 3)
+        held += [torch.clamp(torch.round(r / step) * step, -F8_MAX, F8_MAX), torch.where(top > 0, top / F8_MAX, 0)[:, 0]]
+    held[2] = torch.where((held[2] == 0) & (v > 0), 2.0 ** -9, held[2])
+    return p, *held
