@@ -1,0 +1,114 @@
+/*
+ * lqg_learn.h — C ABI of the learned-filter operators and of the AdamW step in liblqg_hip.so (MI355X, gfx950).
+ *
+ * Conventions as in lqg_hip.h: plain C, the caller owns all device memory, calls are stream-ordered and asynchronous, nothing is
+ * allocated, retained or synchronised; 0 on success, < 0 invalid argument (nothing launched), > 0 a hipError_t of the launch.
+ * Sequences are [batch][time][channel] with a channel stride of 1 and any batch / time strides (in elements).
+ */
+#ifndef LQG_LEARN_H
+#define LQG_LEARN_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* element types */
+enum { LQG_T_F32 = 0, LQG_T_BF16 = 1, LQG_T_F16 = 2, LQG_T_F64 = 3 };
+
+typedef struct lqg_seq { const void* ptr; int64_t sb, st, sg; } lqg_seq;      /* sg: stride of the group axis (scan's B and C) */
+typedef struct lqg_param { const void* ptr; int32_t type; int32_t pad; } lqg_param;  /* contiguous, its own type; ptr NULL: absent */
+
+/*
+ * Short causal convolution over each channel:  y[b,t,d] = act(bias[d] + sum_k w[d,k] xs[b, t-(W-1)+k, d]),  1 <= W <= 8,
+ * xs = `state` ([B][W-1][D] contiguous, oldest first; NULL: zeros) followed by x.  Steps t >= lengths[b] (NULL: T; values are
+ * clamped to 0..T) are padding: y is 0 there, x is not used.  state_out [B][W-1][D] (or NULL): the rows that the next call needs.
+ */
+typedef struct lqg_conv {
+  int32_t type, W, silu, pad;
+  int64_t B, T, D;
+  lqg_seq x, y;
+  lqg_param w, bias;
+  const void* state;
+  void* state_out;
+  const int32_t* lengths;
+} lqg_conv;
+int lqg_causal_conv(const lqg_conv* p, void* stream);
+
+/* Gradients of lqg_causal_conv: dy -> dx [B][T][D] contiguous, dstate [B][W-1][D] or NULL, dw [D][W] and dbias [D] (types of w and
+ * bias; either may be NULL).  dstate_out: gradient of state_out or NULL.  Workspace: lqg_causal_conv_grad_workspace bytes. */
+size_t lqg_causal_conv_grad_workspace(const lqg_conv* p);
+int lqg_causal_conv_grad(const lqg_conv* p, lqg_seq dy, const void* dstate_out, void* dx, void* dstate, void* dw, void* dbias,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step: x, y are [B][D] (T = 1; strides sb), `state` is moved on in place (state_out is ignored). */
+int lqg_causal_conv_step(const lqg_conv* p, void* stream);
+
+/*
+ * Selective state-space scan, one diagonal system of N states per channel, 1 <= N <= 64:
+ *   dl = delta + delta_bias, through softplus if asked;   h_t = exp(dl_t A) h_{t-1} + dl_t B_t u_t;
+ *   y_t = (sum_n C_t h_t + D u_t) [* silu(z_t)]
+ * A [D][N]; B, C [batch][time][G][N], group g serves channels g D/G ..; state [B][D][N] float or NULL (zeros).
+ * Padding as above: y is 0 and h stays.  state_out [B][D][N] float or NULL.
+ * checkpoints (or NULL): lqg_scan_checkpoint_bytes of memory that lqg_selective_scan_grad reads.
+ */
+typedef struct lqg_selscan {
+  int32_t type, softplus;
+  int64_t B, T, D, N, G;
+  lqg_seq u, delta, z, Bm, Cm, y;      /* z.ptr NULL: no gate */
+  lqg_param A, Dskip, delta_bias;
+  const float* state;
+  float* state_out;
+  const int32_t* lengths;
+  void* checkpoints;
+  int32_t chunks, pad;                 /* pieces the time axis is cut into: 0 = the rule, else 1 .. 64 */
+} lqg_selscan;
+size_t lqg_selscan_workspace(const lqg_selscan* p);
+size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p);
+int lqg_selective_scan(const lqg_selscan* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients (all contiguous; state's may be NULL): du, ddelta, dz [B][T][D], dBm, dCm [B][T][G][N] in the sequences' type;
+ * dA [D][N], dD [D], ddelta_bias [D] in the parameters' types; dstate [B][D][N] float.  dstate_out: gradient of state_out or NULL. */
+typedef struct lqg_selscan_bars {
+  lqg_seq dy;
+  const float* dstate_out;
+  void *du, *ddelta, *dz, *dBm, *dCm, *dA, *dD, *ddelta_bias;
+  float* dstate;
+} lqg_selscan_bars;
+size_t lqg_selscan_grad_workspace(const lqg_selscan* p);
+int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_bars* g, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step: T = 1, `state` ([B][D][N] float) is moved on in place; sequences use their sb (and sg) strides. */
+int lqg_selective_scan_step(const lqg_selscan* p, float* state, void* stream);
+
+/*
+ * AdamW over many tensors.  Tensor i has numel[i] contiguous elements of `type`, its moments start at element offset[i] (a multiple
+ * of 256) of the moment arrays.  One step:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g g;  p = p (1 - lr wd) - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
+ * every operation rounded by itself, in float (LQG_T_F64: in double).
+ * bits 32: exp_avg, exp_avg_sq are arrays of float (LQG_T_F64: double).  bits 8: exp_avg and exp_avg_sq hold e4m3 values of m and of
+ * sqrt(v), in units of a float scale for each 256 elements (exp_avg_scale, exp_avg_sq_scale): scale = largest magnitude / 448 (0,
+ * and values 0, below 1e-30); a root that is not 0 is held as 2^-9 units at least.
+ * step_state NULL: t = step.  Else it points to three doubles {t, 1/(1-b1^t), 1/(1-b2^t)}, which lqg_adamw_advance moves on.
+ */
+typedef struct lqg_adamw {
+  int32_t type, bits, count, pad;
+  void* const* params;                 /* host arrays of `count` device pointers / sizes */
+  const void* const* grads;
+  const int64_t* numel;
+  const int64_t* offset;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const double* step_state;
+} lqg_adamw;
+int lqg_adamw_step(const lqg_adamw* p, void* stream);
+int lqg_adamw_advance(double* step_state, double beta1, double beta2, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -1,1 +1,1 @@
-from lqg_amd.belief import kf  # noqa: F401
+from lqg_amd.belief import kf, ssm  # noqa: F401

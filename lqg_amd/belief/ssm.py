@@ -1,0 +1,342 @@
+"""lqg_amd.belief.ssm — a LEARNED filter beside the optimal one (belief.kf): a selective state-space scan and the short causal
+convolution in front of it, forward and backward over whole trials, and step by step.
+
+Where the Kalman filter's belief follows x^_{t+1} = (A - B L - K F) x^_t + K y_t with gains computed from a known model, here the state
+of every channel d is a diagonal linear system whose step size and input / output maps are functions of the data, handed in per step:
+
+    h_t = exp(delta_t A) h_{t-1} + delta_t B_t u_t,      y_t = C_t . h_t + D u_t          [* silu(z_t)]
+
+Axes are those of the framework's trajectories: [trial, time, channel].  Sequences are float32, bfloat16 or float16, all of one type;
+states of the scan, and all arithmetic, are float32.  Any trial / time strides are taken as they are (slices of one projection's
+output); a channel stride other than 1 costs a copy.  `lengths` [trial] (int32 or int64, on the device) marks padded trials: outputs
+and gradients at and behind a trial's length are 0, its state is that after its last step, and what the padding holds — NaN included —
+is never used.  Lengths outside 0..T count as the nearer end.  Computation is on the GPU only; no call synchronises."""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from lqg_amd import _abi, _learn, options
+from lqg_amd._abi import LqgHipError
+
+MAX_WIDTH, MAX_STATES = 8, 64
+
+
+def _need(ok, what):
+    if not ok:
+        raise LqgHipError(what)
+
+
+def _sequence(t, name, dims, like=None):
+    _need(isinstance(t, torch.Tensor) and t.dim() == dims, f"{name}: a tensor of {dims} dimensions is needed, got "
+          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    _need(t.dtype in _learn.SEQ_TYPES, f"{name}: float32, bfloat16 or float16 is needed, got {t.dtype}")
+    if like is not None:
+        _need(t.dtype == like.dtype and t.device == like.device,
+              f"{name}: {t.dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _on_gpu(t):
+    _need(t.device.type == "cuda", f"lqg_amd computes on MI355X only: tensors are on '{t.device}'; there is no CPU fallback")
+
+
+def _parameter(t, name, shape, like):
+    if t is None:
+        return None
+    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == shape, f"{name}: shape {shape} is needed, got "
+          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    _need(t.dtype in _learn.SEQ_TYPES and t.device == like.device,
+          f"{name}: float32, bfloat16 or float16 on {like.device} is needed, got {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
+def _state(t, name, shape, dtype, like, in_place=False):
+    if t is None:
+        return None
+    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype and t.device == like.device,
+          f"{name}: {dtype} {shape} on {like.device} is needed, got "
+          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if in_place:
+        _need(t.is_contiguous(), f"{name}: a contiguous tensor is needed, since the step moves it on in place")
+        return t
+    return t.contiguous()
+
+
+def _lengths(t, B, like):
+    if t is None:
+        return None
+    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == (B,) and t.dtype in (torch.int32, torch.int64) and t.device == like.device,
+          f"lengths: int32 or int64 [{B}] on {like.device} is needed")
+    # (clamped before the narrowing, which would wrap)
+    return (t.clamp(0, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t).contiguous()
+
+
+def _no_gradient(what, instead, *tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise LqgHipError(f"{what} has no gradient (its state is moved on in place): call it under torch.no_grad(), or {instead}")
+
+
+def _separate(state, name, *others):
+    """An in-place state must not be read through another argument while it is written."""
+    if state is None or not state.numel():
+        return
+    lo, hi = state.data_ptr(), state.data_ptr() + state.numel() * state.element_size()
+    for t in others:
+        if t is not None and t.numel():
+            a = t.data_ptr()
+            b = a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            _need(b <= lo or a >= hi, f"{name}: it shares memory with another argument")
+
+
+# ------------------------------------------------------------------------------------------------ short causal convolution
+
+def _conv_args(x, w, bias, silu):
+    p = _learn.Conv()
+    p.type, p.W, p.silu = _learn.TYPES[x.dtype], w.shape[1], int(bool(silu))
+    p.w, p.bias = _learn.param(w), _learn.param(bias)
+    return p
+
+
+class _Conv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, state, lengths, silu, want_state):
+        B, T, D = x.shape
+        W = w.shape[1]
+        y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+        last = torch.empty((B, W - 1, D), dtype=x.dtype, device=x.device) if want_state else None
+        lib = _learn.load()
+        p = _conv_args(x, w, bias, silu)
+        p.B, p.T, p.D, p.x, p.y = B, T, D, _learn.seq(x), _learn.seq(y)
+        p.state, p.state_out, p.lengths = _learn.ptr(state), _learn.ptr(last), _learn.ptr(lengths)
+        with _learn.on_device(x.device):
+            _abi.check(lib.lqg_causal_conv(C.byref(p), _learn.stream(x.device)), "lqg_causal_conv")
+        ctx.save_for_backward(x, w, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, w, bias, state, lengths = ctx.saved_tensors
+        B, T, D = x.shape
+        W = w.shape[1]
+        if dy is None and dlast is None:
+            return (None,) * 7
+        dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else dy
+        dy = dy if dy.stride(-1) == 1 or D == 1 else dy.contiguous()
+        dlast = None if dlast is None else dlast.contiguous()
+        dev = x.device
+        dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        dw, dbias = torch.empty_like(w), None if bias is None else torch.empty_like(bias)
+        dstate = None if state is None else torch.empty_like(state)
+        lib = _learn.load()
+        p = _conv_args(x, w, bias, ctx.silu)
+        p.B, p.T, p.D, p.x = B, T, D, _learn.seq(x)
+        p.state, p.lengths = _learn.ptr(state), _learn.ptr(lengths)
+        with _learn.on_device(dev):
+            n = lib.lqg_causal_conv_grad_workspace(C.byref(p))
+            ws = _learn.scratch(n, dev)
+            _abi.check(lib.lqg_causal_conv_grad(C.byref(p), _learn.seq(dy), _learn.ptr(dlast), _learn.ptr(dx), _learn.ptr(dstate),
+                                                _learn.ptr(dw), _learn.ptr(dbias), _learn.ptr(ws), n, _learn.stream(dev)),
+                       "lqg_causal_conv_grad")
+        return dx, dw, dbias, dstate, None, None, None
+
+
+def _conv_check(x, weight, bias, dims):
+    x = _sequence(x, "x", dims)
+    D = x.shape[-1]
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] == D and 1 <= weight.shape[1] <= MAX_WIDTH,
+          f"weight: shape ({D}, 1 .. {MAX_WIDTH}) is needed")
+    return x, _parameter(weight, "weight", tuple(weight.shape), x), _parameter(bias, "bias", (D,), x)
+
+
+def causal_conv(x, weight, bias=None, *, state=None, lengths=None, silu=False, return_state=False):
+    """y[b, t, d] = act(bias[d] + sum_k weight[d, k] x[b, t - (W-1) + k, d]): a causal filter of W = 1 .. 8 taps over each channel of
+    x [trial, time, channel]; act is silu or nothing.
+
+    state [trial, W-1, channel] (type of x): the inputs before the first step, oldest first; None: zeros.  return_state: also the
+    inputs that a following call, or `causal_conv_step`, continues from.  Differentiable in x, weight, bias and state (once)."""
+    x, w, bias = _conv_check(x, weight, bias, 3)
+    B, T, D = x.shape
+    W = w.shape[1]
+    state = _state(state, "state", (B, W - 1, D), x.dtype, x)
+    lengths = _lengths(lengths, B, x)
+    _on_gpu(x)
+    if not x.numel():
+        return _empty_conv(x, w, bias, state, return_state)
+    y, last = _Conv.apply(x, w, bias, state, lengths, bool(silu), bool(return_state))
+    return (y, last) if return_state else y
+
+
+def _zero_like_sum(*tensors):
+    """0 that depends on the given tensors: gradients of an empty call are zeros rather than absent."""
+    return sum(t.sum() * 0 if t.numel() else t.sum() for t in tensors if t is not None and t.requires_grad)
+
+
+def _empty_conv(x, w, bias, state, return_state):
+    W = w.shape[1]
+    y = x * 1
+    if torch.is_grad_enabled():
+        y = y + _zero_like_sum(w, bias, state)
+    last = x.new_zeros(x.shape[0], W - 1, x.shape[2]) if state is None else state.clone()
+    return (y, last) if return_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, *, silu=False):
+    """One step of `causal_conv`: x [trial, channel] -> y [trial, channel]; state [trial, W-1, channel] (contiguous, type of x) is moved
+    on IN PLACE.  No gradient."""
+    _no_gradient("causal_conv_step", "use causal_conv", x, state, weight, bias)
+    x, w, bias = _conv_check(x, weight, bias, 2)
+    B, D = x.shape
+    W = w.shape[1]
+    _need(state is not None, f"state: {(B, W - 1, D)} is needed")
+    state = _state(state, "state", (B, W - 1, D), x.dtype, x, in_place=True)
+    _separate(state, "state", x, w, bias)
+    _on_gpu(x)
+    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    if not y.numel():
+        return y
+    p = _conv_args(x, w, bias, silu)
+    p.B, p.T, p.D, p.x, p.y, p.state = B, 1, D, _learn.row(x), _learn.row(y), _learn.ptr(state)
+    with _learn.on_device(x.device):
+        _abi.check(_learn.load().lqg_causal_conv_step(C.byref(p), _learn.stream(x.device)), "lqg_causal_conv_step")
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+# ------------------------------------------------------------------------------------------------ selective scan
+
+def _scan_args(u, A, G, D, delta_bias, softplus):
+    p = _learn.SelScan()
+    p.type, p.softplus = _learn.TYPES[u.dtype], int(softplus)
+    p.D, p.N, p.G, p.chunks = u.shape[-1], A.shape[1], G, options.get("SELSCAN_CHUNKS")
+    p.A, p.Dskip, p.delta_bias = _learn.param(A), _learn.param(D), _learn.param(delta_bias)
+    return p
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
+        nB, T, nD = u.shape
+        N, G, dev = A.shape[1], Bm.shape[2], u.device
+        y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
+        last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
+        lib = _learn.load()
+        p = _scan_args(u, A, G, D, delta_bias, softplus)
+        p.B, p.T = nB, T
+        p.u, p.delta, p.z, p.Bm, p.Cm, p.y = (_learn.seq(t) for t in (u, delta, z, Bm, Cm, y))
+        p.state, p.state_out, p.lengths = _learn.ptr(state), _learn.ptr(last), _learn.ptr(lengths)
+        with _learn.on_device(dev):
+            ck = _learn.scratch(lib.lqg_selscan_checkpoint_bytes(C.byref(p)), dev) if keep else None
+            p.checkpoints = _learn.ptr(ck)
+            n = lib.lqg_selscan_workspace(C.byref(p))
+            ws = _learn.scratch(n, dev)
+            _abi.check(lib.lqg_selective_scan(C.byref(p), _learn.ptr(ws), n, _learn.stream(dev)), "lqg_selective_scan")
+        ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck = ctx.saved_tensors
+        if dy is None and dlast is None:
+            return (None,) * 13
+        nB, T, nD = u.shape
+        N, G, dev = A.shape[1], Bm.shape[2], u.device
+        dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
+        dy = dy if dy.stride(-1) == 1 or nD == 1 else dy.contiguous()
+        dlast = None if dlast is None else dlast.contiguous()
+        new = lambda *shape: torch.empty(shape, dtype=u.dtype, device=dev)  # noqa: E731
+        du, ddelta, dz = new(nB, T, nD), new(nB, T, nD), None if z is None else new(nB, T, nD)
+        dBm, dCm, dA = new(nB, T, G, N), new(nB, T, G, N), torch.empty_like(A)
+        dD, dbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
+        dstate = None if state is None else torch.empty_like(state)
+        lib = _learn.load()
+        p = _scan_args(u, A, G, D, delta_bias, ctx.softplus)
+        p.B, p.T = nB, T
+        p.u, p.delta, p.z, p.Bm, p.Cm = (_learn.seq(t) for t in (u, delta, z, Bm, Cm))
+        p.lengths, p.checkpoints = _learn.ptr(lengths), _learn.ptr(ck)
+        g = _learn.SelScanBars()
+        g.dy, g.dstate_out, g.dstate = _learn.seq(dy), _learn.ptr(dlast), _learn.ptr(dstate)
+        g.du, g.ddelta, g.dz, g.dBm, g.dCm = (_learn.ptr(t) for t in (du, ddelta, dz, dBm, dCm))
+        g.dA, g.dD, g.ddelta_bias = _learn.ptr(dA), _learn.ptr(dD), _learn.ptr(dbias)
+        with _learn.on_device(dev):
+            n = lib.lqg_selscan_grad_workspace(C.byref(p))
+            ws = _learn.scratch(n, dev)
+            _abi.check(lib.lqg_selective_scan_grad(C.byref(p), C.byref(g), _learn.ptr(ws), n, _learn.stream(dev)),
+                       "lqg_selective_scan_grad")
+        return du, ddelta, dA, dBm, dCm, dD, dz, dbias, dstate, None, None, None, None
+
+
+def _scan_check(u, delta, A, B, C_, D, z, delta_bias, dims):
+    u = _sequence(u, "u", dims)
+    nD = u.shape[-1]
+    delta = _sequence(delta, "delta", dims, u)
+    z = None if z is None else _sequence(z, "z", dims, u)
+    for t, name in ((delta, "delta"), (z, "z")):
+        _need(t is None or t.shape == u.shape, f"{name}: the shape of u, {tuple(u.shape)}, is needed")
+    _need(isinstance(A, torch.Tensor) and A.dim() == 2 and A.shape[0] == nD and 1 <= A.shape[1] <= MAX_STATES,
+          f"A: shape ({nD}, 1 .. {MAX_STATES}) is needed")
+    A = _parameter(A, "A", tuple(A.shape), u)
+    N = A.shape[1]
+    maps = []
+    for t, name in ((B, "B"), (C_, "C")):
+        if isinstance(t, torch.Tensor) and t.dim() == dims:
+            t = t.unsqueeze(-2)                    # one group
+        t = _sequence(t, name, dims + 1, u)
+        _need(t.shape[:-2] == u.shape[:-1] and t.shape[-1] == N and t.shape[-2] >= 1 and nD % t.shape[-2] == 0,
+              f"{name}: shape {tuple(u.shape[:-1])} + (groups that divide {nD}, {N}) is needed, got {tuple(t.shape)}")
+        maps.append(t)
+    _need(maps[0].shape == maps[1].shape, "B and C: the same groups are needed")
+    return u, delta, A, *maps, _parameter(D, "D", (nD,), u), z, _parameter(delta_bias, "delta_bias", (nD,), u)
+
+
+def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus=False, state=None, lengths=None,
+                   return_state=False):
+    """y_t = C_t . h_t + D u_t, h_t = exp(dl_t A) h_{t-1} + dl_t B_t u_t with dl = delta + delta_bias (through softplus if asked); with
+    z, y_t * silu(z_t).
+
+    u, delta, z [trial, time, channel]; A [channel, N], N = 1 .. 64; B, C [trial, time, N] or [trial, time, group, N], each group
+    serving channels / groups neighbouring channels; D, delta_bias [channel].  state [trial, channel, N] float32: h before the first
+    step (None: zeros); return_state: also h after the last.  Differentiable in every tensor but lengths (once); a call that needs no
+    gradient keeps nothing, one that does keeps a state for every 16 steps (8 for N > 32)."""
+    u, delta, A, Bm, Cm, D, z, delta_bias = _scan_check(u, delta, A, B, C, D, z, delta_bias, 3)
+    nB, T, nD = u.shape
+    state = _state(state, "state", (nB, nD, A.shape[1]), torch.float32, u)
+    lengths = _lengths(lengths, nB, u)
+    _on_gpu(u)
+    inputs = (u, delta, A, Bm, Cm, D, z, delta_bias, state)
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    if not u.numel():
+        y = u * 1 + _zero_like_sum(*inputs[1:]) if keep else u.clone()
+        last = torch.zeros((nB, nD, A.shape[1]), dtype=torch.float32, device=u.device) if state is None else state.clone()
+        return (y, last) if return_state else y
+    y, last = _Scan.apply(*inputs, lengths, bool(softplus), bool(return_state), keep)
+    return (y, last) if return_state else y
+
+
+def selective_scan_step(u, delta, state, A, B, C, D=None, *, z=None, delta_bias=None, softplus=False):
+    """One step of `selective_scan`: u, delta, z [trial, channel], B, C [trial, N] or [trial, group, N] -> y [trial, channel]; state
+    [trial, channel, N] (float32, contiguous) is moved on IN PLACE.  No gradient."""
+    _no_gradient("selective_scan_step", "use selective_scan", u, delta, state, A, B, C, D, z, delta_bias)
+    u, delta, A, Bm, Cm, D, z, delta_bias = _scan_check(u, delta, A, B, C, D, z, delta_bias, 2)
+    nB, nD = u.shape
+    _need(state is not None, f"state: {(nB, nD, A.shape[1])} is needed")
+    state = _state(state, "state", (nB, nD, A.shape[1]), torch.float32, u, in_place=True)
+    _separate(state, "state", u, delta, A, Bm, Cm, D, z, delta_bias)
+    _on_gpu(u)
+    y = torch.empty((nB, nD), dtype=u.dtype, device=u.device)
+    if not y.numel():
+        return y
+    p = _scan_args(u, A, Bm.shape[1], D, delta_bias, softplus)
+    p.B, p.T = nB, 1
+    p.u, p.delta, p.z, p.Bm, p.Cm, p.y = (_learn.row(t) for t in (u, delta, z, Bm, Cm, y))
+    lib = _learn.load()
+    with _learn.on_device(u.device):
+        _abi.check(lib.lqg_selective_scan_step(p, state.data_ptr(), _learn.stream(u.device)), "lqg_selective_scan_step")
+    torch.autograd.graph.increment_version(state)
+    return y

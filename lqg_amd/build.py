@@ -27,12 +27,20 @@ HEADERS = ["lqg_small.hpp", "lqg_rng.hpp", "lqg_kernels.hpp", "lqg_launch.hpp", 
 COOP_HEADERS = ["lqg_small.hpp", "lqg_rng.hpp", "lqg_kernels.hpp", "lqg_launch.hpp", "lqg_trial_chunk.hpp", "lqg_coop.hpp", "lqg_coop_launch.hpp",
                 "../../include/lqg_hip.h"]
 SCAN_HEADERS = COOP_HEADERS + ["lqg_scan.hpp"]
+LEARN_HEADERS = ["lqg_learn.hpp", "lqg_selscan.hpp", "../../include/lqg_hip.h", "../../include/lqg_learn.h"]
+# the learned-filter operators and the AdamW step (include/lqg_learn.h), with the flags each is compiled with on top of FLAGS.  No
+# packed fp32 instructions; the AdamW step without contraction, so that its bits are those of the formula operation by operation.
+_NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+LEARN = {"conv.o": ("lqg_conv.hip", _NO_PACKED), "adamw.o": ("lqg_adamw.hip", _NO_PACKED + ["-ffp-contract=off"]),
+         "selscan.o": ("lqg_selscan.hip", _NO_PACKED),
+         **{f"selscan_{t}.o": ("lqg_selscan.hip", _NO_PACKED + [f"-DLQG_SELSCAN_TYPE={t}"]) for t in ("float", "bf16", "f16")}}
 ADJ_HEADERS = ["lqg_small.hpp", "lqg_adjoint.hpp", "lqg_adjoint_launch.hpp", "../../include/lqg_hip.h"]
 # headers each source depends on (an adjoint-kernel edit must not recompile the forward kernels and vice versa)
 DEPS = {"lqg_inst.hip": HEADERS, "lqg_adjoint_inst.hip": ADJ_HEADERS, "lqg_coop_inst.hip": COOP_HEADERS,
         "lqg_scan_inst.hip": SCAN_HEADERS, "lqg_setup.hip": ["../../include/lqg_hip.h"],
         "lqg_coop_adjoint.hip": ["lqg_coop_launch.hpp", "../../include/lqg_hip.h"],
-        "lqg_abi.hip": sorted(set(HEADERS + ADJ_HEADERS + ["lqg_coop_launch.hpp"]))}
+        "lqg_abi.hip": sorted(set(HEADERS + ADJ_HEADERS + ["lqg_coop_launch.hpp"])),
+        **{src: LEARN_HEADERS for src, _ in LEARN.values()}}
 FAMILIES = ("FORWARD", "RICCATI", "KALMAN", "TRIAL", "SIM", "ADJOINT")
 ADJOINT_MAX_JOINT = 12          # on-demand libraries get the gradient sweep up to x + b = 12 (33 s per dtype at 12; minutes beyond)
 
@@ -52,6 +60,8 @@ def jobs(lists=None, extra_defs=()):
     js = [("abi.o", "lqg_abi.hip", extra_defs), ("coop.o", "lqg_coop_inst.hip", extra_defs),
           ("scan.o", "lqg_scan_inst.hip", extra_defs), ("setup.o", "lqg_setup.hip", extra_defs),
           ("coopadj.o", "lqg_coop_adjoint.hip", extra_defs)]
+    if lists is None:                # (auxiliary per-shape libraries do without: nothing in them depends on a model's shape)
+        js += [(obj, src, flags + extra_defs) for obj, (src, flags) in LEARN.items()]
     for fam, tuples in (lists or dims_lists()).items():
         for t in tuples:
             for dt in ("F32", "F64"):
@@ -80,10 +90,10 @@ STAMP = LIB + ".stamp"
 def source_hash():
     """Content hash of every source that goes into the library (+ compile flags): mtimes do not survive the
     snapshot to the GPU box, the hash does."""
-    h = hashlib.sha256(" ".join(FLAGS).encode())
+    h = hashlib.sha256(" ".join(FLAGS + [x for _, v in LEARN.values() for x in v]).encode())
     for f in sorted(set(HEADERS + ADJ_HEADERS + SCAN_HEADERS + ["lqg_abi.hip", "lqg_inst.hip", "lqg_adjoint_inst.hip",
                                                                 "lqg_coop_inst.hip", "lqg_scan_inst.hip", "lqg_setup.hip",
-                                                                "lqg_coop_adjoint.hip"])):
+                                                                "lqg_coop_adjoint.hip"] + LEARN_HEADERS + [src for src, _ in LEARN.values()])):
         h.update(open(os.path.join(CSRC, f), "rb").read())
     return h.hexdigest()
 

@@ -1,0 +1,92 @@
+// lqg_learn.hpp — what the learned-filter operators (lqg_conv.hip, lqg_selscan.hip) and the AdamW step (lqg_adamw.hip) share:
+// element types, elementary functions, broadcasts and reductions inside a wave, and the sum over rows that ends their gradients.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/lqg_hip.h"
+#include "../../include/lqg_learn.h"
+
+namespace lqg {
+namespace learn {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// One rounding to the stored type (round to nearest even); arithmetic is in float throughout.
+template <class T> __device__ inline float up(T v) { return (float)v; }
+template <class T> __device__ inline T down(float v) { return (T)v; }
+
+__device__ inline float load_param(const lqg_param& p, long i) {
+  if (p.type == LQG_T_F32) return static_cast<const float*>(p.ptr)[i];
+  if (p.type == LQG_T_BF16) return (float)static_cast<const bf16*>(p.ptr)[i];
+  return (float)static_cast<const f16*>(p.ptr)[i];
+}
+
+__device__ inline void store_as(void* p, int type, long i, float v) {
+  if (type == LQG_T_F32) static_cast<float*>(p)[i] = v;
+  else if (type == LQG_T_BF16) static_cast<bf16*>(p)[i] = (bf16)v;
+  else static_cast<f16*>(p)[i] = (f16)v;
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// 2^x by the hardware's exponential (1 ulp; results below 2^-126 are 0)
+__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// 1 / (1 + e^-x)
+__device__ inline float sigmoid(float x) { return rcp_hw(1.0f + exp2_hw(-LOG2E * x)); }
+
+// softplus(x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1].  The logarithm as 2 atanh(s), s = e / (2 + e) <= 1/3: its series in s^2
+// keeps the RELATIVE error at a few ulp for small e too (time constants of 1000 steps are x = -7), where log of the rounded 1 + e
+// keeps only the absolute one.  First dropped term: s^18 / 19 <= 1.4e-10 of the sum.
+__device__ inline float softplus(float x) {
+  const float e = exp2_hw(-LOG2E * fabsf(x));
+  const float s = e * rcp_hw(2.0f + e), q = s * s;
+  float p = 1.0f / 17.0f;
+  p = fmaf(p, q, 1.0f / 15.0f);
+  p = fmaf(p, q, 1.0f / 13.0f);
+  p = fmaf(p, q, 1.0f / 11.0f);
+  p = fmaf(p, q, 1.0f / 9.0f);
+  p = fmaf(p, q, 1.0f / 7.0f);
+  p = fmaf(p, q, 1.0f / 5.0f);
+  p = fmaf(p, q, 1.0f / 3.0f);
+  const float l = 2.0f * fmaf(s * q, p, s);
+  return x != x ? x : fmaxf(x, 0.0f) + l;       // (fmaxf drops a NaN)
+}
+
+// lane K of each row of 16 lanes, in all lanes of that row: a modifier of the consuming instruction's operand, no instruction of its own
+template <int K>
+__device__ inline float row_bcast(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + K, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ inline float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_ROR8 = 0x128;
+
+// Workgroups of a one-dimensional grid, checked against the 2^32 threads a launch may have.
+inline bool grid_fits(long groups, int threads) { return groups > 0 && groups <= 0x7fffffffL && groups * (long)threads < (1L << 32); }
+
+// out[o][c] = sum over the rows r = o, o + outs, .. of in[r][c], in double, in a fixed order; outs = 1: stored as `type` to final[c's
+// place].  Two launches (rows -> 64 -> 1) when rows are many.  Defined in lqg_conv.hip.
+struct RowSum {
+  const float* in;         // [rows][cols]
+  long rows, cols;
+  float* mid;              // [min(rows, 64)][cols] workspace
+};
+// column c of the sum goes to seg[s] with begin[s] <= c < begin[s + 1], at place perm(c - begin[s]): [cols / inner][inner] -> transposed
+struct RowSumOut {
+  void* ptr[3];
+  int32_t type[3];
+  long begin[4];
+  long major[3], minor[3];     // column c' of segment s is (c' / minor, c' % minor) -> stored at (c' % minor) * major + c' / minor
+};
+hipError_t row_sum(const RowSum& s, const RowSumOut& out, hipStream_t stream);
+inline long row_sum_mid_rows(long rows) { return rows > 256 ? 64 : 0; }
+
+inline hipError_t last() { return hipGetLastError(); }
+
+}  // namespace learn
+}  // namespace lqg

@@ -1,0 +1,146 @@
+// lqg_selscan.hip — selective state-space scan (include/lqg_learn.h): with -DLQG_SELSCAN_TYPE=<type> the kernels for sequences of that
+// type, without it the C entry points.
+#include "lqg_selscan.hpp"
+
+using namespace lqg::learn;
+
+#ifdef LQG_SELSCAN_TYPE
+namespace lqg {
+namespace learn {
+typedef LQG_SELSCAN_TYPE IT;
+template <> int ScanOf<IT>::run(int what, const ScanArgs& a, hipStream_t st) { return by_states<IT>(what, a, st); }
+template <> int ScanOf<IT>::groups(const ScanArgs& a, long groups, hipStream_t st) { return launch_groups<IT>(a, groups, st); }
+template <> int ScanOf<IT>::step(const ScanArgs& a, float* state, hipStream_t st) { return launch_step<IT>(a, state, st); }
+}  // namespace learn
+}  // namespace lqg
+#else
+namespace lqg {
+namespace learn {
+#define X(IT)                                                                         \
+  template <> int ScanOf<IT>::run(int, const ScanArgs&, hipStream_t);                 \
+  template <> int ScanOf<IT>::groups(const ScanArgs&, long, hipStream_t);             \
+  template <> int ScanOf<IT>::step(const ScanArgs&, float*, hipStream_t);
+X(float) X(bf16) X(f16)
+#undef X
+}  // namespace learn
+}  // namespace lqg
+
+namespace {
+
+int check(const lqg_selscan* p) {
+  if (!p) return LQG_ERR_NULL;
+  if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
+  if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > (1L << 24) || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
+  if (p->chunks < 0 || p->chunks > 64) return LQG_ERR_ARG;
+  for (const lqg_param* q : {&p->A, &p->Dskip, &p->delta_bias})
+    if (q->ptr && q->type != LQG_T_F32 && q->type != LQG_T_BF16 && q->type != LQG_T_F16) return LQG_ERR_ARG;
+  return 0;
+}
+
+int tile_of(long N) { return N > 32 ? 8 : 16; }
+
+ScanArgs describe(const lqg_selscan* p) {
+  ScanArgs a{};
+  a.p = *p;
+  const long TT = tile_of(p->N);
+  a.Dg = p->D / p->G;
+  a.bpg = (a.Dg + 63) / 64;
+  a.blocks = a.bpg * p->G;
+  a.tiles = (p->T + TT - 1) / TT;
+  a.chunks = 1;
+  if (p->chunks) a.chunks = p->chunks;
+  if (a.chunks > a.tiles) a.chunks = a.tiles;
+  const long per = (a.tiles + a.chunks - 1) / a.chunks;
+  a.chunk = per * TT;
+  a.chunks = (a.tiles + per - 1) / per;               // no empty chunk
+  return a;
+}
+
+long carry_floats(const ScanArgs& a) { return a.chunks > 1 ? a.p.B * a.chunks * (a.p.N + 1) * a.p.D : 0; }
+
+int by_type(int what, const ScanArgs& a, hipStream_t st) {
+  if (a.p.type == LQG_T_F32) return ScanOf<float>::run(what, a, st);
+  if (a.p.type == LQG_T_BF16) return ScanOf<bf16>::run(what, a, st);
+  return ScanOf<f16>::run(what, a, st);
+}
+
+bool have(const lqg_selscan* p) { return p->u.ptr && p->delta.ptr && p->A.ptr && p->Bm.ptr && p->Cm.ptr; }
+
+struct GradSpace { long carry, group, rows, cols, mid, total; };
+GradSpace grad_space(const ScanArgs& a) {
+  GradSpace s;
+  s.carry = carry_floats(a);
+  s.group = a.blocks * a.p.B * a.p.T * a.p.N;
+  s.rows = a.p.B * a.chunks;
+  s.cols = (a.p.N + 2) * a.p.D;
+  s.mid = row_sum_mid_rows(s.rows) * s.cols;
+  s.total = s.carry + 2 * s.group + s.rows * s.cols + s.mid;
+  return s;
+}
+
+}  // namespace
+
+extern "C" size_t lqg_selscan_workspace(const lqg_selscan* p) {
+  return check(p) ? 0 : (size_t)carry_floats(describe(p)) * sizeof(float);
+}
+extern "C" size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p) {
+  return check(p) ? 0 : (size_t)(p->B * describe(p).tiles * p->N * p->D) * sizeof(float);
+}
+extern "C" size_t lqg_selscan_grad_workspace(const lqg_selscan* p) {
+  return check(p) ? 0 : (size_t)grad_space(describe(p)).total * sizeof(float);
+}
+
+extern "C" int lqg_selective_scan(const lqg_selscan* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(p)) return rc;
+  if (!have(p) || !p->y.ptr) return LQG_ERR_NULL;
+  ScanArgs a = describe(p);
+  const long carry = carry_floats(a);
+  if (carry && !workspace) return LQG_ERR_NULL;
+  if (workspace_bytes < carry * sizeof(float)) return LQG_ERR_WORKSPACE;
+  a.hl = static_cast<float*>(workspace);
+  a.sd = a.hl + (carry ? p->B * a.chunks * p->N * p->D : 0);
+  return by_type(0, a, (hipStream_t)stream);
+}
+
+extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_bars* g, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  if (const int rc = check(p)) return rc;
+  if (!g || !have(p) || !p->checkpoints || !workspace) return LQG_ERR_NULL;
+  if (!g->dy.ptr || !g->du || !g->ddelta || !g->dBm || !g->dCm || (p->z.ptr && !g->dz)) return LQG_ERR_NULL;
+  ScanArgs a = describe(p);
+  a.g = *g;
+  const GradSpace s = grad_space(a);
+  if (workspace_bytes < s.total * sizeof(float)) return LQG_ERR_WORKSPACE;
+  float* ws = static_cast<float*>(workspace);
+  a.hl = ws;
+  a.sd = ws + (s.carry ? p->B * a.chunks * p->N * p->D : 0);
+  a.partB = ws + s.carry;
+  a.partC = a.partB + s.group;
+  a.partP = a.partC + s.group;
+  hipStream_t st = (hipStream_t)stream;
+  const long n = p->B * p->T * p->G * p->N, groups = (n + 255) / 256;
+  if (!grid_fits(groups, 256)) return LQG_ERR_ARG;
+  if (const int rc = by_type(1, a, st)) return rc;
+  const int rc = p->type == LQG_T_F32 ? ScanOf<float>::groups(a, groups, st)
+                 : p->type == LQG_T_BF16 ? ScanOf<bf16>::groups(a, groups, st) : ScanOf<f16>::groups(a, groups, st);
+  if (rc) return rc;
+  RowSum r{a.partP, s.rows, s.cols, a.partP + s.rows * s.cols};
+  RowSumOut o{};
+  o.ptr[0] = g->dA, o.type[0] = p->A.type, o.major[0] = p->N, o.minor[0] = p->D;
+  o.ptr[1] = g->dD, o.type[1] = p->Dskip.type, o.major[1] = 1, o.minor[1] = p->D;
+  o.ptr[2] = g->ddelta_bias, o.type[2] = p->delta_bias.type, o.major[2] = 1, o.minor[2] = p->D;
+  o.begin[1] = p->N * p->D, o.begin[2] = (p->N + 1) * p->D, o.begin[3] = s.cols;
+  return (int)row_sum(r, o, st);
+}
+
+extern "C" int lqg_selective_scan_step(const lqg_selscan* p, float* state, void* stream) {
+  if (const int rc = check(p)) return rc;
+  if (p->T != 1) return LQG_ERR_ARG;
+  if (!have(p) || !p->y.ptr || !state) return LQG_ERR_NULL;
+  ScanArgs a = describe(p);
+  hipStream_t st = (hipStream_t)stream;
+  if (p->type == LQG_T_F32) return ScanOf<float>::step(a, state, st);
+  if (p->type == LQG_T_BF16) return ScanOf<bf16>::step(a, state, st);
+  return ScanOf<f16>::step(a, state, st);
+}
+#endif

@@ -1,4 +1,4 @@
-"""scipy.optimize.minimize with gradients from torch.autograd — the role of lqg/optim.py:14-169 (`minimize`: the
+"""`minimize` — scipy.optimize.minimize with gradients from torch.autograd — the role of lqg/optim.py:14-169 (`minimize`: the
 reference wraps scipy with `jit(grad(fun))`, optim.py:142-147).
 
 `fun(x, *args)` is written with torch ops on a parameter "tree" x (a tensor, or a dict / list / tuple of tensors or
@@ -6,10 +6,18 @@ floats) and returns a scalar tensor; for a likelihood it would build a model fro
 `-model.log_likelihood(data).sum()`, which is differentiable through the HIP adjoint sweep (lqg_amd/grad.py).  With an
 initialised process group and trial-sharded data, all-reduce inside `fun` is not needed: pass `group=` and the value and
 gradient are summed over ranks here (one all-reduce of 1 + P numbers per evaluation, lqg_amd/dist.py).
+
+`AdamW` — the first-order loop's step for the same trees, on the device and without a synchronisation: one HIP launch for all tensors
+(lqg_amd/csrc/lqg_adamw.hip).  `infer.max_likelihood` steps with it.
 """
+import ctypes as C
+
 import numpy as np
 import scipy.optimize
 import torch
+
+from lqg_amd import _abi, _learn
+from lqg_amd._abi import LqgHipError
 
 
 def _flatten(tree):
@@ -86,3 +94,178 @@ def minimize(fun, x0, method=None, args=(), bounds=None, constraints=(), tol=Non
                                   constraints=constraints, tol=tol, options=options)
     res["x"] = rebuild(unravel(res["x"], False))
     return res
+
+
+STATE_BLOCK = 256        # elements of a tensor that share one scale in 8-bit states; every tensor's states begin at a multiple of it
+
+
+class AdamW:
+    """m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr weight_decay) - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
+    for every tensor of a tree (a tensor, or dicts / lists / tuples of tensors; an iterator is read into a list), in place, in as many
+    launches as there are types of tensors (one per 96 tensors).
+
+        opt = AdamW(params, lr=1e-2)
+        loss(params).backward();  opt.step();  opt.zero_grad()
+
+    Tensors are contiguous leaves on one GPU; float32, bfloat16 and float16 may be mixed, float64 ones take an optimiser of their own.
+    Arithmetic is float32 (float64 for float64 tensors), every operation rounded by itself; a narrower tensor is rounded once when it is
+    written.  Tensors whose `.grad` is None are left as they are, states included.
+
+    state_bits=32: moments in float32 (float64 for float64 tensors).  state_bits=8: m and sqrt(v) as e4m3 values in units of one float32
+    scale for every 256 elements of a tensor, the block's largest magnitude being 448 units (the root, since an 8-bit float spans 18
+    octaves and the update divides by the root; one that is not 0 is held as the least value at least).  A quarter of the memory; a
+    NaN or infinite gradient makes its block NaN, where in 32 bits it reaches its own element alone.
+
+    lr, betas, eps, weight_decay are attributes that may be changed between steps.  capturable=True keeps the step count on the device,
+    so that `step` can be captured into a graph and replayed (lr and the other numbers are those of the capture); without it a
+    capture is refused, since the graph would repeat one step count."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
+        if not isinstance(params, (torch.Tensor, dict, list, tuple)):
+            params = list(params)
+        self.params = _tensors(params)
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.state_bits, self.capturable = state_bits, bool(capturable)
+        self._numbers()
+        if state_bits not in (8, 32):
+            raise LqgHipError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if not self.params:
+            raise LqgHipError("AdamW: no tensors to step")
+        seen, wide = set(), [p.dtype == torch.float64 for p in self.params]
+        dev = self.params[0].device
+        for p in self.params:
+            if p.dtype not in _learn.TYPES:
+                raise LqgHipError(f"AdamW: unsupported dtype {p.dtype}: float32, float64, bfloat16 or float16")
+            if p.device != dev:
+                raise LqgHipError(f"AdamW: tensors on {dev} and {p.device}: one device is needed")
+            if not p.is_leaf:
+                raise LqgHipError("AdamW: a tensor is not a leaf: its gradient is not kept")
+            if not p.is_contiguous():
+                raise LqgHipError(f"AdamW: a contiguous tensor is needed, got strides {tuple(p.stride())} for {tuple(p.shape)}")
+            if p.numel() and p.data_ptr() in seen:
+                raise LqgHipError("AdamW: the same tensor twice")
+            seen.add(p.data_ptr())
+        if any(wide) and not all(wide):
+            raise LqgHipError("AdamW: float64 tensors take an optimiser of their own")
+        if any(wide) and state_bits == 8:
+            raise LqgHipError("AdamW: float64 tensors keep 32-bit or wider states: state_bits=8 is not for them")
+        if dev.type != "cuda":
+            raise LqgHipError(f"lqg_amd computes on MI355X only: tensors are on '{dev}'; there is no CPU fallback")
+        self.device = dev
+        self._sizes = [(p.dtype, p.device, p.numel()) for p in self.params]
+        self.offsets, total = [], 0
+        for p in self.params:
+            self.offsets.append(total)
+            total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        moment = torch.float64 if any(wide) else torch.float32
+        if state_bits == 8:
+            self._state = {name: torch.zeros(total, dtype=torch.float8_e4m3fn, device=dev) for name in ("exp_avg", "exp_rms")}
+            self._state.update({name + "_scale": torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=dev)
+                                for name in ("exp_avg", "exp_rms")})
+        else:
+            self._state = {name: torch.zeros(total, dtype=moment, device=dev) for name in ("exp_avg", "exp_avg_sq")}
+        self._step = 0
+        self._counter = torch.tensor([0.0, 1.0, 1.0], dtype=torch.float64, device=dev) if capturable else None
+        # one call per type of tensor: its indices, and the C arrays that describe it
+        self._calls = []
+        for dtype in dict.fromkeys(p.dtype for p in self.params):
+            index = [i for i, p in enumerate(self.params) if p.dtype == dtype and p.numel()]
+            if index:
+                n = len(index)
+                call = _learn.AdamW()
+                call.type, call.bits = _learn.TYPES[dtype], state_bits
+                arrays = (C.c_void_p * n)(), (C.c_void_p * n)(), (C.c_int64 * n)(), (C.c_int64 * n)()
+                call.params, call.grads, call.numel, call.offset = (C.addressof(x) for x in arrays)
+                first, second = ("exp_avg", "exp_rms") if state_bits == 8 else ("exp_avg", "exp_avg_sq")
+                call.exp_avg, call.exp_avg_sq = self._state[first].data_ptr(), self._state[second].data_ptr()
+                if state_bits == 8:
+                    call.exp_avg_scale = self._state["exp_avg_scale"].data_ptr()
+                    call.exp_avg_sq_scale = self._state["exp_rms_scale"].data_ptr()
+                call.step_state = _learn.ptr(self._counter)
+                self._calls.append((index, call, arrays))
+
+    def _numbers(self):
+        b1, b2 = self.betas
+        if not (self.lr >= 0 and self.eps >= 0 and self.weight_decay >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
+            raise LqgHipError(f"AdamW: lr, eps, weight_decay >= 0 and 0 <= betas < 1 are needed, got lr={self.lr}, betas={self.betas}, "
+                              f"eps={self.eps}, weight_decay={self.weight_decay}")
+        return b1, b2
+
+    @torch.no_grad()
+    def step(self):
+        """One update from the tensors' `.grad`."""
+        b1, b2 = self._numbers()
+        if not self.capturable and torch.cuda.is_current_stream_capturing():
+            raise LqgHipError("AdamW.step: the step count of this optimiser is on the host, and a captured graph would repeat it: "
+                              "use capturable=True")
+        kept, moved = [], []
+        for index, call, (params, grads, numel, offset) in self._calls:
+            n = 0
+            for i in index:
+                p = self.params[i]
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse or g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+                    raise LqgHipError(f"AdamW.step: a dense gradient of {p.dtype} {tuple(p.shape)} is needed, got {g.dtype} {tuple(g.shape)}")
+                if (p.dtype, p.device, p.numel()) != self._sizes[i] or not p.is_contiguous():
+                    raise LqgHipError("AdamW.step: a tensor's type, device, size or order is not what it was")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    kept.append(g)
+                params[n], grads[n], numel[n], offset[n] = p.data_ptr(), g.data_ptr(), p.numel(), self.offsets[i]
+                moved.append(p)
+                n += 1
+            call.count = n
+        lib = _learn.load()
+        self._step += 1
+        with _learn.on_device(self.device):
+            stream = _learn.stream(self.device)
+            if self.capturable:
+                _abi.check(lib.lqg_adamw_advance(self._counter.data_ptr(), b1, b2, stream), "lqg_adamw_advance")
+            for _, call, _ in self._calls:
+                if call.count:
+                    call.lr, call.beta1, call.beta2, call.eps, call.weight_decay = self.lr, b1, b2, self.eps, self.weight_decay
+                    call.step = self._step
+                    _abi.check(lib.lqg_adamw_step(C.byref(call), stream), "lqg_adamw_step")
+        torch.autograd.graph.increment_version(moved)
+
+    def zero_grad(self):
+        """Forget the gradients."""
+        for p in self.params:
+            p.grad = None
+
+    def steps(self):
+        """Steps taken (capturable: read back from the device)."""
+        return int(self._counter[0]) if self.capturable else self._step
+
+    def state_dict(self):
+        """{"step", and the states themselves: "exp_avg" with "exp_avg_sq", or (8 bits) with "exp_avg_scale", "exp_rms" and
+        "exp_rms_scale"}.  Tensors are the optimiser's own, laid out one parameter after the other at multiples of 256 elements
+        (`offsets`); copy what has to outlive the next step."""
+        return dict(step=self.steps() if self.capturable and not torch.cuda.is_current_stream_capturing() else self._step, **self._state)
+
+    def load_state_dict(self, state):
+        """Copies what `state_dict` of an optimiser over tensors of the same sizes gave."""
+        if set(state) != {"step", *self._state} or int(state["step"]) < 0:
+            raise LqgHipError(f"AdamW.load_state_dict: {sorted(['step', *self._state])} are needed, got {sorted(state)}")
+        for k, t in self._state.items():
+            if not isinstance(state[k], torch.Tensor) or state[k].shape != t.shape or state[k].dtype != t.dtype:
+                raise LqgHipError(f"AdamW.load_state_dict: {k} needs {t.dtype} {tuple(t.shape)}")
+        for k, t in self._state.items():
+            t.copy_(state[k])
+        self._step = int(state["step"])
+        if self.capturable:
+            b1, b2 = self._numbers()
+            inv = [1 / (1 - b ** self._step) if self._step else 1.0 for b in (b1, b2)]
+            self._counter.copy_(torch.tensor([float(self._step), *inv], dtype=torch.float64))
+
+
+def _tensors(tree):
+    if isinstance(tree, torch.Tensor):
+        return [tree]
+    if isinstance(tree, dict):
+        tree = list(tree.values())
+    if not isinstance(tree, (list, tuple)):
+        raise LqgHipError(f"AdamW: a tensor is needed, got {type(tree).__name__}")
+    return [t for x in tree for t in _tensors(x)]

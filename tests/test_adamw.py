@@ -1,0 +1,416 @@
+"""lqg_amd.optim.AdamW: the step over many tensors, with 32-bit and 8-bit states, against float64."""
+import pytest
+import torch
+
+import learn_oracle as O
+from lqg_amd._abi import LqgHipError
+from lqg_amd.optim import AdamW
+
+gpu = pytest.mark.gpu
+F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+HYPER = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU)
+
+def test_adamw_refuses():
+    t = torch.zeros(4)
+    leaf = torch.zeros(3, requires_grad=True)
+    for bad, msg in (
+            (lambda: AdamW([]), "no tensors"), (lambda: AdamW([t], state_bits=4), "state_bits"), (lambda: AdamW([t], lr=-1), "lr"),
+            (lambda: AdamW([t], lr=float("nan")), "lr"), (lambda: AdamW([t], betas=(1.0, 0.9)), "betas"),
+            (lambda: AdamW([t], eps=-1e-8), "eps"), (lambda: AdamW({"a": [t, 3.0]}), "a tensor is needed, got float"),
+            (lambda: AdamW([t.int()]), "unsupported dtype"), (lambda: AdamW([t, t]), "same tensor twice"),
+            (lambda: AdamW([torch.zeros(3, 4).t()]), "contiguous"), (lambda: AdamW([leaf * 2]), "not a leaf"),
+            (lambda: AdamW([t, t.double()]), "of their own"), (lambda: AdamW([t.double()], state_bits=8), "32-bit or wider"),
+            (lambda: AdamW([t, torch.zeros(3, device="meta")]), "one device"), (lambda: AdamW(iter([t])), "no CPU fallback")):
+        with pytest.raises(LqgHipError, match=msg):
+            bad()
+
+
+# ------------------------------------------------------------------------------------------------ values
+
+SIZES = ((1,), (3,), (255,), (256,), (257,), (5, 77), (2049,), (0,), (4, 4, 4), (100, 100), (1023,), (2048,))
+
+
+def tensors(dtype, sizes=SIZES, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    make = lambda s: (torch.randn(*s, generator=g, dtype=torch.float64) * scale).to(dtype).cuda()  # noqa: E731
+    return [make(s) for s in sizes]
+
+
+def unit(dtype):
+    """Half a step of the arithmetic."""
+    return 2.0 ** -53 if dtype == F64 else 2.0 ** -24
+
+
+def arenas(opt):
+    return {k: v.double().cpu() for k, v in opt.state_dict().items() if k != "step"}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (F32, F64, BF16, F16))
+def test_steps_in_32_bits(dtype):
+    params = [p.requires_grad_() for p in tensors(dtype)]
+    opt = AdamW(params, **HYPER)
+    for step in range(1, 4):
+        before = arenas(opt)
+        was, grads = [p.detach().double().cpu() for p in params], tensors(dtype, seed=step, scale=0.1)
+        for p, g in zip(params, grads):
+            p.grad = g
+        version = params[0]._version
+        opt.step()
+        assert opt.steps() == step and params[0]._version > version
+        after = arenas(opt)
+        e = unit(dtype)
+        for p, p0, g, off in zip(params, was, grads, opt.offsets):
+            n, shape = p.numel(), p.shape
+            m0, v0 = (before[k][off:off + n].view(shape) for k in ("exp_avg", "exp_avg_sq"))
+            g = g.double().cpu()
+            want, m, v = O.adamw(p0, g, m0, v0, step, **HYPER)
+            # two products, their constants and a sum: 5 roundings; the square has one more
+            size = lambda a, b: a.abs() + b.abs()  # noqa: E731
+            assert ((after["exp_avg"][off:off + n].view(shape) - m).abs() <= 5 * e * size(0.9 * m0, 0.1 * g) + 1e-45).all()
+            assert ((after["exp_avg_sq"][off:off + n].view(shape) - v).abs() <= 6 * e * size(0.99 * v0, 0.01 * g * g) + 1e-45).all()
+            # quotient: numerator 5 + 2, root (6 + 2) / 2 + 1, sum with eps 2, quotient, lr: 18 roundings of sizes at most lr |m| / far
+            num = size(0.9 * m0, 0.1 * g) / (1 - 0.9 ** step)
+            far = torch.sqrt(v / (1 - 0.99 ** step)) + HYPER["eps"]
+            bound = e * (18 * HYPER["lr"] * num / far + 4 * p0.abs()) + O.half(dtype) * want.abs() * (1 + 2.0 ** -8) + (2.0 ** -25 if dtype == F16 else 0)
+            assert ((p.detach().double().cpu() - want).abs() <= bound).all(), (shape, step)
+
+
+@gpu
+def test_the_bits_of_the_formula():
+    """float64: the bits of the update written in torch operations, one rounding each (what infer.max_likelihood's loop computed)."""
+    z = tensors(F64, ((7,),))[0]
+    p = z.clone().requires_grad_()
+    opt = AdamW(p, lr=0.05, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)
+    m, v = torch.zeros_like(z), torch.zeros_like(z)
+    for step in range(1, 20):
+        g = tensors(F64, ((7,),), seed=step)[0]
+        p.grad = g
+        opt.step()
+        m = 0.9 * m + (1 - 0.9) * g
+        v = 0.999 * v + (1 - 0.999) * g * g
+        z = z - 0.05 * (m / (1 - 0.9 ** step)) / (torch.sqrt(v / (1 - 0.999 ** step)) + 1e-8)
+        assert torch.equal(p.detach(), z), step
+
+
+def check8(opt, params, before, was, grads, step, dtype):
+    """One 8-bit step: the parameters and scales to rounding; each held value is the nearest e4m3 value of the exact quotient, or, where
+    that quotient is within the arithmetic's rounding of the middle between two values, the other one.  (A value that is not the nearest is
+    more than half a step away, so the bound of half a step and the slack says just that.  How many of them there are depends on the
+    data: quotients of two 8-bit significands meet middles exactly, a count has no bound of its own.)"""
+    after = arenas(opt)
+    e = 2.0 ** -24
+    total = before["exp_avg"].numel()
+    full = {k: torch.zeros(total, dtype=torch.float64) for k in ("m", "r", "me", "re")}
+    for p, p0, g, off in zip(params, was, grads, opt.offsets):
+        n = p.numel()
+        at = slice(off, off + n)
+        m0 = before["exp_avg"][at] * before["exp_avg_scale"].repeat_interleave(256)[at]
+        r0 = before["exp_rms"][at] * before["exp_rms_scale"].repeat_interleave(256)[at]
+        g, q = g.double().cpu().view(-1), p0.view(-1)
+        want, m, v = O.adamw(q, g, m0, r0 * r0, step, **HYPER)
+        num = (0.9 * m0).abs() + (0.1 * g).abs()
+        far = torch.sqrt(v / (1 - 0.99 ** step)) + HYPER["eps"]
+        bound = e * (22 * HYPER["lr"] * num / (1 - 0.9 ** step) / far + 4 * q.abs()) + O.half(dtype) * want.abs() * (1 + 2.0 ** -8)
+        got, fine = p.detach().double().cpu().view(-1), torch.isfinite(want)
+        assert torch.equal(torch.isfinite(got), fine)
+        assert ((got - want).abs() <= bound + (2.0 ** -25 if dtype == F16 else 0))[fine].all(), (tuple(p.shape), step)
+        full["m"][at], full["r"][at] = m, torch.sqrt(v)
+        full["me"][at], full["re"][at] = 7 * e * num, 6 * e * torch.sqrt(v)
+    for k, key, root in (("m", "exp_avg", False), ("r", "exp_rms", True)):
+        _, scale = O.pack8(full[k], root)
+        whole = torch.isfinite(full[k].view(-1, 256)).all(1)
+        assert not torch.isfinite(after[key + "_scale"])[~whole].any()
+        assert ((after[key + "_scale"] - scale).abs() <= 10 * e * scale + full[k + "e"].view(-1, 256).amax(1) / 448)[whole].all()
+        got, sc, whole = after[key], scale.repeat_interleave(256), whole.repeat_interleave(256)
+        # within half a step of e4m3 of the exact quotient, and the quotient's own rounding
+        x = torch.where(sc > 0, full[k] / sc.clamp(min=1e-300), 0)
+        half = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 4)
+        slack = full[k + "e"] / sc.clamp(min=1e-300) + 20 * e * x.abs()
+        least = torch.full_like(x, 2.0 ** -9 if root else 0.0)
+        ok = ((got - x).abs() <= half * (1 + 2.0 ** -20) + slack) | ((x > 0) & (x < 2.0 ** -9) & (got == least))
+        assert ok[whole].all(), (key, step)
+        if root:
+            assert ((got > 0) | (full[k] == 0) | (sc == 0))[whole].all()
+
+
+@gpu
+@pytest.mark.parametrize("sign", (1, -1))
+@pytest.mark.parametrize("dtype", (F32, BF16, F16))
+def test_steps_in_8_bits(dtype, sign):
+    """(sign 1: gradients up to 2^19 and more, which float16 holds as infinities: their elements become NaN and their blocks' states with
+    them; sign -1: down to 2^-19.)"""
+    params = [p.requires_grad_() for p in tensors(dtype)]
+    opt = AdamW(params, **HYPER, state_bits=8)
+    for step in range(1, 5):
+        before, was = arenas(opt), [p.detach().double().cpu() for p in params]
+        grads = tensors(dtype, seed=step, scale=0.1)
+        for i, g in enumerate(grads):
+            if g.numel() > 200:                      # a wide range within a block, zeros among it
+                g.mul_(torch.exp2(sign * (-torch.arange(g.numel(), device="cuda") % 20)).view(g.shape).to(dtype))
+                g.view(-1)[::7] = 0
+            params[i].grad = g
+        opt.step()
+        check8(opt, params, before, was, grads, step, dtype)
+
+
+@gpu
+def test_every_8_bit_value_survives():
+    """Unpacking and packing: with no gradient and b1 = b2 = 0.5 a block halves, and its codes stay (for roots: times sqrt(1/2))."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes[127] = codes[255] = 0x7E                   # (NaN's place: the largest value instead)
+    codes[128] = 0
+    p = torch.zeros(256, device="cuda", requires_grad=True)
+    p.grad = torch.zeros_like(p)
+    opt = AdamW(p, betas=(0.5, 0.5), state_bits=8)
+    held = codes.cuda().view(torch.float8_e4m3fn)
+    opt.load_state_dict(dict(step=3, exp_avg=held, exp_rms=(codes & 127).cuda().view(torch.float8_e4m3fn),
+                             exp_avg_scale=torch.full((1,), 0.25, device="cuda"), exp_rms_scale=torch.full((1,), 0.5, device="cuda")))
+    opt.step()
+    s = opt.state_dict()
+    assert torch.equal(s["exp_avg"].float(), held.float()) and float(s["exp_avg_scale"]) == 0.125
+    assert torch.equal(s["exp_rms"].float(), (codes & 127).cuda().view(torch.float8_e4m3fn).float())
+    assert abs(float(s["exp_rms_scale"]) - 0.5 ** 1.5) < 1e-7
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_zero_and_broken_gradients(bits):
+    p = torch.ones(600, device="cuda", requires_grad=True)
+    opt = AdamW(p, lr=0.1, weight_decay=0.0, state_bits=bits)
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    assert torch.equal(p.detach(), torch.ones_like(p))               # 0 / (0 + eps)
+    assert all(float(t.float().abs().sum()) == 0 for k, t in opt.state_dict().items() if k != "step")
+    p.grad = torch.ones_like(p)
+    p.grad[300], p.grad[599] = float("nan"), float("inf")
+    opt.step()
+    bad = ~torch.isfinite(p.detach())
+    assert bad[300] and bad[599] and int(bad.sum()) == 2
+    p.grad = torch.ones_like(p)
+    opt.step()
+    bad = ~torch.isfinite(p.detach())
+    assert not bad[:256].any() and bad[300]
+    if bits == 32:
+        assert int(bad.sum()) == 2
+    else:
+        assert bad[256:].all()                       # a block's scale carries it to the block
+
+
+@gpu
+def test_tiny_gradients_do_not_explode_in_8_bits():
+    """Elements 2^20 and more below their block's largest keep updates of at most a few lr (a root held as 0 would give |m| / eps)."""
+    g = torch.Generator().manual_seed(4)
+    p = torch.zeros(4096, device="cuda", requires_grad=True)
+    opt = AdamW(p, lr=1e-3, weight_decay=0.0, state_bits=8)
+    scale = torch.exp2(-torch.randint(0, 40, (4096,), generator=g).float()).cuda()
+    for _ in range(30):
+        was = p.detach().clone()
+        p.grad = torch.randn(4096, generator=g).cuda() * scale
+        opt.step()
+        # |m| <= its value in full + half a step of its code against a root no smaller than half a step below its own: at most
+        # max|g| sums give 1 / sqrt(1 - b2) = 31 lr in full precision as well
+        assert float((p.detach() - was).abs().max()) < 40e-3
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_mixed_trees_missing_gradients_and_many_tensors(bits):
+    """Three types in a tree of 250 tensors (three launches for one type): the same as one optimiser each; a tensor without a
+    gradient stays, with its states."""
+    g = torch.Generator().manual_seed(1)
+    sizes = [(int(torch.randint(1, 600, (1,), generator=g)),) for _ in range(250)]
+    kinds = [(F32, BF16, F16)[i % 3] if i < 60 else F32 for i in range(250)]
+    make = lambda: [tensors(k, (s,), seed=j)[0].requires_grad_() for j, (k, s) in enumerate(zip(kinds, sizes))]  # noqa: E731
+    a, b = make(), make()
+    one = AdamW({"x": a[:100], "y": (a[100], a[101:])}, **HYPER, state_bits=bits)
+    each = [AdamW(p, **HYPER, state_bits=bits) for p in b]
+    for step in range(3):
+        for j, (p, q) in enumerate(zip(a, b)):
+            p.grad = None if (j + step) % 5 == 0 and j % 2 else tensors(p.dtype, (tuple(p.shape),), seed=1000 * step + j)[0]
+            q.grad = p.grad
+        one.step()
+        for opt in each:
+            opt.step()
+    for j, (p, q) in enumerate(zip(a, b)):
+        assert torch.equal(p.detach(), q.detach()), j
+    for j, opt in enumerate(each):
+        for k, t in opt.state_dict().items():
+            if k != "step":
+                per = 256 if k.endswith("scale") else 1
+                off = one.offsets[j] // per
+                assert torch.equal(one.state_dict()[k][off:off + t.numel()].float(), t.float()), (j, k)
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("dtype", (F32, BF16))
+def test_alignment_and_neighbours(bits, dtype):
+    """Views at odd places give the same bits as aligned tensors, and what lies around them stays."""
+    host = torch.full((5000,), 7.0, dtype=dtype, device="cuda")
+    gh = tensors(dtype, ((5000,),), seed=3)[0]
+    view = host[3:3 + 2999]
+    plain = view.clone().requires_grad_()
+    odd = view.detach().requires_grad_()
+    odd.grad, plain.grad = gh[1:3000], gh[1:3000].clone()
+    A, B = AdamW(odd, **HYPER, state_bits=bits), AdamW(plain, **HYPER, state_bits=bits)
+    for _ in range(2):
+        A.step(), B.step()
+    assert torch.equal(odd.detach(), plain.detach())
+    assert (host[:3] == 7).all() and (host[3002:] == 7).all()
+    strided = tensors(dtype, ((2999, 2),), seed=3)[0][:, 0]
+    odd.grad, plain.grad = strided, strided.contiguous()
+    A.step(), B.step()
+    assert torch.equal(odd.detach(), plain.detach())
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_states_saved_and_loaded(bits):
+    a, b = ([p.requires_grad_() for p in tensors(F32)] for _ in range(2))
+    A = AdamW(a, **HYPER, state_bits=bits)
+    for step in range(2):
+        for p, g in zip(a, tensors(F32, seed=step + 1)):
+            p.grad = g
+        A.step()
+    B = AdamW(b, **HYPER, state_bits=bits, capturable=True)
+    B.load_state_dict({k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in A.state_dict().items()})
+    for p, q, g in zip(a, b, tensors(F32, seed=9)):
+        q.data.copy_(p.data)
+        p.grad = q.grad = g
+    A.step(), B.step()
+    assert B.steps() == A.steps() == 3
+    for p, q in zip(a, b):                           # (1 / (1 - b^t) in double on the device, in float on the host: one rounding)
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-8)
+    with pytest.raises(LqgHipError, match="are needed"):
+        A.load_state_dict({"step": 1})
+    with pytest.raises(LqgHipError, match="exp_avg needs"):
+        A.load_state_dict({**A.state_dict(), "exp_avg": torch.zeros(5, device="cuda")})
+    A.zero_grad()
+    assert all(p.grad is None for p in a)
+    kept = [p.detach().clone() for p in a]
+    A.step()
+    assert all(torch.equal(p.detach(), q) for p, q in zip(a, kept))
+
+
+@gpu
+def test_step_refuses():
+    p = torch.zeros(6, device="cuda", requires_grad=True)
+    opt = AdamW(p)
+    p.grad = torch.zeros(6, device="cuda").to_sparse()
+    with pytest.raises(LqgHipError, match="dense gradient"):
+        opt.step()
+    p.grad = None
+    opt.lr = -1.0
+    with pytest.raises(LqgHipError, match="lr"):
+        opt.step()
+    opt.lr = 1e-3
+    p.data = torch.zeros(7, device="cuda")
+    p.grad = torch.zeros(7, device="cuda")
+    with pytest.raises(LqgHipError, match="not what it was"):
+        opt.step()
+    q = torch.zeros(6, device="cuda", requires_grad=True)
+    host = AdamW(q)
+    q.grad = torch.ones_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = q.grad + 1                               # (a capture needs something in it)
+        with pytest.raises(LqgHipError, match="capturable=True"):
+            host.step()
+    del x
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_captured_step(bits):
+    """A captured step replayed, with eager work between: the steps of an eager optimiser."""
+    p, q = (tensors(F32, ((3000,),))[0].requires_grad_() for _ in range(2))
+    p.grad = torch.zeros_like(p)
+    A, B = AdamW(p, **HYPER, state_bits=bits, capturable=True), AdamW(q, **HYPER, state_bits=bits, capturable=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        A.step()
+    A.load_state_dict({**{k: torch.zeros_like(v) for k, v in A.state_dict().items() if k != "step"}, "step": 0})
+    for step in range(4):
+        g = tensors(F32, ((3000,),), seed=step + 1)[0]
+        with torch.no_grad():
+            p.grad.copy_(g)
+        q.grad = g
+        graph.replay()
+        B.step()
+        torch.cuda.synchronize()
+        assert A.steps() == B.steps() == step + 1
+        assert torch.equal(p.detach(), q.detach())
+
+
+@gpu
+def test_other_stream():
+    p, q = (tensors(F32)[8].requires_grad_() for _ in range(2))
+    A, B = AdamW(p, **HYPER), AdamW(q, **HYPER)
+    p.grad = q.grad = tensors(F32, seed=5)[8]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        A.step()
+    torch.cuda.current_stream().wait_stream(side)
+    B.step()
+    assert torch.equal(p.detach(), q.detach())
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_a_learned_filter_is_trained_and_run(bits):
+    """Convolution, scan and step together: the gradients of a one-step-ahead predictor of tracking data against float64, its update,
+    and a trial run step by step as in training."""
+    import lqg_amd
+    from lqg_amd.belief import ssm
+    x = lqg_amd.BoundedActor(T=40, device="cuda").simulate(3, n=6).float()[..., :2]
+    x = x / x.std()
+    g = torch.Generator().manual_seed(0)
+    D, N = 24, 6
+    shape = dict(inp=(2, D), conv=(D, 4), dt=(D, D), dt_bias=(D,), A_log=(D, N), bc=(D, 2 * N), skip=(D,), out=(D, 2))
+    w = {k: (torch.randn(*s, generator=g) * 0.3).cuda().requires_grad_() for k, s in shape.items()}
+    lengths = torch.tensor([40, 33, 40, 17, 2, 40], device="cuda", dtype=torch.int32)
+    live = (torch.arange(40, device="cuda") < lengths[:, None])[..., None]
+
+    def loss(w, x, conv, scan, live):
+        u = conv(x[:, :40] @ w["inp"], w["conv"])
+        maps = u @ w["bc"]
+        y = scan(u, u @ w["dt"], -torch.exp(w["A_log"]), maps[..., :N], maps[..., N:], w["skip"], w["dt_bias"])
+        return (torch.where(live, y @ w["out"] - x[:, 1:], 0) ** 2).mean()
+
+    own = loss(w, x, lambda a, k: ssm.causal_conv(a, k, silu=True, lengths=lengths),
+               lambda u, dl, A, B, C, D_, b: ssm.selective_scan(u, dl, A, B, C, D_, delta_bias=b, softplus=True, lengths=lengths), live)
+    own.backward()
+    up = {k: t.detach().double().cpu().requires_grad_() for k, t in w.items()}
+    n = lengths.cpu().long()
+    ref = loss(up, x.double().cpu(), lambda a, k: O.conv(a, k, None, None, n, True)[0],
+               lambda u, dl, A, B, C, D_, b: O.scan(u, dl, A, B[:, :, None], C[:, :, None], D_, None, b, True, None, n)[0], live.cpu())
+    ref.backward()
+    assert abs(float(own.detach()) / float(ref.detach()) - 1) < 1e-5
+    for k in w:
+        err = float((w[k].grad.double().cpu() - up[k].grad).norm() / up[k].grad.norm())
+        # some 10^3 float roundings of 2^-24 on the longest path, partly cancelling sums of 10^2 terms
+        assert err < 1e-4, (k, err)
+    was = {k: t.detach().double().cpu() for k, t in w.items()}
+    opt = AdamW(w, **HYPER, state_bits=bits)
+    opt.step()
+    for k in w:
+        want = O.adamw(was[k], w[k].grad.double().cpu(), torch.zeros(()), torch.zeros(()), 1, **HYPER)[0]
+        assert float((w[k].detach().double().cpu() - want).abs().max()) < 1e-6
+    with torch.no_grad():
+        xin = x[:, :40] @ w["inp"]
+        u = ssm.causal_conv(xin, w["conv"], silu=True)
+        maps, dt, A = u @ w["bc"], u @ w["dt"], -torch.exp(w["A_log"])
+        y = ssm.selective_scan(u, dt, A, maps[..., :N], maps[..., N:], w["skip"], delta_bias=w["dt_bias"], softplus=True)
+        cs, hs = torch.zeros(6, 3, D, device="cuda"), torch.zeros(6, D, N, device="cuda")
+        for t in range(40):
+            ut = ssm.causal_conv_step(xin[:, t].contiguous(), cs, w["conv"], silu=True)
+            assert torch.equal(ut, u[:, t])
+            yt = ssm.selective_scan_step(ut, dt[:, t], hs, A, maps[:, t, :N], maps[:, t, N:], w["skip"], delta_bias=w["dt_bias"], softplus=True)
+            assert float((yt - y[:, t]).abs().max()) <= 1e-5 * float(y.abs().max())
