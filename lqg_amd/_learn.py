@@ -29,7 +29,7 @@ class SelScan(C.Structure):
     _fields_ = [("type", C.c_int32), ("softplus", C.c_int32), ("B", C.c_int64), ("T", C.c_int64), ("D", C.c_int64), ("N", C.c_int64),
                 ("G", C.c_int64), ("u", Seq), ("delta", Seq), ("z", Seq), ("Bm", Seq), ("Cm", Seq), ("y", Seq), ("A", Param),
                 ("Dskip", Param), ("delta_bias", Param), ("state", C.c_void_p), ("state_out", C.c_void_p), ("lengths", C.c_void_p),
-                ("checkpoints", C.c_void_p), ("chunks", C.c_int32), ("pad", C.c_int32)]
+                ("checkpoints", C.c_void_p), ("chunks", C.c_int32), ("channels", C.c_int32)]
 
 
 class SelScanBars(C.Structure):

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from lqg_amd import _abi, _learn, options
 from lqg_amd._abi import LqgHipError
 
-MAX_WIDTH, MAX_STATES = 8, 64
+MAX_WIDTH, MAX_STATES, MAX_STRIDE = 8, 64, 1 << 25
 
 
 def _need(ok, what):
@@ -34,7 +34,12 @@ def _sequence(t, name, dims, like=None):
     if like is not None:
         _need(t.dtype == like.dtype and t.device == like.device,
               f"{name}: {t.dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if _as_it_is(t) else t.contiguous()
+
+
+def _as_it_is(t):
+    """Channels next to each other, and steps near enough for the kernels' 32-bit offsets inside a tile."""
+    return (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) <= MAX_STRIDE)
 
 
 def _on_gpu(t):
@@ -125,7 +130,7 @@ class _Conv(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 7
         dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else dy
-        dy = dy if dy.stride(-1) == 1 or D == 1 else dy.contiguous()
+        dy = dy if _as_it_is(dy) else dy.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
         dev = x.device
         dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
@@ -211,7 +216,8 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False):
 def _scan_args(u, A, G, D, delta_bias, softplus):
     p = _learn.SelScan()
     p.type, p.softplus = _learn.TYPES[u.dtype], int(softplus)
-    p.D, p.N, p.G, p.chunks = u.shape[-1], A.shape[1], G, options.get("SELSCAN_CHUNKS")
+    p.D, p.N, p.G = u.shape[-1], A.shape[1], G
+    p.chunks, p.channels = options.get("SELSCAN_CHUNKS"), options.get("SELSCAN_CHANNELS")
     p.A, p.Dskip, p.delta_bias = _learn.param(A), _learn.param(D), _learn.param(delta_bias)
     return p
 
@@ -248,7 +254,7 @@ class _Scan(torch.autograd.Function):
         nB, T, nD = u.shape
         N, G, dev = A.shape[1], Bm.shape[2], u.device
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
-        dy = dy if dy.stride(-1) == 1 or nD == 1 else dy.contiguous()
+        dy = dy if _as_it_is(dy) else dy.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
         new = lambda *shape: torch.empty(shape, dtype=u.dtype, device=dev)  # noqa: E731
         du, ddelta, dz = new(nB, T, nD), new(nB, T, nD), None if z is None else new(nB, T, nD)

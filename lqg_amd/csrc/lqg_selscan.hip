@@ -2,6 +2,8 @@
 // type, without it the C entry points.
 #include "lqg_selscan.hpp"
 
+#include <algorithm>
+
 using namespace lqg::learn;
 
 #ifdef LQG_SELSCAN_TYPE
@@ -27,11 +29,15 @@ X(float) X(bf16) X(f16)
 
 namespace {
 
+constexpr int64_t MAX_STRIDE = 1 << 25;       // rows of a tile are addressed by 32-bit offsets: 16 x 2^25 x 4 bytes
+
 int check(const lqg_selscan* p) {
   if (!p) return LQG_ERR_NULL;
   if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
   if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > (1L << 24) || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
-  if (p->chunks < 0 || p->chunks > 64) return LQG_ERR_ARG;
+  if (p->chunks < 0 || p->chunks > 64 || (p->channels != 0 && p->channels != 32 && p->channels != 64)) return LQG_ERR_ARG;
+  for (const lqg_seq* q : {&p->u, &p->delta, &p->z, &p->Bm, &p->Cm, &p->y})
+    if (q->st < 0 || q->st > MAX_STRIDE) return LQG_ERR_ARG;
   for (const lqg_param* q : {&p->A, &p->Dskip, &p->delta_bias})
     if (q->ptr && q->type != LQG_T_F32 && q->type != LQG_T_BF16 && q->type != LQG_T_F16) return LQG_ERR_ARG;
   return 0;
@@ -44,11 +50,13 @@ ScanArgs describe(const lqg_selscan* p) {
   a.p = *p;
   const long TT = tile_of(p->N);
   a.Dg = p->D / p->G;
-  a.bpg = (a.Dg + 63) / 64;
+  a.ch = p->N > 16 ? 64 : p->channels ? p->channels : 32;
+  a.bpg = (a.Dg + a.ch - 1) / a.ch;
   a.blocks = a.bpg * p->G;
   a.tiles = (p->T + TT - 1) / TT;
-  a.chunks = 1;
-  if (p->chunks) a.chunks = p->chunks;
+  // Waves enough for two on each of the 1024 SIMDs; a chunk is at least 8 tiles.
+  const long waves = a.blocks * p->B * (p->N > 16 ? 8 : p->N > 8 ? 4 : p->N > 4 ? 2 : 1);
+  a.chunks = p->chunks ? p->chunks : std::min(std::min(64L, (a.tiles + 7) / 8), (2048 + waves - 1) / waves);
   if (a.chunks > a.tiles) a.chunks = a.tiles;
   const long per = (a.tiles + a.chunks - 1) / a.chunks;
   a.chunk = per * TT;
@@ -106,6 +114,7 @@ extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_b
                                        void* stream) {
   if (const int rc = check(p)) return rc;
   if (!g || !have(p) || !p->checkpoints || !workspace) return LQG_ERR_NULL;
+  if (g->dy.st < 0 || g->dy.st > MAX_STRIDE) return LQG_ERR_ARG;
   if (!g->dy.ptr || !g->du || !g->ddelta || !g->dBm || !g->dCm || (p->z.ptr && !g->dz)) return LQG_ERR_NULL;
   ScanArgs a = describe(p);
   a.g = *g;

@@ -20,7 +20,7 @@ constexpr float LN2 = 0.6931471805599453f;
 struct ScanArgs {
   lqg_selscan p;
   lqg_selscan_bars g;
-  long Dg, bpg, blocks;          // channels of a group, blocks of 64 of them, blocks in all
+  long Dg, bpg, blocks, ch;      // channels of a group, blocks of `ch` of them, blocks in all
   long chunks, chunk, tiles;     // chunks of the time axis, their steps (a multiple of TT), tiles of TT steps in T
   float *hl, *sd;                // carries [B][chunks][N][D], sums of dl [B][chunks][D]
   float *partB, *partC, *partP;  // gradients: [blocks][B][T][N] twice, [B * chunks][N + 2][D]
@@ -30,55 +30,140 @@ template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, lo
   return static_cast<const IT*>(s.ptr) + b * s.sb + off;
 }
 
-// where a workgroup is
-template <int NS, int TT> struct Place {
-  int lane, w;
-  long blk, b, c, grp, d, n0, len, t0, t1, tiles;
+// The shape of a workgroup: CH channels x NS NW 64 / CH states, TT steps a tile.
+template <int CH_, int NS_, int NW_, int TT_> struct Shape {
+  static constexpr int CH = CH_, NS = NS_, NW = NW_, TT = TT_;
+  static constexpr int LS = 64 / CH;          // groups of NS states in a wave
+  static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
+  static constexpr int R = TT / PS;           // elements of a tile (TT x CH) that a thread prepares and finishes: rows PS apart
+  static constexpr int Q = TT * NS / 16;      // registers of a tile's B (or C)
+  static_assert(TT % PS == 0 && TT * NS % 16 == 0 && CH % 16 == 0, "");
+};
+
+// where a thread is
+template <class S> struct Place {
+  int lane, tid, ch, n0, row, tiles, full;    // ch: its channel in the block (as lane and as thread: the same); row: its first row
+  long b, c, blk, grp, t0, t1, len;
+  unsigned d;                                 // its channel, repeated past the end of the group (`on` false: nothing is stored)
   bool on;
   __device__ Place(const ScanArgs& a) {
     lane = threadIdx.x;
-    w = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
-    blk = blockIdx.x % a.blocks;
-    const long rest = blockIdx.x / a.blocks;
-    c = rest % a.chunks;
-    b = rest / a.chunks;
-    grp = blk / a.bpg;
-    const long in = (blk % a.bpg) * 64 + lane;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
+    tid = w * 64 + lane;
+    ch = lane % S::CH;
+    n0 = (w * S::LS + lane / S::CH) * S::NS;
+    row = w * S::LS + lane / S::CH;
+    // Workgroups go to the 8 dies in turn; give each die neighbouring blocks, which share cache lines and the group's B and C.
+    const unsigned G = gridDim.x, x = blockIdx.x % 8, q = G / 8, r = G % 8;
+    const unsigned id = x * q + min(x, r) + blockIdx.x / 8;
+    blk = id % (unsigned)a.blocks;
+    const unsigned rest = id / (unsigned)a.blocks;
+    c = rest % (unsigned)a.chunks;
+    b = rest / (unsigned)a.chunks;
+    grp = (unsigned)blk / (unsigned)a.bpg;
+    const long in = (blk - grp * a.bpg) * S::CH + ch;
     on = in < a.Dg;
-    d = grp * a.Dg + (on ? in : a.Dg - 1);          // lanes past the group's end repeat its last channel and store nothing
-    n0 = w * NS;
+    d = (unsigned)(grp * a.Dg + (on ? in : a.Dg - 1));
     len = a.p.T;
     if (a.p.lengths) {
       const long l = a.p.lengths[b];
       len = l < 0 ? 0 : (l < len ? l : len);
     }
     t0 = c * a.chunk;
-    t1 = min(t0 + a.chunk, a.p.T);
-    const long end = min(t1, len);
-    tiles = end > t0 ? (end - t0 + TT - 1) / TT : 0;
+    t1 = min(t0 + a.chunk, (long)a.p.T);
+    const long live = min(t1, len) - t0;
+    tiles = live > 0 ? (int)((live + S::TT - 1) / S::TT) : 0;   // tiles that hold a step before the end
+    full = live > 0 ? (int)(live / S::TT) : 0;                  // and those that hold nothing else
   }
 };
 
-template <int NS> __device__ inline void load_A2(const ScanArgs& a, long d, long n0, float (&A2)[NS]) {
+template <class S> __device__ inline void load_A2(const ScanArgs& a, const Place<S>& at, float (&A2)[S::NS]) {
 #pragma unroll
-  for (int j = 0; j < NS; ++j) A2[j] = n0 + j < a.p.N ? load_param(a.p.A, d * a.p.N + n0 + j) * LOG2E : 0.0f;
+  for (int j = 0; j < S::NS; ++j) A2[j] = at.n0 + j < a.p.N ? load_param(a.p.A, at.d * a.p.N + at.n0 + j) * LOG2E : 0.0f;
 }
 
-// a tile's B or C: value (t, j) in register (t NS + j) / 16, lane (t NS + j) % 16 of each row; 0 behind the end and past N
-template <class IT, int NS, int TT>
-__device__ inline void load_bc(const lqg_seq& s, long b, long grp, long t0, long n0, long len, long N, int lane, float (&r)[TT * NS / 16]) {
+// One sequence of the workgroup's rows: a uniform pointer to the current tile, the thread's own offset in it (32 bits: strides are
+// below 2^25), rows PS apart.
+template <class IT, class S> struct Stream {
+  const IT* p;
+  unsigned off;
+  long st;
+  __device__ Stream(const lqg_seq& s, const Place<S>& at) : p(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st),
+      off((unsigned)(at.row * s.st) + at.d), st(s.st) {}
+  __device__ void tile(int i) { p += (long)i * S::TT * st; }
+  // rows of the tile `ahead` tiles on; a partial tile's rows behind the end are not read
+  __device__ void load(IT (&r)[S::R], int ahead, bool whole, long left, int row) const {
+    const IT* q = p + (long)ahead * S::TT * st;
+    if (whole) {
 #pragma unroll
-  for (int q = 0; q < TT * NS / 16; ++q) {
-    const int f = q * 16 + (lane & 15);
-    const long t = t0 + f / NS, n = n0 + f % NS;
-    r[q] = t < len && n < N ? up(seq<IT>(s, b, grp * s.sg)[t * s.st + n]) : 0.0f;
+      for (int i = 0; i < S::R; ++i) r[i] = (q + (long)i * S::PS * st)[off];
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::R; ++i) r[i] = row + i * S::PS < left ? (q + (long)i * S::PS * st)[off] : (IT)0.0f;
+    }
+  }
+};
+
+// a tile's B or C: value (t, j) of a lane's states in register (t NS + j) / 16, lane (t NS + j) % 16 of its row of 16
+template <class IT, class S> struct Maps {
+  const IT* p;
+  unsigned off;
+  long st;
+  int t;
+  bool ok[S::NS > 16 ? 2 : 1];
+  bool all;
+  __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : st(s.st) {
+    const int f = at.lane & 15, j = f % S::NS;
+    t = f / S::NS;
+    p = static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg;
+    ok[0] = at.n0 + j < a.p.N;
+    off = (unsigned)(t * s.st) + (ok[0] ? at.n0 + j : 0);
+  }
+  __device__ void tile(int i) { p += (long)i * S::TT * st; }
+  __device__ void load(IT (&r)[S::Q], int ahead, bool whole, long left) const {
+    const IT* q = p + (long)ahead * S::TT * st;
+    constexpr int step = 16 / S::NS;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < S::Q; ++i) r[i] = (q + (long)i * step * st)[off];
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::Q; ++i) r[i] = t + i * step < left ? (q + (long)i * step * st)[off] : (IT)0.0f;
+    }
+  }
+  __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q]) const {
+#pragma unroll
+    for (int i = 0; i < S::Q; ++i) v[i] = ok[0] ? up(r[i]) : 0.0f;
+  }
+};
+
+template <class S, int T, int J> __device__ inline float bc(const float (&r)[S::Q]) {
+  return row_bcast<(T * S::NS + J) % 16>(r[(T * S::NS + J) / 16]);
+}
+
+// y += sum_j bc(C)(t, j) h[j].  The broadcast is an operand modifier of the multiply-add, which the compiler does not fold there (it would
+// copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart from the broadcast's read.
+#define LQG_FMAC_BCAST(Y, C, K, X) "v_fmac_f32_dpp " Y ", " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
+template <class S, int T> __device__ inline void dot_bcast(float& y, const float (&C)[S::Q], const float (&h)[S::NS]) {
+  constexpr int f = T * S::NS, k = f % 16;
+  if constexpr (S::NS == 2) {
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c4", "%2") LQG_FMAC_BCAST("%0", "%1", "%c5", "%3")
+        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "n"(k), "n"(k + 1));
+  } else if constexpr (S::NS == 4) {
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
+        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
+        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k), "n"(k + 1), "n"(k + 2), "n"(k + 3));
+  } else {
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
+        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
+        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k), "n"(k + 1), "n"(k + 2), "n"(k + 3));
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
+        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
+        : "+v"(y) : "v"(C[f / 16]), "v"(h[4]), "v"(h[5]), "v"(h[6]), "v"(h[7]), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
   }
 }
-template <int NS, int T, int J, int Q> __device__ inline float bc(const float (&r)[Q]) {
-  return row_bcast<(T * NS + J) % 16>(r[(T * NS + J) / 16]);
-}
 
-// compile-time loop: f(integral_constant<int, I>) for I = 0 .. N-1
+// compile-time loop: f(Int<I>) for I = 0 .. N-1, or downwards
 template <int I> struct Int { static constexpr int v = I; };
 template <int N, int I = 0, class F> __device__ __forceinline__ void each(F&& f) {
   if constexpr (I < N) {
@@ -97,21 +182,24 @@ __device__ inline float step_size(const ScanArgs& a, float raw) { return a.p.sof
 
 // ------------------------------------------------------------------------------------------------ forward
 // CARRY: leave each chunk's end state from zero and its sum of dl instead of y.
-template <class IT, int NS, int NW, int TT, bool CARRY>
-__global__ __launch_bounds__(64 * NW) void k_scan(const ScanArgs a) {
-  constexpr int RW = TT / NW, Q = TT * NS / 16;
-  __shared__ float2 s_in[2][TT][64];
-  __shared__ float s_y[CARRY ? 1 : 2][CARRY ? 1 : TT][NW][64];
-  const Place<NS, TT> at(a);
-  const long D = a.p.D, N = a.p.N, d = at.d, b = at.b;
-  const int lane = at.lane, w = at.w;
+// Iteration i: finish tile i-1, prepare tile i+1, request tile i+2, walk tile i; one barrier.
+template <class IT, class S, bool CARRY>
+__global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
+  constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
+  __shared__ float2 s_in[2][TT][CH];                      // dl, dl u
+  __shared__ float2 s_out[2][CARRY ? 1 : TT][CH];         // D u, silu(z): read by the thread that wrote them
+  __shared__ float s_y[2][CARRY ? 1 : TT][PS][CH];
+  const Place<S> at(a);
+  const long D = a.p.D, N = a.p.N, b = at.b;
+  const unsigned d = at.d;
+  const int ch = at.ch, part = at.row;
   float A2[NS], h[NS], sum = 0.0f;
-  load_A2<NS>(a, d, at.n0, A2);
+  load_A2<S>(a, at, A2);
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     h[j] = !CARRY && a.p.state && at.n0 + j < N ? a.p.state[(b * D + d) * N + at.n0 + j] : 0.0f;
   if (!CARRY) {
-    for (long c = 0; c < at.c; ++c) {                   // the chunks before this one
+    for (long c = 0; c < at.c; ++c) {                     // the chunks before this one
       const float sd = a.sd[(b * a.chunks + c) * D + d];
       const float* hl = a.hl + ((b * a.chunks + c) * N + at.n0) * D + d;
 #pragma unroll
@@ -122,84 +210,98 @@ __global__ __launch_bounds__(64 * NW) void k_scan(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = !CARRY && a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = !CARRY && a.p.z.ptr;
-  struct Rows { IT u[RW], dl[RW], z[RW]; };
-  auto load = [&](Rows& r, long t0) {
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const long t = min(t0 + w * RW + i, at.len - 1);
-      r.u[i] = seq<IT>(a.p.u, b, t * a.p.u.st)[d];
-      r.dl[i] = seq<IT>(a.p.delta, b, t * a.p.delta.st)[d];
-      if (gate) r.z[i] = seq<IT>(a.p.z, b, t * a.p.z.st)[d];
-    }
+  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at);
+  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  IT ru[R], rdl[R], rz[R], rB[Q], rC[Q];
+  long left = at.len - at.t0;                             // steps before the end, from the current tile on
+  auto load = [&](int ahead, bool whole) {
+    su.load(ru, ahead, whole, left - ahead * TT, at.row);
+    sdl.load(rdl, ahead, whole, left - ahead * TT, at.row);
+    if (gate) sz.load(rz, ahead, whole, left - ahead * TT, at.row);
   };
-  auto prepare = [&](const Rows& r, long t0, int buf) {
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const bool live = t0 + w * RW + i < at.len;
-      const float dl = live ? step_size(a, up(r.dl[i]) + bias) : 0.0f;
-      s_in[buf][w * RW + i][lane] = make_float2(dl, live ? dl * up(r.u[i]) : 0.0f);
-    }
+  auto load_maps = [&](int ahead, bool whole) {
+    mB.load(rB, ahead, whole, left - ahead * TT);
+    if (!CARRY) mC.load(rC, ahead, whole, left - ahead * TT);
   };
-  IT* y = CARRY ? nullptr : const_cast<IT*>(seq<IT>(a.p.y, b, d));
-  auto finish = [&](const Rows& r, long t0, int buf) {
+  auto prepare = [&](int ahead, int buf) {
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const long t = t0 + w * RW + i;
-      float v = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) v += s_y[buf][w * RW + i][k][lane];
-      v = fmaf(Dk, up(r.u[i]), v);
-      if (gate) {
-        const float z = up(r.z[i]);
-        v *= z * sigmoid(z);
+    for (int i = 0; i < R; ++i) {
+      const int row = at.row + i * PS;
+      const bool live = row + ahead * TT < left;
+      const float u = up(ru[i]), dl = live ? step_size(a, up(rdl[i]) + bias) : 0.0f;
+      s_in[buf][row][ch] = make_float2(dl, live ? dl * u : 0.0f);
+      if (!CARRY) {
+        float g = 1.0f;
+        if (gate) {
+          const float z = up(rz[i]);
+          g = z * sigmoid(z);
+        }
+        s_out[buf][row][ch] = make_float2(Dk * u, g);
       }
-      if (t < at.t1 && at.on) y[t * a.p.y.st] = down<IT>(t < at.len ? v : 0.0f);
+    }
+  };
+  IT* y = CARRY ? nullptr : const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st;
+  const unsigned yoff = (unsigned)(at.row * a.p.y.st) + d;
+  auto finish = [&](IT* yt, long left, long room, int buf) {   // left: steps before the end, room: steps of the chunk, from this tile on
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int row = at.row + i * PS;
+      const float2 o = s_out[buf][row][ch];
+      float v = o.x;
+#pragma unroll
+      for (int k = 0; k < PS; ++k) v += s_y[buf][row][k][ch];
+      if (gate) v *= o.y;
+      if (row < room && at.on) (yt + (long)i * PS * a.p.y.st)[yoff] = down<IT>(row < left ? v : 0.0f);
     }
   };
 
-  Rows before, now, next, after;
-  float B[Q], C[Q], Bn[Q], Cn[Q];
+  float B[Q], C[Q];
   if (at.tiles > 0) {
-    load(now, at.t0);
-    load_bc<IT, NS, TT>(a.p.Bm, b, at.grp, at.t0, at.n0, at.len, N, lane, B);
-    if (!CARRY) load_bc<IT, NS, TT>(a.p.Cm, b, at.grp, at.t0, at.n0, at.len, N, lane, C);
-    prepare(now, at.t0, 0);
-    if (at.tiles > 1) load(next, at.t0 + TT);
+    load(0, at.full > 0);
+    load_maps(0, at.full > 0);
+    prepare(0, 0);
+    mB.widen(rB, B);
+    if (!CARRY) mC.widen(rC, C);
+    if (at.tiles > 1) load(1, at.full > 1);
   }
   __syncthreads();
-  for (long i = 0; i < at.tiles; ++i) {
-    const long t0 = at.t0 + i * TT;
-    const int buf = (int)(i & 1);
+  float* ck = !CARRY && a.p.checkpoints ? static_cast<float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT) * N + at.n0) * D + d : nullptr;
+  for (int i = 0; i < at.tiles; ++i) {
+    const int buf = i & 1;
+    if (!CARRY && i > 0) finish(y - TT * a.p.y.st, left + TT, left + TT + (at.t1 - at.len), buf ^ 1);
     if (i + 1 < at.tiles) {
-      prepare(next, t0 + TT, buf ^ 1);
-      load_bc<IT, NS, TT>(a.p.Bm, b, at.grp, t0 + TT, at.n0, at.len, N, lane, Bn);
-      if (!CARRY) load_bc<IT, NS, TT>(a.p.Cm, b, at.grp, t0 + TT, at.n0, at.len, N, lane, Cn);
+      prepare(1, buf ^ 1);
+      load_maps(1, i + 1 < at.full);
     }
-    if (i + 2 < at.tiles) load(after, t0 + 2 * TT);
-    if (!CARRY && a.p.checkpoints && at.on) {
-      float* ck = static_cast<float*>(a.p.checkpoints) + ((b * a.tiles + t0 / TT) * N + at.n0) * D + d;
+    if (i + 2 < at.tiles) load(2, i + 2 < at.full);
+    if (!CARRY && ck) {
 #pragma unroll
       for (int j = 0; j < NS; ++j)
-        if (at.n0 + j < N) ck[j * D] = h[j];
+        if (at.on && at.n0 + j < N) ck[j * D] = h[j];
+      ck += N * D;
     }
     each<TT>([&](auto tc) {
       constexpr int t = decltype(tc)::v;
-      const float2 in = s_in[buf][t][lane];
-      float v = 0.0f;
+      const float2 in = s_in[buf][t][ch];
       each<NS>([&](auto jc) {
         constexpr int j = decltype(jc)::v;
-        h[j] = fmaf(exp2_hw(in.x * A2[j]), h[j], bc<NS, t, j>(B) * in.y);
-        if (!CARRY) v = fmaf(bc<NS, t, j>(C), h[j], v);
+        h[j] = fmaf(exp2_hw(in.x * A2[j]), h[j], bc<S, t, j>(B) * in.y);
       });
-      if (CARRY) sum += in.x;
-      else s_y[buf][t][w][lane] = v;
+      if (CARRY) {
+        sum += in.x;
+      } else {
+        float v = 0.0f;
+        dot_bcast<S, t>(v, C, h);
+        s_y[buf][t][part][ch] = v;
+      }
     });
-    if (!CARRY && i > 0) finish(before, t0 - TT, buf ^ 1);
-    before = now;
-    now = next;
-    next = after;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) B[q] = Bn[q], C[q] = Cn[q];
+    if (i + 1 < at.tiles) {
+      mB.widen(rB, B);
+      if (!CARRY) mC.widen(rC, C);
+    }
+    su.tile(1), sdl.tile(1), sz.tile(1), mB.tile(1), mC.tile(1);
+    if (!CARRY) y += TT * a.p.y.st;
+    left -= TT;
     __syncthreads();
   }
   if (CARRY) {
@@ -208,12 +310,13 @@ __global__ __launch_bounds__(64 * NW) void k_scan(const ScanArgs a) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
       if (at.n0 + j < N) hl[j * D] = h[j];
-    if (w == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
+    if (at.row == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
     return;
   }
-  if (at.tiles > 0) finish(before, at.t0 + (at.tiles - 1) * TT, (int)((at.tiles - 1) & 1));
+  if (at.tiles > 0) finish(y - TT * a.p.y.st, left + TT, left + TT + (at.t1 - at.len), (at.tiles - 1) & 1);
   if (!at.on) return;
-  for (long t = at.t0 + at.tiles * TT + w; t < at.t1; t += NW) y[t * a.p.y.st] = down<IT>(0.0f);
+  for (long t = at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS)       // padding behind the last tile
+    (y + (t - at.tiles * TT) * a.p.y.st)[d] = down<IT>(0.0f);
   if (a.p.state_out && at.c == a.chunks - 1) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
@@ -241,27 +344,79 @@ template <int BIT> __device__ inline float merge(float x, float y, int lane) {
     return keep + dpp<BIT == 3 ? DPP_ROR8 : BIT == 2 ? DPP_HALF_MIRROR : BIT == 1 ? DPP_XOR2 : DPP_XOR1>(give);
   }
 }
+constexpr int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
+
+// dB and dC: 2 NS values of each step, summed over the CH channels of a wave.  A tree of merges over the lane bits of the channel: bits
+// of the step on the upper ones, bits of the value on the lower, so that one sum ends in each lane: 2 instructions a value and not 12.
+template <class S> struct ChannelSum {
+  static constexpr int K = 2 * S::NS, KG = K < 8 ? K : 8;                   // values of a step, of a group that ends together
+  static constexpr int TB = log2_of(S::CH) - log2_of(KG), TG = 1 << TB;     // bits of the step in the tree, steps of a tree
+  float held[TB][K];
+  // v: the values of step T (steps come downwards); true when the tree of steps T .. T + TG - 1 is whole: out has K / KG sums
+  template <int T> __device__ bool add(float (&v)[K], int lane, float (&out)[K / KG]) {
+    return level<T, 0>(v, lane, out);
+  }
+  template <int T, int L> __device__ bool level(float (&v)[K], int lane, float (&out)[K / KG]) {
+    if constexpr (L == TB) {
+#pragma unroll
+      for (int o = 0; o < K / KG; ++o) {
+        float x[KG];
+#pragma unroll
+        for (int k = 0; k < KG; ++k) x[k] = v[o * KG + k];
+        values<KG>(x, lane);
+        out[o] = x[0];
+      }
+      return true;
+    } else if constexpr (T >> L & 1) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) held[L][k] = v[k];
+      return false;
+    } else {
+      constexpr int BIT = log2_of(S::CH) - 1 - L;
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = merge<BIT>(v[k], held[L][k], lane);
+      return level<T, L + 1>(v, lane, out);
+    }
+  }
+  template <int M> __device__ static void values(float (&x)[KG], int lane) {
+    if constexpr (M > 1) {
+#pragma unroll
+      for (int k = 0; k < M / 2; ++k) x[k] = merge<log2_of(M) - 1>(x[k], x[k + M / 2], lane);
+      values<M / 2>(x, lane);
+    }
+  }
+  // which step (from the tree's first) and which value of a group a lane ends with
+  __device__ static int step_of(int lane) {
+    int t = 0;
+#pragma unroll
+    for (int l = 0; l < TB; ++l) t |= (lane >> (log2_of(S::CH) - 1 - l) & 1) << l;
+    return t;
+  }
+  __device__ static int value_of(int lane) { return lane & (KG - 1); }
+};
 
 // CARRY: leave each chunk's carry (lambda at its start from 0 at its end) and its sum of dl.
-template <class IT, int NS, int NW, int TT, bool CARRY>
-__global__ __launch_bounds__(64 * NW) void k_scan_grad(const ScanArgs a) {
-  constexpr int RW = TT / NW, Q = TT * NS / 16;
-  __shared__ float2 s_in[2][TT][64];
-  __shared__ float s_dy[2][TT][64];
-  __shared__ float2 s_sum[CARRY ? 1 : TT][NW][64];
-  __shared__ float s_y[CARRY ? 1 : TT][NW][64];
-  const Place<NS, TT> at(a);
-  const long D = a.p.D, N = a.p.N, T = a.p.T, d = at.d, b = at.b;
-  const int lane = at.lane, w = at.w;
+template <class IT, class S, bool CARRY>
+__global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
+  constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
+  __shared__ float2 s_in[2][TT][CH];                      // dl, dl u
+  __shared__ float s_dy[2][TT][CH];                       // dY
+  __shared__ float s_own[3][CARRY ? 1 : TT][CH];          // u, d dl / d delta, dy silu'(z): read by the thread that wrote them
+  __shared__ float2 s_sum[CARRY ? 1 : TT][PS][CH];        // s1, s2
+  __shared__ float s_y[CARRY ? 1 : TT][PS][CH];
+  const Place<S> at(a);
+  const long D = a.p.D, N = a.p.N, T = a.p.T, b = at.b;
+  const unsigned d = at.d;
+  const int lane = at.lane, ch = at.ch, part = at.row;
   float A2[NS], lam[NS], dA[NS], sum = 0.0f, dDk = 0.0f, dbias = 0.0f;
-  load_A2<NS>(a, d, at.n0, A2);
+  load_A2<S>(a, at, A2);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     dA[j] = 0.0f;
     lam[j] = !CARRY && a.g.dstate_out && at.n0 + j < N ? a.g.dstate_out[(b * D + d) * N + at.n0 + j] : 0.0f;
   }
   if (!CARRY) {
-    for (long c = a.chunks - 1; c > at.c; --c) {        // the chunks after this one
+    for (long c = a.chunks - 1; c > at.c; --c) {          // the chunks after this one
       const float sd = a.sd[(b * a.chunks + c) * D + d];
       const float* hl = a.hl + ((b * a.chunks + c) * N + at.n0) * D + d;
 #pragma unroll
@@ -272,166 +427,168 @@ __global__ __launch_bounds__(64 * NW) void k_scan_grad(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = a.p.z.ptr;
-  struct Rows { IT u[RW], dl[RW], z[RW], dy[RW]; };
-  auto load = [&](Rows& r, long t0) {
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const long t = min(t0 + w * RW + i, at.len - 1);
-      r.u[i] = seq<IT>(a.p.u, b, t * a.p.u.st)[d];
-      r.dl[i] = seq<IT>(a.p.delta, b, t * a.p.delta.st)[d];
-      r.dy[i] = seq<IT>(a.g.dy, b, t * a.g.dy.st)[d];
-      if (gate) r.z[i] = seq<IT>(a.p.z, b, t * a.p.z.st)[d];
-    }
+  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at), sdy(a.g.dy, at);
+  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  IT ru[R], rdl[R], rz[R], rdy[R], rB[Q], rC[Q];
+  const int last = at.tiles - 1;
+  su.tile(last), sdl.tile(last), sz.tile(last), sdy.tile(last), mB.tile(last), mC.tile(last);
+  long left = at.len - at.t0 - (long)last * TT;           // steps before the end, from the current tile on
+  auto load = [&](int ahead, bool whole) {
+    su.load(ru, ahead, whole, left - ahead * TT, at.row);
+    sdl.load(rdl, ahead, whole, left - ahead * TT, at.row);
+    sdy.load(rdy, ahead, whole, left - ahead * TT, at.row);
+    if (gate) sz.load(rz, ahead, whole, left - ahead * TT, at.row);
   };
-  auto prepare = [&](const Rows& r, long t0, int buf) {
+  auto load_maps = [&](int ahead, bool whole) {
+    mC.load(rC, ahead, whole, left - ahead * TT);
+    if (!CARRY) mB.load(rB, ahead, whole, left - ahead * TT);
+  };
+  auto prepare = [&](int ahead, int buf) {
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const bool live = t0 + w * RW + i < at.len && at.on;
-      const float dl = live ? step_size(a, up(r.dl[i]) + bias) : 0.0f;
-      float dy = up(r.dy[i]);
+    for (int i = 0; i < R; ++i) {
+      const int row = at.row + i * PS;
+      const bool live = row + ahead * TT < left && at.on;
+      const float raw = up(rdl[i]) + bias, dl = live ? step_size(a, raw) : 0.0f, u = up(ru[i]), dy = up(rdy[i]);
+      float dY = dy, dg = 0.0f;
       if (gate) {
-        const float z = up(r.z[i]);
-        dy *= z * sigmoid(z);
+        const float z = up(rz[i]), sg = sigmoid(z);
+        dY *= z * sg;
+        dg = dy * (sg * fmaf(z, 1.0f - sg, 1.0f));
       }
-      s_in[buf][w * RW + i][lane] = make_float2(dl, live ? dl * up(r.u[i]) : 0.0f);
-      s_dy[buf][w * RW + i][lane] = live ? dy : 0.0f;
+      s_in[buf][row][ch] = make_float2(dl, live ? dl * u : 0.0f);
+      s_dy[buf][row][ch] = live ? dY : 0.0f;
+      if (!CARRY) {
+        s_own[0][row][ch] = u;
+        s_own[1][row][ch] = a.p.softplus ? sigmoid(raw) : 1.0f;
+        s_own[2][row][ch] = dg;
+      }
     }
   };
-  const long out0 = b * T * D + d;
-  auto finish = [&](const Rows& r, long t0, int buf) {
+  IT* du = static_cast<IT*>(a.g.du) + (b * T + at.t0 + (long)last * TT) * D;
+  IT* ddelta = static_cast<IT*>(a.g.ddelta) + (b * T + at.t0 + (long)last * TT) * D;
+  IT* dz = static_cast<IT*>(a.g.dz) + (gate ? (b * T + at.t0 + (long)last * TT) * D : 0);
+  const unsigned ooff = (unsigned)(at.row * D) + d;
+  auto finish = [&](int buf) {
+    const long room = left + (at.t1 - at.len);
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int row = w * RW + i;
-      const long t = t0 + row;
+    for (int i = 0; i < R; ++i) {
+      const int row = at.row + i * PS;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        const float2 s = s_sum[row][k][lane];
+      for (int k = 0; k < PS; ++k) {
+        const float2 s = s_sum[row][k][ch];
         s1 += s.x;
         s2 += s.y;
       }
-      const float dl = s_in[buf][row][lane].x, dY = s_dy[buf][row][lane], u = up(r.u[i]);
-      const bool live = t < at.len;
-      float ddl = fmaf(u, s1, LN2 * s2);
-      if (a.p.softplus) ddl *= sigmoid(up(r.dl[i]) + bias);
+      const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[0][row][ch];
+      const bool live = row < left, store = row < room && at.on;
+      const float ddl = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
       if (live && at.on) {
         dDk = fmaf(dY, u, dDk);
         dbias += ddl;
       }
-      if (t < at.t1 && at.on) {
-        static_cast<IT*>(a.g.du)[out0 + t * D] = down<IT>(live ? fmaf(dl, s1, Dk * dY) : 0.0f);
-        static_cast<IT*>(a.g.ddelta)[out0 + t * D] = down<IT>(live ? ddl : 0.0f);
+      const long o = (long)i * PS * D;
+      if (store) {
+        (du + o)[ooff] = down<IT>(live ? fmaf(dl, s1, Dk * dY) : 0.0f);
+        (ddelta + o)[ooff] = down<IT>(live ? ddl : 0.0f);
       }
       if (gate) {
         float y = Dk * u;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) y += s_y[row][k][lane];
-        const float z = up(r.z[i]), sg = sigmoid(z);
-        const float dz = up(r.dy[i]) * y * (sg * fmaf(z, 1.0f - sg, 1.0f));
-        if (t < at.t1 && at.on) static_cast<IT*>(a.g.dz)[out0 + t * D] = down<IT>(live ? dz : 0.0f);
+        for (int k = 0; k < PS; ++k) y += s_y[row][k][ch];
+        if (store) (dz + o)[ooff] = down<IT>(live ? y * s_own[2][row][ch] : 0.0f);
       }
     }
   };
 
-  const float* ck = CARRY ? nullptr : static_cast<const float*>(a.p.checkpoints) + (b * a.tiles * N + at.n0) * D + d;
-  Rows now, next;
-  float B[Q], C[Q], h0[NS];
-  auto load_tile = [&](long t0) {
-    load_bc<IT, NS, TT>(a.p.Cm, b, at.grp, t0, at.n0, at.len, N, lane, C);
-    if (CARRY) return;
-    load_bc<IT, NS, TT>(a.p.Bm, b, at.grp, t0, at.n0, at.len, N, lane, B);
+  const float* ck = CARRY ? nullptr : static_cast<const float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT + last) * N + at.n0) * D + d;
+  float B[Q], C[Q], h0[NS], hn[NS];
+  auto load_ck = [&](const float* p) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) h0[j] = at.n0 + j < N ? ck[((t0 / TT) * N + j) * D] : 0.0f;
+    for (int j = 0; j < NS; ++j) hn[j] = at.n0 + j < N ? p[j * D] : 0.0f;
   };
   if (at.tiles > 0) {
-    load(now, at.t0 + (at.tiles - 1) * TT);
-    prepare(now, at.t0 + (at.tiles - 1) * TT, (int)((at.tiles - 1) & 1));
+    load(0, last < at.full);
+    load_maps(0, last < at.full);
+    if (!CARRY) load_ck(ck);
+    prepare(0, last & 1);
+    mC.widen(rC, C);
+    if (!CARRY) {
+      mB.widen(rB, B);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) h0[j] = hn[j];
+    }
+    if (last > 0) load(-1, true);
   }
   __syncthreads();
-  for (long i = at.tiles - 1; i >= 0; --i) {
-    const long t0 = at.t0 + i * TT;
-    const int buf = (int)(i & 1);
-    load_tile(t0);
-    if (i > 0) load(next, t0 - TT);
+  float *pB = nullptr, *pC = nullptr;
+  if (!CARRY) {
+    const long o = ((at.blk * a.p.B + b) * T + at.t0 + (long)last * TT) * N;
+    pB = a.partB + o, pC = a.partC + o;
+  }
+  for (int i = last; i >= 0; --i) {
+    const int buf = i & 1;
+    if (i > 0) {
+      load_maps(-1, true);
+      if (!CARRY) load_ck(ck - N * D);
+    }
     if constexpr (CARRY) {
       each_back<TT - 1>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float dl = s_in[buf][t][lane].x, dY = s_dy[buf][t][lane];
+        const float dl = s_in[buf][t][ch].x, dY = s_dy[buf][t][ch];
         sum += dl;
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
-          lam[j] = exp2_hw(dl * A2[j]) * fmaf(bc<NS, t, j>(C), dY, lam[j]);
+          lam[j] = exp2_hw(dl * A2[j]) * fmaf(bc<S, t, j>(C), dY, lam[j]);
         });
       });
     } else {
       float hh[TT][NS], aa[TT][NS];
       each<TT>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float2 in = s_in[buf][t][lane];
-        float y = 0.0f;
+        const float2 in = s_in[buf][t][ch];
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
           aa[t][j] = exp2_hw(in.x * A2[j]);
-          hh[t][j] = fmaf(aa[t][j], t ? hh[t ? t - 1 : 0][j] : h0[j], bc<NS, t, j>(B) * in.y);
-          if (gate) y = fmaf(bc<NS, t, j>(C), hh[t][j], y);
+          hh[t][j] = fmaf(aa[t][j], t ? hh[t ? t - 1 : 0][j] : h0[j], bc<S, t, j>(B) * in.y);
         });
-        if (gate) s_y[t][w][lane] = y;
+        if (gate) {
+          float y = 0.0f;
+          dot_bcast<S, t>(y, C, hh[t]);
+          s_y[t][part][ch] = y;
+        }
       });
       float tA[NS];
 #pragma unroll
       for (int j = 0; j < NS; ++j) tA[j] = 0.0f;
-      // dB, dC of 8 steps x 8 values end as one value per lane: step bits on lane bits 5, 4, 3, value bits on 2, 1, 0
-      constexpr int K = 2 * NS;
-      float p0[K], p1[K], p2[K];
+      ChannelSum<S> sums;
       each_back<TT - 1>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float2 in = s_in[buf][t][lane];
-        const float dY = s_dy[buf][t][lane];
-        float v[K], s1 = 0.0f, s2 = 0.0f;
+        const float2 in = s_in[buf][t][ch];
+        const float dY = s_dy[buf][t][ch];
+        float v[2 * NS], gg[NS], s1 = 0.0f, s2 = 0.0f;
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
-          const float g = fmaf(bc<NS, t, j>(C), dY, lam[j]);
+          const float g = fmaf(bc<S, t, j>(C), dY, lam[j]);
+          gg[j] = g;
           v[j] = g * in.y;
           v[NS + j] = dY * hh[t][j];
-          s1 = fmaf(bc<NS, t, j>(B), g, s1);
           lam[j] = aa[t][j] * g;
           const float q = lam[j] * (t ? hh[t ? t - 1 : 0][j] : h0[j]);
           s2 = fmaf(A2[j], q, s2);
           tA[j] = fmaf(q, in.x, tA[j]);
         });
-        s_sum[t][w][lane] = make_float2(s1, s2);
-        if constexpr (t & 1) {
+        dot_bcast<S, t>(s1, B, gg);
+        s_sum[t][part][ch] = make_float2(s1, s2);
+        using CS = ChannelSum<S>;
+        float out[CS::K / CS::KG];
+        if (sums.template add<t>(v, lane, out)) {
+          const int ts = t + CS::step_of(lane);
+          if (ts < left + (at.t1 - at.len)) {
 #pragma unroll
-          for (int k = 0; k < K; ++k) p0[k] = v[k];
-        } else {
-#pragma unroll
-          for (int k = 0; k < K; ++k) v[k] = merge<5>(v[k], p0[k], lane);
-          if constexpr (t & 2) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) p1[k] = v[k];
-          } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] = merge<4>(v[k], p1[k], lane);
-            if constexpr (t & 4) {
-#pragma unroll
-              for (int k = 0; k < K; ++k) p2[k] = v[k];
-            } else {
-#pragma unroll
-              for (int k = 0; k < K; ++k) v[k] = merge<3>(v[k], p2[k], lane);
-#pragma unroll
-              for (int o = 0; o < K; o += 8) {
-                float x[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = merge<2>(v[o + k], v[o + k + 4], lane);
-                x[0] = merge<1>(x[0], x[2], lane);
-                x[1] = merge<1>(x[1], x[3], lane);
-                x[0] = merge<0>(x[0], x[1], lane);
-                const int k = o + (lane & 4) + (lane & 1) * 1 + (lane & 2);
-                const long ts = t0 + t + (lane >> 5 & 1) + (lane >> 4 & 1) * 2 + (lane >> 3 & 1) * 4;
-                const long n = at.n0 + k % NS;
-                float* part = k < NS ? a.partB : a.partC;
-                if (ts < at.t1 && n < N) part[((at.blk * a.p.B + b) * T + ts) * N + n] = x[0];
-              }
+            for (int o = 0; o < CS::K / CS::KG; ++o) {
+              const int k = o * CS::KG + CS::value_of(lane), n = at.n0 + k % NS;
+              if (n < N) (k < NS ? pB : pC)[(unsigned)(ts * (int)N + n)] = out[o];
             }
           }
         }
@@ -439,16 +596,25 @@ __global__ __launch_bounds__(64 * NW) void k_scan_grad(const ScanArgs a) {
 #pragma unroll
       for (int j = 0; j < NS; ++j) dA[j] += tA[j];
     }
-    if constexpr (CARRY) {
-      if (i > 0) prepare(next, t0 - TT, buf ^ 1);
-      __syncthreads();
-    } else {
-      __syncthreads();
-      finish(now, t0, buf);
-      if (i > 0) prepare(next, t0 - TT, buf ^ 1);
-      now = next;
-      __syncthreads();
+    __syncthreads();
+    if (!CARRY) finish(buf);
+    if (i > 0) {
+      prepare(-1, buf ^ 1);
+      if (i > 1) load(-2, true);
+      mC.widen(rC, C);
+      if (!CARRY) {
+        mB.widen(rB, B);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) h0[j] = hn[j];
+      }
     }
+    su.tile(-1), sdl.tile(-1), sz.tile(-1), sdy.tile(-1), mB.tile(-1), mC.tile(-1);
+    left += TT;
+    if (!CARRY) {
+      du -= TT * D, ddelta -= TT * D, pB -= TT * N, pC -= TT * N, ck -= N * D;
+      if (gate) dz -= TT * D;
+    }
+    __syncthreads();
   }
   if constexpr (CARRY) {
     if (!at.on) return;
@@ -456,30 +622,30 @@ __global__ __launch_bounds__(64 * NW) void k_scan_grad(const ScanArgs a) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
       if (at.n0 + j < N) hl[j * D] = lam[j];
-    if (w == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
+    if (at.row == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
   } else {
-    for (long t = at.t0 + at.tiles * TT + w; t < at.t1; t += NW) {       // padding
-      if (!at.on) break;
+    const long out0 = b * T * D + d;
+    for (long t = at.t0 + (long)at.tiles * TT + at.row; t < at.t1 && at.on; t += PS) {       // padding
       static_cast<IT*>(a.g.du)[out0 + t * D] = down<IT>(0.0f);
       static_cast<IT*>(a.g.ddelta)[out0 + t * D] = down<IT>(0.0f);
       if (gate) static_cast<IT*>(a.g.dz)[out0 + t * D] = down<IT>(0.0f);
     }
-    s_sum[0][w][lane] = make_float2(dDk, dbias);
+    s_sum[0][part][ch] = make_float2(dDk, dbias);
     __syncthreads();
     if (!at.on) return;
-    float* part = a.partP + (b * a.chunks + at.c) * (N + 2) * D + d;
+    float* out = a.partP + (b * a.chunks + at.c) * (N + 2) * D + d;
 #pragma unroll
     for (int j = 0; j < NS; ++j)
       if (at.n0 + j < N) {
-        part[(at.n0 + j) * D] = dA[j];
+        out[(at.n0 + j) * D] = dA[j];
         if (a.g.dstate && at.c == 0) a.g.dstate[(b * D + d) * N + at.n0 + j] = lam[j];
       }
-    if (w == 0) {
+    if (at.row == 0) {
       float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int k = 0; k < NW; ++k) s.x += s_sum[0][k][lane].x, s.y += s_sum[0][k][lane].y;
-      part[N * D] = s.x;
-      part[(N + 1) * D] = s.y;
+      for (int k = 0; k < PS; ++k) s.x += s_sum[0][k][ch].x, s.y += s_sum[0][k][ch].y;
+      out[N * D] = s.x;
+      out[(N + 1) * D] = s.y;
     }
   }
 }
@@ -540,31 +706,41 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* stat
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-inline int waves_of(long N) { return N > 16 ? 8 : N > 8 ? 4 : N > 4 ? 2 : 1; }
-
-template <class IT, int NS, int NW, int TT> int launch(int what, const ScanArgs& a, hipStream_t st) {
+template <class IT, class S> int launch(int what, const ScanArgs& a, hipStream_t st) {
   const long groups = a.blocks * a.chunks * a.p.B;
-  if (!grid_fits(groups, 64 * NW)) return LQG_ERR_ARG;
-  const dim3 g((unsigned)groups), t(64, NW);
+  if (!grid_fits(groups, 64 * S::NW)) return LQG_ERR_ARG;
+  const dim3 g((unsigned)groups), t(64, S::NW);
   if (what == 0) {
-    if (a.chunks > 1) hipLaunchKernelGGL((k_scan<IT, NS, NW, TT, true>), g, t, 0, st, a);
-    hipLaunchKernelGGL((k_scan<IT, NS, NW, TT, false>), g, t, 0, st, a);
+    if (a.chunks > 1) hipLaunchKernelGGL((k_scan<IT, S, true>), g, t, 0, st, a);
+    hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
   } else {
-    if (a.chunks > 1) hipLaunchKernelGGL((k_scan_grad<IT, NS, NW, TT, true>), g, t, 0, st, a);
-    hipLaunchKernelGGL((k_scan_grad<IT, NS, NW, TT, false>), g, t, 0, st, a);
+    if (a.chunks > 1) hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
+    hipLaunchKernelGGL((k_scan_grad<IT, S, false>), g, t, 0, st, a);
   }
   return (int)last();
 }
 
 template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
-  if (a.p.N > 32) return launch<IT, 8, 8, 8>(what, a, st);
-  switch (waves_of(a.p.N)) {
-    case 1: return launch<IT, 4, 1, 16>(what, a, st);
-    case 2: return launch<IT, 4, 2, 16>(what, a, st);
-    case 4: return launch<IT, 4, 4, 16>(what, a, st);
-    default: return launch<IT, 4, 8, 16>(what, a, st);
+  const long N = a.p.N;
+  if (N > 32) return launch<IT, Shape<64, 8, 8, 8>>(what, a, st);
+  if (N > 16) return launch<IT, Shape<64, 4, 8, 16>>(what, a, st);
+#ifdef NS4
+  if (N > 8) return launch<IT, Shape<64, 4, 4, 16>>(what, a, st);
+  if (N > 4) return launch<IT, Shape<64, 4, 2, 16>>(what, a, st);
+  return launch<IT, Shape<64, 4, 1, 16>>(what, a, st);
+#else
+  if (a.ch == 32) {
+    if (N > 8) return launch<IT, Shape<32, 2, 4, 16>>(what, a, st);
+    if (N > 4) return launch<IT, Shape<32, 2, 2, 16>>(what, a, st);
+    return launch<IT, Shape<32, 2, 1, 16>>(what, a, st);
   }
+  if (N > 8) return launch<IT, Shape<64, 2, 8, 16>>(what, a, st);
+  if (N > 4) return launch<IT, Shape<64, 2, 4, 16>>(what, a, st);
+  if (N > 2) return launch<IT, Shape<64, 2, 2, 16>>(what, a, st);
+  return launch<IT, Shape<64, 2, 1, 16>>(what, a, st);
+#endif
 }
+
 template <class IT> int launch_step(ScanArgs a, float* state, hipStream_t st) {
   const int lpc = a.p.N > 32 ? 16 : a.p.N > 16 ? 8 : a.p.N > 8 ? 4 : a.p.N > 4 ? 2 : 1;
   a.blocks = (a.p.D * lpc + 255) / 256;
