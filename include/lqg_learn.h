@@ -51,7 +51,7 @@ int lqg_causal_conv_step(const lqg_conv* p, void* stream);
  *   dl = delta + delta_bias, through softplus if asked;   h_t = exp(dl_t A) h_{t-1} + dl_t B_t u_t;
  *   y_t = (sum_n C_t h_t + D u_t) [* silu(z_t)]
  * A [D][N]; B, C [batch][time][G][N], group g serves channels g D/G ..; state [B][D][N] float or NULL (zeros).
- * Time strides of at most 2^25.  Padding as above: y is 0 and h stays.  state_out [B][D][N] float or NULL.
+ * D and time strides below 2^22.  Padding as above: y is 0 and h stays.  state_out [B][D][N] float or NULL.
  * checkpoints (or NULL): lqg_scan_checkpoint_bytes of memory that lqg_selective_scan_grad reads.
  */
 typedef struct lqg_selscan {

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from lqg_amd import _abi, _learn, options
 from lqg_amd._abi import LqgHipError
 
-MAX_WIDTH, MAX_STATES, MAX_STRIDE = 8, 64, 1 << 25
+MAX_WIDTH, MAX_STATES, MAX_STRIDE = 8, 64, (1 << 22) - 1
 
 
 def _need(ok, what):

@@ -37,22 +37,13 @@ __device__ inline float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 // 1 / (1 + e^-x)
 __device__ inline float sigmoid(float x) { return rcp_hw(1.0f + exp2_hw(-LOG2E * x)); }
 
-// softplus(x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1].  The logarithm as 2 atanh(s), s = e / (2 + e) <= 1/3: its series in s^2
-// keeps the RELATIVE error at a few ulp for small e too (time constants of 1000 steps are x = -7), where log of the rounded 1 + e
-// keeps only the absolute one.  First dropped term: s^18 / 19 <= 1.4e-10 of the sum.
+// softplus(x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1].  w = 1 + e is rounded: what that drops, c = e - (w - 1) (exact), comes back as
+// log(1 + e) = log(w) + c / w - .. ~ log(w) + c (c is 0 or w's half step: leaving the 1 / w out costs a quarter of an ulp), so the RELATIVE
+// error stays at a few ulp for small e too: time constants of 1000 steps are x = -7.  A NaN reaches e.
 __device__ inline float softplus(float x) {
   const float e = exp2_hw(-LOG2E * fabsf(x));
-  const float s = e * rcp_hw(2.0f + e), q = s * s;
-  float p = 1.0f / 17.0f;
-  p = fmaf(p, q, 1.0f / 15.0f);
-  p = fmaf(p, q, 1.0f / 13.0f);
-  p = fmaf(p, q, 1.0f / 11.0f);
-  p = fmaf(p, q, 1.0f / 9.0f);
-  p = fmaf(p, q, 1.0f / 7.0f);
-  p = fmaf(p, q, 1.0f / 5.0f);
-  p = fmaf(p, q, 1.0f / 3.0f);
-  const float l = 2.0f * fmaf(s * q, p, s);
-  return x != x ? x : fmaxf(x, 0.0f) + l;       // (fmaxf drops a NaN)
+  const float w = 1.0f + e, c = e - (w - 1.0f);
+  return fmaxf(x, 0.0f) + fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, c);
 }
 
 // lane K of each row of 16 lanes, in all lanes of that row: a modifier of the consuming instruction's operand, no instruction of its own

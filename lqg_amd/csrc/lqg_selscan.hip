@@ -29,12 +29,12 @@ X(float) X(bf16) X(f16)
 
 namespace {
 
-constexpr int64_t MAX_STRIDE = 1 << 25;       // rows of a tile are addressed by 32-bit offsets: 16 x 2^25 x 4 bytes
+constexpr int64_t MAX_STRIDE = (1 << 22) - 1;  // rows of a tile are at 32-bit byte offsets, products of 24-bit numbers
 
 int check(const lqg_selscan* p) {
   if (!p) return LQG_ERR_NULL;
   if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
-  if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > (1L << 24) || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
+  if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > MAX_STRIDE || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
   if (p->chunks < 0 || p->chunks > 64 || (p->channels != 0 && p->channels != 32 && p->channels != 64)) return LQG_ERR_ARG;
   for (const lqg_seq* q : {&p->u, &p->delta, &p->z, &p->Bm, &p->Cm, &p->y})
     if (q->st < 0 || q->st > MAX_STRIDE) return LQG_ERR_ARG;

@@ -82,24 +82,31 @@ template <class S> __device__ inline void load_A2(const ScanArgs& a, const Place
   for (int j = 0; j < S::NS; ++j) A2[j] = at.n0 + j < a.p.N ? load_param(a.p.A, at.d * a.p.N + at.n0 + j) * LOG2E : 0.0f;
 }
 
-// One sequence of the workgroup's rows: a uniform pointer to the current tile, the thread's own offset in it (32 bits: strides are
-// below 2^25), rows PS apart.
+// Row t of a tile is read at a uniform pointer plus a 32-bit offset of the thread, in bytes (row strides are below 2^24 of them).  Both
+// ways of a load issue the same number of instructions, so that the counter of outstanding loads can be waited on exactly: loads run two
+// tiles ahead and a wait for one tile's must not wait for the next one's.
+template <class IT> __device__ inline IT at_byte(const IT* p, unsigned off) {
+  return *reinterpret_cast<const IT*>(reinterpret_cast<const char*>(p) + off);
+}
+
+// One sequence: R rows of the thread in each tile, PS apart.
 template <class IT, class S> struct Stream {
-  const IT* p;
-  unsigned off;
-  long st;
-  __device__ Stream(const lqg_seq& s, const Place<S>& at) : p(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st),
-      off((unsigned)(at.row * s.st) + at.d), st(s.st) {}
-  __device__ void tile(int i) { p += (long)i * S::TT * st; }
-  // rows of the tile `ahead` tiles on; a partial tile's rows behind the end are not read
-  __device__ void load(IT (&r)[S::R], int ahead, bool whole, long left, int row) const {
-    const IT* q = p + (long)ahead * S::TT * st;
-    if (whole) {
+  const IT* p;                                // the chunk's first row
+  unsigned off, step;                         // the thread's first row and channel; bytes of a row
+  __device__ Stream(const lqg_seq& s, const Place<S>& at)
+      : p(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st), off(__umul24(at.row, (unsigned)s.st * sizeof(IT)) + at.d * (unsigned)sizeof(IT)),
+        step((unsigned)s.st * sizeof(IT)) {}
+  __device__ const IT* tile(int k) const { return reinterpret_cast<const IT*>(reinterpret_cast<const char*>(p) + (long)k * S::TT * step); }
+  // tile k; left: steps before the end from its first row on (>= 1): rows behind the end repeat the last one
+  __device__ void load(IT (&r)[S::R], int k, long left, const Place<S>& at) const {
+    const IT* q = tile(k);
+    if (left >= S::TT) {
 #pragma unroll
-      for (int i = 0; i < S::R; ++i) r[i] = (q + (long)i * S::PS * st)[off];
+      for (int i = 0; i < S::R; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(reinterpret_cast<const char*>(q) + (long)i * S::PS * step), off);
     } else {
 #pragma unroll
-      for (int i = 0; i < S::R; ++i) r[i] = row + i * S::PS < left ? (q + (long)i * S::PS * st)[off] : (IT)0.0f;
+      for (int i = 0; i < S::R; ++i)
+        r[i] = at_byte(q, __umul24(min(at.row + i * S::PS, (int)left - 1), step) + at.d * (unsigned)sizeof(IT));
     }
   }
 };
@@ -107,33 +114,38 @@ template <class IT, class S> struct Stream {
 // a tile's B or C: value (t, j) of a lane's states in register (t NS + j) / 16, lane (t NS + j) % 16 of its row of 16
 template <class IT, class S> struct Maps {
   const IT* p;
-  unsigned off;
-  long st;
+  unsigned off, step, n;
   int t;
-  bool ok[S::NS > 16 ? 2 : 1];
-  bool all;
-  __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : st(s.st) {
+  bool ok;
+  __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : step((unsigned)s.st * sizeof(IT)) {
     const int f = at.lane & 15, j = f % S::NS;
     t = f / S::NS;
     p = static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg;
-    ok[0] = at.n0 + j < a.p.N;
-    off = (unsigned)(t * s.st) + (ok[0] ? at.n0 + j : 0);
+    ok = at.n0 + j < a.p.N;
+    n = (ok ? at.n0 + j : 0) * sizeof(IT);
+    off = __umul24(t, step) + n;
   }
-  __device__ void tile(int i) { p += (long)i * S::TT * st; }
-  __device__ void load(IT (&r)[S::Q], int ahead, bool whole, long left) const {
-    const IT* q = p + (long)ahead * S::TT * st;
-    constexpr int step = 16 / S::NS;
-    if (whole) {
+  __device__ void load(IT (&r)[S::Q], int k, long left) const {
+    constexpr int rows = 16 / S::NS;
+    const char* q = reinterpret_cast<const char*>(p) + (long)k * S::TT * step;
+    if (left >= S::TT) {
 #pragma unroll
-      for (int i = 0; i < S::Q; ++i) r[i] = (q + (long)i * step * st)[off];
+      for (int i = 0; i < S::Q; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(q + (long)i * rows * step), off);
     } else {
 #pragma unroll
-      for (int i = 0; i < S::Q; ++i) r[i] = t + i * step < left ? (q + (long)i * step * st)[off] : (IT)0.0f;
+      for (int i = 0; i < S::Q; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(q), __umul24(min(t + i * rows, (int)left - 1), step) + n);
     }
   }
-  __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q]) const {
+  // behind the end and past N: 0
+  __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q], long left) const {
+    constexpr int rows = 16 / S::NS;
+    if (left >= S::TT) {
 #pragma unroll
-    for (int i = 0; i < S::Q; ++i) v[i] = ok[0] ? up(r[i]) : 0.0f;
+      for (int i = 0; i < S::Q; ++i) v[i] = ok ? up(r[i]) : 0.0f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::Q; ++i) v[i] = ok && t + i * rows < left ? up(r[i]) : 0.0f;
+    }
   }
 };
 
@@ -182,7 +194,7 @@ __device__ inline float step_size(const ScanArgs& a, float raw) { return a.p.sof
 
 // ------------------------------------------------------------------------------------------------ forward
 // CARRY: leave each chunk's end state from zero and its sum of dl instead of y.
-// Iteration i: finish tile i-1, prepare tile i+1, request tile i+2, walk tile i; one barrier.
+// Iteration i: finish tile i-1, prepare tile i+1, request tile i+3's rows and tile i+2's maps, walk tile i; one barrier.
 template <class IT, class S, bool CARRY>
 __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
   constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
@@ -210,79 +222,83 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = !CARRY && a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = !CARRY && a.p.z.ptr;
-  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at);
-  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
-  IT ru[R], rdl[R], rz[R], rB[Q], rC[Q];
-  long left = at.len - at.t0;                             // steps before the end, from the current tile on
-  auto load = [&](int ahead, bool whole) {
-    su.load(ru, ahead, whole, left - ahead * TT, at.row);
-    sdl.load(rdl, ahead, whole, left - ahead * TT, at.row);
-    if (gate) sz.load(rz, ahead, whole, left - ahead * TT, at.row);
+  const Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at);
+  const Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  struct Rows { IT u[R], dl[R], z[R]; } rows[2];          // of tile k: rows[k & 1]
+  struct RawMaps { IT B[Q], C[Q]; } maps[2];
+  const int last = at.tiles - 1;
+  const long live = at.len - at.t0;                       // steps before the end from the chunk's first on
+  auto load = [&](Rows& r, int k) {
+    k = min(k, last);
+    su.load(r.u, k, live - (long)k * TT, at);
+    sdl.load(r.dl, k, live - (long)k * TT, at);
+    if (!CARRY) sz.load(r.z, k, live - (long)k * TT, at);
   };
-  auto load_maps = [&](int ahead, bool whole) {
-    mB.load(rB, ahead, whole, left - ahead * TT);
-    if (!CARRY) mC.load(rC, ahead, whole, left - ahead * TT);
+  auto load_maps = [&](RawMaps& m, int k) {
+    k = min(k, last);
+    mB.load(m.B, k, live - (long)k * TT);
+    if (!CARRY) mC.load(m.C, k, live - (long)k * TT);
   };
-  auto prepare = [&](int ahead, int buf) {
+  auto prepare = [&](const Rows& r, int k, int buf) {
+    const bool whole = live - (long)k * TT >= TT;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
-      const bool live = row + ahead * TT < left;
-      const float u = up(ru[i]), dl = live ? step_size(a, up(rdl[i]) + bias) : 0.0f;
-      s_in[buf][row][ch] = make_float2(dl, live ? dl * u : 0.0f);
+      const float u = up(r.u[i]);
+      float dl = step_size(a, up(r.dl[i]) + bias), du = dl * u;
+      if (!whole && row + (long)k * TT >= live) dl = du = 0.0f;
+      s_in[buf][row][ch] = make_float2(dl, du);
       if (!CARRY) {
-        float g = 1.0f;
-        if (gate) {
-          const float z = up(rz[i]);
-          g = z * sigmoid(z);
-        }
-        s_out[buf][row][ch] = make_float2(Dk * u, g);
+        const float z = up(r.z[i]);
+        s_out[buf][row][ch] = make_float2(Dk * u, gate ? z * sigmoid(z) : 1.0f);
       }
     }
   };
-  IT* y = CARRY ? nullptr : const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st;
-  const unsigned yoff = (unsigned)(at.row * a.p.y.st) + d;
-  auto finish = [&](IT* yt, long left, long room, int buf) {   // left: steps before the end, room: steps of the chunk, from this tile on
+  // Lanes past the end of the group repeat its last channel: they store the same values to the same places.
+  IT* const y0 = CARRY ? nullptr : const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st;
+  const unsigned ystep = (unsigned)a.p.y.st * sizeof(IT), yoff = __umul24(at.row, ystep) + d * (unsigned)sizeof(IT);
+  auto finish = [&](int k, int buf, long left, long room) {   // left: steps before the end, room: steps of the chunk, from the tile on
+    char* q = reinterpret_cast<char*>(y0) + (long)k * TT * ystep;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
       const float2 o = s_out[buf][row][ch];
       float v = o.x;
 #pragma unroll
-      for (int k = 0; k < PS; ++k) v += s_y[buf][row][k][ch];
-      if (gate) v *= o.y;
-      if (row < room && at.on) (yt + (long)i * PS * a.p.y.st)[yoff] = down<IT>(row < left ? v : 0.0f);
+      for (int p = 0; p < PS; ++p) v += s_y[buf][row][p][ch];
+      v *= o.y;
+      if (row < room) *reinterpret_cast<IT*>(q + (long)i * PS * ystep + yoff) = down<IT>(row < left ? v : 0.0f);
     }
   };
 
-  float B[Q], C[Q];
   if (at.tiles > 0) {
-    load(0, at.full > 0);
-    load_maps(0, at.full > 0);
-    prepare(0, 0);
-    mB.widen(rB, B);
-    if (!CARRY) mC.widen(rC, C);
-    if (at.tiles > 1) load(1, at.full > 1);
+    load(rows[0], 0);
+    load(rows[1], 1);
+    load_maps(maps[0], 0);
+    load_maps(maps[1], 1);
+    prepare(rows[0], 0, 0);
+    load(rows[0], 2);
   }
   __syncthreads();
   float* ck = !CARRY && a.p.checkpoints ? static_cast<float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT) * N + at.n0) * D + d : nullptr;
-  for (int i = 0; i < at.tiles; ++i) {
-    const int buf = i & 1;
-    if (!CARRY && i > 0) finish(y - TT * a.p.y.st, left + TT, left + TT + (at.t1 - at.len), buf ^ 1);
-    if (i + 1 < at.tiles) {
-      prepare(1, buf ^ 1);
-      load_maps(1, i + 1 < at.full);
-    }
-    if (i + 2 < at.tiles) load(2, i + 2 < at.full);
+  auto iteration = [&](int i, auto parity) {
+    constexpr int P = decltype(parity)::v;
+    if (!CARRY && i > 0) finish(i - 1, P ^ 1, TT, TT);
+    prepare(rows[P ^ 1], i + 1, P ^ 1);                   // (behind the last tile: not read)
+    load(rows[P ^ 1], i + 3);
+    float B[Q], C[Q];
+    mB.widen(maps[P].B, B, live - (long)i * TT);
+    if (!CARRY) mC.widen(maps[P].C, C, live - (long)i * TT);
+    load_maps(maps[P], i + 2);
     if (!CARRY && ck) {
 #pragma unroll
       for (int j = 0; j < NS; ++j)
-        if (at.on && at.n0 + j < N) ck[j * D] = h[j];
+        if (at.n0 + j < N) ck[j * D] = h[j];
       ck += N * D;
     }
     each<TT>([&](auto tc) {
       constexpr int t = decltype(tc)::v;
-      const float2 in = s_in[buf][t][ch];
+      const float2 in = s_in[P][t][ch];
       each<NS>([&](auto jc) {
         constexpr int j = decltype(jc)::v;
         h[j] = fmaf(exp2_hw(in.x * A2[j]), h[j], bc<S, t, j>(B) * in.y);
@@ -292,17 +308,14 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
       } else {
         float v = 0.0f;
         dot_bcast<S, t>(v, C, h);
-        s_y[buf][t][part][ch] = v;
+        s_y[P][t][part][ch] = v;
       }
     });
-    if (i + 1 < at.tiles) {
-      mB.widen(rB, B);
-      if (!CARRY) mC.widen(rC, C);
-    }
-    su.tile(1), sdl.tile(1), sz.tile(1), mB.tile(1), mC.tile(1);
-    if (!CARRY) y += TT * a.p.y.st;
-    left -= TT;
     __syncthreads();
+  };
+  for (int i = 0; i < at.tiles; i += 2) {
+    iteration(i, Int<0>{});
+    if (i + 1 < at.tiles) iteration(i + 1, Int<1>{});
   }
   if (CARRY) {
     if (!at.on) return;
@@ -313,10 +326,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     if (at.row == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
     return;
   }
-  if (at.tiles > 0) finish(y - TT * a.p.y.st, left + TT, left + TT + (at.t1 - at.len), (at.tiles - 1) & 1);
+  if (last >= 0) finish(last, last & 1, live - (long)last * TT, at.t1 - at.t0 - (long)last * TT);
   if (!at.on) return;
-  for (long t = at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS)       // padding behind the last tile
-    (y + (t - at.tiles * TT) * a.p.y.st)[d] = down<IT>(0.0f);
+  for (long t = (long)at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS)       // padding behind the last tile
+    (y0 + t * a.p.y.st)[d] = down<IT>(0.0f);
   if (a.p.state_out && at.c == a.chunks - 1) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
   const Place<S> at(a);
   const long D = a.p.D, N = a.p.N, T = a.p.T, b = at.b;
   const unsigned d = at.d;
-  const int lane = at.lane, ch = at.ch, part = at.row;
+  const int ch = at.ch, part = at.row;
   float A2[NS], lam[NS], dA[NS], sum = 0.0f, dDk = 0.0f, dbias = 0.0f;
   load_A2<S>(a, at, A2);
 #pragma unroll
@@ -427,36 +440,43 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = a.p.z.ptr;
-  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at), sdy(a.g.dy, at);
-  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
-  IT ru[R], rdl[R], rz[R], rdy[R], rB[Q], rC[Q];
+  const Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at), sdy(a.g.dy, at);
+  const Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  struct Rows { IT u[R], dl[R], z[R], dy[R]; } rows[2];   // of tile k: rows[k & 1]
+  struct RawMaps { IT B[Q], C[Q]; float h[NS]; } maps[2]; // h: the checkpoint at the tile's start
   const int last = at.tiles - 1;
-  su.tile(last), sdl.tile(last), sz.tile(last), sdy.tile(last), mB.tile(last), mC.tile(last);
-  long left = at.len - at.t0 - (long)last * TT;           // steps before the end, from the current tile on
-  auto load = [&](int ahead, bool whole) {
-    su.load(ru, ahead, whole, left - ahead * TT, at.row);
-    sdl.load(rdl, ahead, whole, left - ahead * TT, at.row);
-    sdy.load(rdy, ahead, whole, left - ahead * TT, at.row);
-    if (gate) sz.load(rz, ahead, whole, left - ahead * TT, at.row);
+  const long live = at.len - at.t0;                       // steps before the end from the chunk's first on
+  const float* const ck = CARRY ? nullptr : static_cast<const float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT) * N + at.n0) * D + d;
+  auto load = [&](Rows& r, int k) {
+    k = max(k, 0);
+    su.load(r.u, k, live - (long)k * TT, at);
+    sdl.load(r.dl, k, live - (long)k * TT, at);
+    sdy.load(r.dy, k, live - (long)k * TT, at);
+    sz.load(r.z, k, live - (long)k * TT, at);
   };
-  auto load_maps = [&](int ahead, bool whole) {
-    mC.load(rC, ahead, whole, left - ahead * TT);
-    if (!CARRY) mB.load(rB, ahead, whole, left - ahead * TT);
+  auto load_maps = [&](RawMaps& m, int k) {
+    k = max(k, 0);
+    mC.load(m.C, k, live - (long)k * TT);
+    if (CARRY) return;
+    mB.load(m.B, k, live - (long)k * TT);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) m.h[j] = ck[((long)k * N + min(j, (int)N - 1 - at.n0)) * D];      // (states past N: any value in bounds)
   };
-  auto prepare = [&](int ahead, int buf) {
+  auto prepare = [&](const Rows& r, int k, int buf) {
+    const bool whole = live - (long)k * TT >= TT;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
-      const bool live = row + ahead * TT < left && at.on;
-      const float raw = up(rdl[i]) + bias, dl = live ? step_size(a, raw) : 0.0f, u = up(ru[i]), dy = up(rdy[i]);
-      float dY = dy, dg = 0.0f;
+      const float raw = up(r.dl[i]) + bias, u = up(r.u[i]), dy = up(r.dy[i]);
+      float dl = step_size(a, raw), dY = dy, dg = 0.0f, du = dl * u;
       if (gate) {
-        const float z = up(rz[i]), sg = sigmoid(z);
+        const float z = up(r.z[i]), sg = sigmoid(z);
         dY *= z * sg;
         dg = dy * (sg * fmaf(z, 1.0f - sg, 1.0f));
       }
-      s_in[buf][row][ch] = make_float2(dl, live ? dl * u : 0.0f);
-      s_dy[buf][row][ch] = live ? dY : 0.0f;
+      if (!at.on || (!whole && row + (long)k * TT >= live)) dl = du = dY = 0.0f;
+      s_in[buf][row][ch] = make_float2(dl, du);
+      s_dy[buf][row][ch] = dY;
       if (!CARRY) {
         s_own[0][row][ch] = u;
         s_own[1][row][ch] = a.p.softplus ? sigmoid(raw) : 1.0f;
@@ -464,78 +484,74 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
       }
     }
   };
-  IT* du = static_cast<IT*>(a.g.du) + (b * T + at.t0 + (long)last * TT) * D;
-  IT* ddelta = static_cast<IT*>(a.g.ddelta) + (b * T + at.t0 + (long)last * TT) * D;
-  IT* dz = static_cast<IT*>(a.g.dz) + (gate ? (b * T + at.t0 + (long)last * TT) * D : 0);
-  const unsigned ooff = (unsigned)(at.row * D) + d;
-  auto finish = [&](int buf) {
-    const long room = left + (at.t1 - at.len);
+  const unsigned ostep = (unsigned)D * sizeof(IT), ooff = __umul24(at.row, ostep) + d * (unsigned)sizeof(IT);
+  const long out0 = (b * T + at.t0) * D;
+  auto finish = [&](int k, int buf) {
+    const long left = live - (long)k * TT, room = at.t1 - at.t0 - (long)k * TT;
+    const long tile = (long)k * TT * ostep;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-      for (int k = 0; k < PS; ++k) {
-        const float2 s = s_sum[row][k][ch];
+      for (int p = 0; p < PS; ++p) {
+        const float2 s = s_sum[row][p][ch];
         s1 += s.x;
         s2 += s.y;
       }
       const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[0][row][ch];
-      const bool live = row < left, store = row < room && at.on;
+      const bool in = row < left && at.on, store = row < room && at.on;
       const float ddl = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
-      if (live && at.on) {
-        dDk = fmaf(dY, u, dDk);
-        dbias += ddl;
-      }
-      const long o = (long)i * PS * D;
-      if (store) {
-        (du + o)[ooff] = down<IT>(live ? fmaf(dl, s1, Dk * dY) : 0.0f);
-        (ddelta + o)[ooff] = down<IT>(live ? ddl : 0.0f);
-      }
+      dDk = fmaf(dY, in ? u : 0.0f, dDk);
+      dbias += in ? ddl : 0.0f;
+      const long o = tile + (long)i * PS * ostep + ooff;
+      auto put = [&](void* p, float v) {
+        if (store) *reinterpret_cast<IT*>(reinterpret_cast<char*>(static_cast<IT*>(p) + out0) + o) = down<IT>(in ? v : 0.0f);
+      };
+      put(a.g.du, fmaf(dl, s1, Dk * dY));
+      put(a.g.ddelta, ddl);
       if (gate) {
         float y = Dk * u;
 #pragma unroll
-        for (int k = 0; k < PS; ++k) y += s_y[row][k][ch];
-        if (store) (dz + o)[ooff] = down<IT>(live ? y * s_own[2][row][ch] : 0.0f);
+        for (int p = 0; p < PS; ++p) y += s_y[row][p][ch];
+        put(a.g.dz, y * s_own[2][row][ch]);
       }
     }
   };
 
-  const float* ck = CARRY ? nullptr : static_cast<const float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT + last) * N + at.n0) * D + d;
-  float B[Q], C[Q], h0[NS], hn[NS];
-  auto load_ck = [&](const float* p) {
-#pragma unroll
-    for (int j = 0; j < NS; ++j) hn[j] = at.n0 + j < N ? p[j * D] : 0.0f;
-  };
   if (at.tiles > 0) {
-    load(0, last < at.full);
-    load_maps(0, last < at.full);
-    if (!CARRY) load_ck(ck);
-    prepare(0, last & 1);
-    mC.widen(rC, C);
-    if (!CARRY) {
-      mB.widen(rB, B);
-#pragma unroll
-      for (int j = 0; j < NS; ++j) h0[j] = hn[j];
-    }
-    if (last > 0) load(-1, true);
+    const int p = last & 1;
+    // (the register sets are named by the tile's parity; at run time one of the two orders)
+    auto begin = [&](auto parity) {
+      constexpr int P = decltype(parity)::v;
+      load(rows[P], last);
+      load(rows[P ^ 1], last - 1);
+      load_maps(maps[P], last);
+      load_maps(maps[P ^ 1], last - 1);
+      prepare(rows[P], last, P);
+      load(rows[P], last - 2);
+    };
+    if (p) begin(Int<1>{});
+    else begin(Int<0>{});
   }
   __syncthreads();
-  float *pB = nullptr, *pC = nullptr;
-  if (!CARRY) {
-    const long o = ((at.blk * a.p.B + b) * T + at.t0 + (long)last * TT) * N;
-    pB = a.partB + o, pC = a.partC + o;
-  }
-  for (int i = last; i >= 0; --i) {
-    const int buf = i & 1;
-    if (i > 0) {
-      load_maps(-1, true);
-      if (!CARRY) load_ck(ck - N * D);
+  const long part0 = ((at.blk * a.p.B + b) * T + at.t0) * N;
+  auto iteration = [&](int i, auto parity) {
+    constexpr int P = decltype(parity)::v;
+    float B[Q], C[Q], h0[NS];
+    mC.widen(maps[P].C, C, live - (long)i * TT);
+    if (!CARRY) {
+      mB.widen(maps[P].B, B, live - (long)i * TT);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) h0[j] = at.n0 + j < N ? maps[P].h[j] : 0.0f;
     }
+    load_maps(maps[P], i - 2);
     if constexpr (CARRY) {
+      prepare(rows[P ^ 1], max(i - 1, 0), P ^ 1);         // (before the first tile: not read)
+      load(rows[P ^ 1], i - 3);
       each_back<TT - 1>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float dl = s_in[buf][t][ch].x, dY = s_dy[buf][t][ch];
+        const float dl = s_in[P][t][ch].x, dY = s_dy[P][t][ch];
         sum += dl;
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
@@ -546,7 +562,7 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
       float hh[TT][NS], aa[TT][NS];
       each<TT>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float2 in = s_in[buf][t][ch];
+        const float2 in = s_in[P][t][ch];
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
           aa[t][j] = exp2_hw(in.x * A2[j]);
@@ -562,10 +578,11 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
 #pragma unroll
       for (int j = 0; j < NS; ++j) tA[j] = 0.0f;
       ChannelSum<S> sums;
+      const long room = at.t1 - at.t0 - (long)i * TT;
       each_back<TT - 1>([&](auto tc) {
         constexpr int t = decltype(tc)::v;
-        const float2 in = s_in[buf][t][ch];
-        const float dY = s_dy[buf][t][ch];
+        const float2 in = s_in[P][t][ch];
+        const float dY = s_dy[P][t][ch];
         float v[2 * NS], gg[NS], s1 = 0.0f, s2 = 0.0f;
         each<NS>([&](auto jc) {
           constexpr int j = decltype(jc)::v;
@@ -582,39 +599,30 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
         s_sum[t][part][ch] = make_float2(s1, s2);
         using CS = ChannelSum<S>;
         float out[CS::K / CS::KG];
-        if (sums.template add<t>(v, lane, out)) {
-          const int ts = t + CS::step_of(lane);
-          if (ts < left + (at.t1 - at.len)) {
+        if (sums.template add<t>(v, at.lane, out)) {
+          const int ts = t + CS::step_of(at.lane);
 #pragma unroll
-            for (int o = 0; o < CS::K / CS::KG; ++o) {
-              const int k = o * CS::KG + CS::value_of(lane), n = at.n0 + k % NS;
-              if (n < N) (k < NS ? pB : pC)[(unsigned)(ts * (int)N + n)] = out[o];
-            }
+          for (int o = 0; o < CS::K / CS::KG; ++o) {
+            const int k = o * CS::KG + CS::value_of(at.lane), n = at.n0 + k % NS;
+            float* p = (k < NS ? a.partB : a.partC) + part0 + (long)i * TT * N;
+            if (ts < room && n < N) p[ts * (int)N + n] = out[o];
           }
         }
       });
 #pragma unroll
       for (int j = 0; j < NS; ++j) dA[j] += tA[j];
+      __syncthreads();
+      finish(i, P);
+      prepare(rows[P ^ 1], max(i - 1, 0), P ^ 1);
+      load(rows[P ^ 1], i - 3);
     }
     __syncthreads();
-    if (!CARRY) finish(buf);
-    if (i > 0) {
-      prepare(-1, buf ^ 1);
-      if (i > 1) load(-2, true);
-      mC.widen(rC, C);
-      if (!CARRY) {
-        mB.widen(rB, B);
-#pragma unroll
-        for (int j = 0; j < NS; ++j) h0[j] = hn[j];
-      }
-    }
-    su.tile(-1), sdl.tile(-1), sz.tile(-1), sdy.tile(-1), mB.tile(-1), mC.tile(-1);
-    left += TT;
-    if (!CARRY) {
-      du -= TT * D, ddelta -= TT * D, pB -= TT * N, pC -= TT * N, ck -= N * D;
-      if (gate) dz -= TT * D;
-    }
-    __syncthreads();
+  };
+  int i = last;
+  if (i >= 0 && (i & 1)) iteration(i--, Int<1>{});
+  for (; i >= 0; i -= 2) {
+    iteration(i, Int<0>{});
+    if (i > 0) iteration(i - 1, Int<1>{});
   }
   if constexpr (CARRY) {
     if (!at.on) return;
@@ -624,11 +632,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
       if (at.n0 + j < N) hl[j * D] = lam[j];
     if (at.row == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
   } else {
-    const long out0 = b * T * D + d;
-    for (long t = at.t0 + (long)at.tiles * TT + at.row; t < at.t1 && at.on; t += PS) {       // padding
-      static_cast<IT*>(a.g.du)[out0 + t * D] = down<IT>(0.0f);
-      static_cast<IT*>(a.g.ddelta)[out0 + t * D] = down<IT>(0.0f);
-      if (gate) static_cast<IT*>(a.g.dz)[out0 + t * D] = down<IT>(0.0f);
+    for (long t = (long)at.tiles * TT + at.row; t < at.t1 - at.t0 && at.on; t += PS) {       // padding
+      static_cast<IT*>(a.g.du)[out0 + t * D + d] = down<IT>(0.0f);
+      static_cast<IT*>(a.g.ddelta)[out0 + t * D + d] = down<IT>(0.0f);
+      if (gate) static_cast<IT*>(a.g.dz)[out0 + t * D + d] = down<IT>(0.0f);
     }
     s_sum[0][part][ch] = make_float2(dDk, dbias);
     __syncthreads();
