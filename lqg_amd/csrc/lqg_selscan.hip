@@ -43,6 +43,8 @@ int check(const lqg_selscan* p) {
   return 0;
 }
 
+// states that the workgroups' shapes have room for (Shape::NP)
+long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
 int tile_of(long N) { return N > 32 ? 8 : 16; }
 
 ScanArgs describe(const lqg_selscan* p) {
@@ -92,7 +94,7 @@ extern "C" size_t lqg_selscan_workspace(const lqg_selscan* p) {
   return check(p) ? 0 : (size_t)carry_floats(describe(p)) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p) {
-  return check(p) ? 0 : (size_t)(p->B * describe(p).tiles * p->N * p->D) * sizeof(float);
+  return check(p) ? 0 : (size_t)(p->B * describe(p).tiles * room_of(p->N) * p->D) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_grad_workspace(const lqg_selscan* p) {
   return check(p) ? 0 : (size_t)grad_space(describe(p)).total * sizeof(float);

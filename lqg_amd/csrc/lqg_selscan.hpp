@@ -35,6 +35,7 @@ template <int CH_, int NS_, int NW_, int TT_> struct Shape {
   static constexpr int CH = CH_, NS = NS_, NW = NW_, TT = TT_;
   static constexpr int LS = 64 / CH;          // groups of NS states in a wave
   static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
+  static constexpr int NP = NS * PS;          // states it has room for
   static constexpr int R = TT / PS;           // elements of a tile (TT x CH) that a thread prepares and finishes: rows PS apart
   static constexpr int Q = TT * NS / 16;      // registers of a tile's B (or C)
   static_assert(TT % PS == 0 && TT * NS % 16 == 0 && CH % 16 == 0, "");
@@ -82,70 +83,64 @@ template <class S> __device__ inline void load_A2(const ScanArgs& a, const Place
   for (int j = 0; j < S::NS; ++j) A2[j] = at.n0 + j < a.p.N ? load_param(a.p.A, at.d * a.p.N + at.n0 + j) * LOG2E : 0.0f;
 }
 
-// Row t of a tile is read at a uniform pointer plus a 32-bit offset of the thread, in bytes (row strides are below 2^24 of them).  Both
-// ways of a load issue the same number of instructions, so that the counter of outstanding loads can be waited on exactly: loads run two
-// tiles ahead and a wait for one tile's must not wait for the next one's.
-template <class IT> __device__ inline IT at_byte(const IT* p, unsigned off) {
-  return *reinterpret_cast<const IT*>(reinterpret_cast<const char*>(p) + off);
-}
+// Row t of a tile is read at a uniform pointer plus a 32-bit offset of the thread, in bytes (row strides are below 2^24 of them).  Loads
+// run two tiles ahead of their use and are never skipped, so that the counter of outstanding loads can be waited on exactly.
+template <class IT> __device__ inline IT at_byte(const char* p, unsigned off) { return *reinterpret_cast<const IT*>(p + off); }
 
 // One sequence: R rows of the thread in each tile, PS apart.
 template <class IT, class S> struct Stream {
-  const IT* p;                                // the chunk's first row
+  const char *p, *q;                          // the chunk's first row; the next tile of `next`
   unsigned off, step;                         // the thread's first row and channel; bytes of a row
   __device__ Stream(const lqg_seq& s, const Place<S>& at)
-      : p(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st), off(__umul24(at.row, (unsigned)s.st * sizeof(IT)) + at.d * (unsigned)sizeof(IT)),
-        step((unsigned)s.st * sizeof(IT)) {}
-  __device__ const IT* tile(int k) const { return reinterpret_cast<const IT*>(reinterpret_cast<const char*>(p) + (long)k * S::TT * step); }
+      : p(reinterpret_cast<const char*>(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st)), q(p),
+        off(__umul24(at.row, (unsigned)s.st * sizeof(IT)) + at.d * (unsigned)sizeof(IT)), step((unsigned)s.st * sizeof(IT)) {}
+  __device__ const char* tile(int k) const { return p + (long)k * S::TT * step; }
+  __device__ void seek(int k) { q = tile(k); }
+  // a whole tile, then on by `way` tiles
+  __device__ void next(IT (&r)[S::R], int way) {
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) r[i] = at_byte<IT>(q + (long)i * S::PS * step, off);
+    q += (long)way * S::TT * (int)step;
+  }
   // tile k; left: steps before the end from its first row on (>= 1): rows behind the end repeat the last one
   __device__ void load(IT (&r)[S::R], int k, long left, const Place<S>& at) const {
-    const IT* q = tile(k);
-    if (left >= S::TT) {
+    const int most = (int)min(left, (long)S::TT) - 1;
 #pragma unroll
-      for (int i = 0; i < S::R; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(reinterpret_cast<const char*>(q) + (long)i * S::PS * step), off);
-    } else {
-#pragma unroll
-      for (int i = 0; i < S::R; ++i)
-        r[i] = at_byte(q, __umul24(min(at.row + i * S::PS, (int)left - 1), step) + at.d * (unsigned)sizeof(IT));
-    }
+    for (int i = 0; i < S::R; ++i)
+      r[i] = at_byte<IT>(tile(k), __umul24(min(at.row + i * S::PS, most), step) + at.d * (unsigned)sizeof(IT));
   }
 };
 
 // a tile's B or C: value (t, j) of a lane's states in register (t NS + j) / 16, lane (t NS + j) % 16 of its row of 16
 template <class IT, class S> struct Maps {
-  const IT* p;
+  static constexpr int rows = 16 / S::NS;     // steps of a register
+  const char *p, *q;
   unsigned off, step, n;
   int t;
   bool ok;
   __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : step((unsigned)s.st * sizeof(IT)) {
     const int f = at.lane & 15, j = f % S::NS;
     t = f / S::NS;
-    p = static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg;
+    p = q = reinterpret_cast<const char*>(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg);
     ok = at.n0 + j < a.p.N;
     n = (ok ? at.n0 + j : 0) * sizeof(IT);
     off = __umul24(t, step) + n;
   }
-  __device__ void load(IT (&r)[S::Q], int k, long left) const {
-    constexpr int rows = 16 / S::NS;
-    const char* q = reinterpret_cast<const char*>(p) + (long)k * S::TT * step;
-    if (left >= S::TT) {
+  __device__ void seek(int k) { q = p + (long)k * S::TT * step; }
+  __device__ void next(IT (&r)[S::Q], int way) {
 #pragma unroll
-      for (int i = 0; i < S::Q; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(q + (long)i * rows * step), off);
-    } else {
-#pragma unroll
-      for (int i = 0; i < S::Q; ++i) r[i] = at_byte(reinterpret_cast<const IT*>(q), __umul24(min(t + i * rows, (int)left - 1), step) + n);
-    }
+    for (int i = 0; i < S::Q; ++i) r[i] = at_byte<IT>(q + (long)i * rows * step, off);
+    q += (long)way * S::TT * (int)step;
   }
-  // behind the end and past N: 0
-  __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q], long left) const {
-    constexpr int rows = 16 / S::NS;
-    if (left >= S::TT) {
+  __device__ void load(IT (&r)[S::Q], int k, long left) const {
+    const int most = (int)min(left, (long)S::TT) - 1;
 #pragma unroll
-      for (int i = 0; i < S::Q; ++i) v[i] = ok ? up(r[i]) : 0.0f;
-    } else {
+    for (int i = 0; i < S::Q; ++i) r[i] = at_byte<IT>(p + (long)k * S::TT * step, __umul24(min(t + i * rows, most), step) + n);
+  }
+  // past N, and behind the end of a tile that is not whole: 0
+  template <bool WHOLE> __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q], long left) const {
 #pragma unroll
-      for (int i = 0; i < S::Q; ++i) v[i] = ok && t + i * rows < left ? up(r[i]) : 0.0f;
-    }
+    for (int i = 0; i < S::Q; ++i) v[i] = ok && (WHOLE || t + i * rows < left) ? up(r[i]) : 0.0f;
   }
 };
 
@@ -153,26 +148,23 @@ template <class S, int T, int J> __device__ inline float bc(const float (&r)[S::
   return row_bcast<(T * S::NS + J) % 16>(r[(T * S::NS + J) / 16]);
 }
 
-// y += sum_j bc(C)(t, j) h[j].  The broadcast is an operand modifier of the multiply-add, which the compiler does not fold there (it would
+// sum_j bc(C)(t, j) h[j].  The broadcast is an operand modifier of the multiply-add, which the compiler folds into products only (it would
 // copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart from the broadcast's read.
-#define LQG_FMAC_BCAST(Y, C, K, X) "v_fmac_f32_dpp " Y ", " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
-template <class S, int T> __device__ inline void dot_bcast(float& y, const float (&C)[S::Q], const float (&h)[S::NS]) {
+#define LQG_FMAC_BCAST(C, K, X) "v_fmac_f32_dpp %0, " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
+template <class S, int T> __device__ inline float dot_bcast(const float (&C)[S::Q], const float (&h)[S::NS]) {
   constexpr int f = T * S::NS, k = f % 16;
+  float y = row_bcast<k>(C[f / 16]) * h[0];
   if constexpr (S::NS == 2) {
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c4", "%2") LQG_FMAC_BCAST("%0", "%1", "%c5", "%3")
-        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "n"(k), "n"(k + 1));
-  } else if constexpr (S::NS == 4) {
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
-        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
-        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k), "n"(k + 1), "n"(k + 2), "n"(k + 3));
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c3", "%2") : "+v"(y) : "v"(C[f / 16]), "v"(h[1]), "n"(k + 1));
   } else {
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
-        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
-        : "+v"(y) : "v"(C[f / 16]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k), "n"(k + 1), "n"(k + 2), "n"(k + 3));
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c6", "%2") LQG_FMAC_BCAST("%0", "%1", "%c7", "%3")
-        LQG_FMAC_BCAST("%0", "%1", "%c8", "%4") LQG_FMAC_BCAST("%0", "%1", "%c9", "%5")
-        : "+v"(y) : "v"(C[f / 16]), "v"(h[4]), "v"(h[5]), "v"(h[6]), "v"(h[7]), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c5", "%2") LQG_FMAC_BCAST("%1", "%c6", "%3") LQG_FMAC_BCAST("%1", "%c7", "%4")
+        : "+v"(y) : "v"(C[f / 16]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k + 1), "n"(k + 2), "n"(k + 3));
+    if constexpr (S::NS == 8)
+      asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c6", "%2") LQG_FMAC_BCAST("%1", "%c7", "%3") LQG_FMAC_BCAST("%1", "%c8", "%4")
+          LQG_FMAC_BCAST("%1", "%c9", "%5")
+          : "+v"(y) : "v"(C[f / 16]), "v"(h[4]), "v"(h[5]), "v"(h[6]), "v"(h[7]), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
   }
+  return y;
 }
 
 // compile-time loop: f(Int<I>) for I = 0 .. N-1, or downwards
@@ -222,31 +214,30 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = !CARRY && a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = !CARRY && a.p.z.ptr;
-  const Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at);
-  const Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at);
+  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
   struct Rows { IT u[R], dl[R], z[R]; } rows[2];          // of tile k: rows[k & 1]
   struct RawMaps { IT B[Q], C[Q]; } maps[2];
   const int last = at.tiles - 1;
   const long live = at.len - at.t0;                       // steps before the end from the chunk's first on
-  auto load = [&](Rows& r, int k) {
+  auto load = [&](Rows& r, int k) __attribute__((always_inline)) {
     k = min(k, last);
     su.load(r.u, k, live - (long)k * TT, at);
     sdl.load(r.dl, k, live - (long)k * TT, at);
     if (!CARRY) sz.load(r.z, k, live - (long)k * TT, at);
   };
-  auto load_maps = [&](RawMaps& m, int k) {
+  auto load_maps = [&](RawMaps& m, int k) __attribute__((always_inline)) {
     k = min(k, last);
     mB.load(m.B, k, live - (long)k * TT);
     if (!CARRY) mC.load(m.C, k, live - (long)k * TT);
   };
-  auto prepare = [&](const Rows& r, int k, int buf) {
-    const bool whole = live - (long)k * TT >= TT;
+  auto prepare = [&](const Rows& r, long left, int buf, auto whole) __attribute__((always_inline)) {        // left: steps before the end from the tile's first row on
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
       const float u = up(r.u[i]);
       float dl = step_size(a, up(r.dl[i]) + bias), du = dl * u;
-      if (!whole && row + (long)k * TT >= live) dl = du = 0.0f;
+      if (!decltype(whole)::v && row >= left) dl = du = 0.0f;
       s_in[buf][row][ch] = make_float2(dl, du);
       if (!CARRY) {
         const float z = up(r.z[i]);
@@ -255,10 +246,9 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     }
   };
   // Lanes past the end of the group repeat its last channel: they store the same values to the same places.
-  IT* const y0 = CARRY ? nullptr : const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st;
   const unsigned ystep = (unsigned)a.p.y.st * sizeof(IT), yoff = __umul24(at.row, ystep) + d * (unsigned)sizeof(IT);
-  auto finish = [&](int k, int buf, long left, long room) {   // left: steps before the end, room: steps of the chunk, from the tile on
-    char* q = reinterpret_cast<char*>(y0) + (long)k * TT * ystep;
+  char* y = CARRY ? nullptr : reinterpret_cast<char*>(const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st);
+  auto finish = [&](int buf, long left, long room, auto whole) __attribute__((always_inline)) {    // the tile at y; left: steps before the end, room: of the chunk
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
@@ -267,8 +257,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
 #pragma unroll
       for (int p = 0; p < PS; ++p) v += s_y[buf][row][p][ch];
       v *= o.y;
-      if (row < room) *reinterpret_cast<IT*>(q + (long)i * PS * ystep + yoff) = down<IT>(row < left ? v : 0.0f);
+      if (decltype(whole)::v || row < room)
+        *reinterpret_cast<IT*>(y + (long)i * PS * ystep + yoff) = down<IT>(decltype(whole)::v || row < left ? v : 0.0f);
     }
+    y += (long)TT * ystep;
   };
 
   if (at.tiles > 0) {
@@ -276,46 +268,68 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     load(rows[1], 1);
     load_maps(maps[0], 0);
     load_maps(maps[1], 1);
-    prepare(rows[0], 0, 0);
+    prepare(rows[0], live, 0, Int<0>{});
     load(rows[0], 2);
   }
   __syncthreads();
-  float* ck = !CARRY && a.p.checkpoints ? static_cast<float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT) * N + at.n0) * D + d : nullptr;
-  auto iteration = [&](int i, auto parity) {
+  const bool keep = !CARRY && a.p.checkpoints;
+  char* ck = keep ? static_cast<char*>(a.p.checkpoints) + (b * a.tiles + at.t0 / TT) * S::NP * D * sizeof(float) : nullptr;
+  const unsigned ckoff = ((unsigned)at.n0 * (unsigned)D + d) * (unsigned)sizeof(float);
+  // FAST: tiles i - 1 .. i + 3 exist and are whole
+  auto iteration = [&](int i, auto parity, auto fast) __attribute__((always_inline)) {
     constexpr int P = decltype(parity)::v;
-    if (!CARRY && i > 0) finish(i - 1, P ^ 1, TT, TT);
-    prepare(rows[P ^ 1], i + 1, P ^ 1);                   // (behind the last tile: not read)
-    load(rows[P ^ 1], i + 3);
-    float B[Q], C[Q];
-    mB.widen(maps[P].B, B, live - (long)i * TT);
-    if (!CARRY) mC.widen(maps[P].C, C, live - (long)i * TT);
-    load_maps(maps[P], i + 2);
-    if (!CARRY && ck) {
-#pragma unroll
-      for (int j = 0; j < NS; ++j)
-        if (at.n0 + j < N) ck[j * D] = h[j];
-      ck += N * D;
+    constexpr bool FAST = decltype(fast)::v;
+    const long left = live - (long)i * TT;
+    if (!CARRY && (FAST || i > 0)) finish(P ^ 1, TT, TT, Int<1>{});
+    prepare(rows[P ^ 1], left - TT, P ^ 1, fast);         // (behind the last tile: not read)
+    if (FAST) {
+      su.next(rows[P ^ 1].u, 1);
+      sdl.next(rows[P ^ 1].dl, 1);
+      if (!CARRY) sz.next(rows[P ^ 1].z, 1);
+    } else {
+      load(rows[P ^ 1], i + 3);
     }
-    each<TT>([&](auto tc) {
+    float B[Q], C[Q];
+    mB.template widen<FAST>(maps[P].B, B, left);
+    if (!CARRY) mC.template widen<FAST>(maps[P].C, C, left);
+    if (FAST) {
+      mB.next(maps[P].B, 1);
+      if (!CARRY) mC.next(maps[P].C, 1);
+    } else {
+      load_maps(maps[P], i + 2);
+    }
+    if (!CARRY && keep) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) *reinterpret_cast<float*>(ck + (long)j * D * sizeof(float) + ckoff) = h[j];
+      ck += (long)S::NP * D * sizeof(float);
+    }
+    float2 in[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) in[t] = s_in[P][t][ch];
+    __builtin_amdgcn_sched_barrier(0);                    // all of the tile's inputs on their way before the first is waited for
+    each<TT>([&](auto tc) __attribute__((always_inline)) {
       constexpr int t = decltype(tc)::v;
-      const float2 in = s_in[P][t][ch];
-      each<NS>([&](auto jc) {
+      each<NS>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::v;
-        h[j] = fmaf(exp2_hw(in.x * A2[j]), h[j], bc<S, t, j>(B) * in.y);
+        h[j] = fmaf(exp2_hw(in[t].x * A2[j]), h[j], bc<S, t, j>(B) * in[t].y);
       });
-      if (CARRY) {
-        sum += in.x;
-      } else {
-        float v = 0.0f;
-        dot_bcast<S, t>(v, C, h);
-        s_y[P][t][part][ch] = v;
-      }
+      if (CARRY) sum += in[t].x;
+      else s_y[P][t][part][ch] = dot_bcast<S, t>(C, h);
     });
     __syncthreads();
   };
-  for (int i = 0; i < at.tiles; i += 2) {
-    iteration(i, Int<0>{});
-    if (i + 1 < at.tiles) iteration(i + 1, Int<1>{});
+  for (int i = 0; i < at.tiles;) {
+    if ((i & 1) && i + 4 < at.full) {                     // pairs (odd, even) while tile i + 4 is whole
+      su.seek(i + 3), sdl.seek(i + 3), sz.seek(i + 3), mB.seek(i + 2), mC.seek(i + 2);
+      for (; i + 4 < at.full; i += 2) {
+        iteration(i, Int<1>{}, Int<1>{});
+        iteration(i + 1, Int<0>{}, Int<1>{});
+      }
+    } else {
+      if (i & 1) iteration(i, Int<1>{}, Int<0>{});
+      else iteration(i, Int<0>{}, Int<0>{});
+      ++i;
+    }
   }
   if (CARRY) {
     if (!at.on) return;
@@ -326,10 +340,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     if (at.row == 0) a.sd[(b * a.chunks + at.c) * D + d] = sum;
     return;
   }
-  if (last >= 0) finish(last, last & 1, live - (long)last * TT, at.t1 - at.t0 - (long)last * TT);
+  if (last >= 0) finish(last & 1, live - (long)last * TT, at.t1 - at.t0 - (long)last * TT, Int<0>{});
   if (!at.on) return;
-  for (long t = (long)at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS)       // padding behind the last tile
-    (y0 + t * a.p.y.st)[d] = down<IT>(0.0f);
+  for (long t = (long)at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS, y += (long)PS * ystep)       // padding behind the last tile
+    *reinterpret_cast<IT*>(y + yoff) = down<IT>(0.0f);
   if (a.p.state_out && at.c == a.chunks - 1) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
@@ -410,7 +424,7 @@ template <class S> struct ChannelSum {
 
 // CARRY: leave each chunk's carry (lambda at its start from 0 at its end) and its sum of dl.
 template <class IT, class S, bool CARRY>
-__global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
+__global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
   constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
   __shared__ float2 s_in[2][TT][CH];                      // dl, dl u
   __shared__ float s_dy[2][TT][CH];                       // dY
@@ -440,30 +454,35 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
   const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
   const float Dk = a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
   const bool gate = a.p.z.ptr;
-  const Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at), sdy(a.g.dy, at);
-  const Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
+  Stream<IT, S> su(a.p.u, at), sdl(a.p.delta, at), sz(gate ? a.p.z : a.p.u, at), sdy(a.g.dy, at);
+  Maps<IT, S> mB(a.p.Bm, a, at), mC(a.p.Cm, a, at);
   struct Rows { IT u[R], dl[R], z[R], dy[R]; } rows[2];   // of tile k: rows[k & 1]
   struct RawMaps { IT B[Q], C[Q]; float h[NS]; } maps[2]; // h: the checkpoint at the tile's start
   const int last = at.tiles - 1;
   const long live = at.len - at.t0;                       // steps before the end from the chunk's first on
-  const float* const ck = CARRY ? nullptr : static_cast<const float*>(a.p.checkpoints) + ((b * a.tiles + at.t0 / TT) * N + at.n0) * D + d;
-  auto load = [&](Rows& r, int k) {
+  const long cktile = S::NP * D * (long)sizeof(float);
+  const char* const ck0 = CARRY ? nullptr : static_cast<const char*>(a.p.checkpoints) + (b * a.tiles + at.t0 / TT) * cktile;
+  const char* ck = ck0;
+  const unsigned ckoff = ((unsigned)at.n0 * (unsigned)D + d) * (unsigned)sizeof(float);
+  auto load = [&](Rows& r, int k) __attribute__((always_inline)) {
     k = max(k, 0);
     su.load(r.u, k, live - (long)k * TT, at);
     sdl.load(r.dl, k, live - (long)k * TT, at);
     sdy.load(r.dy, k, live - (long)k * TT, at);
     sz.load(r.z, k, live - (long)k * TT, at);
   };
-  auto load_maps = [&](RawMaps& m, int k) {
+  auto load_h = [&](RawMaps& m, const char* p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j) m.h[j] = at_byte<float>(p + (long)j * D * sizeof(float), ckoff);
+  };
+  auto load_maps = [&](RawMaps& m, int k) __attribute__((always_inline)) {
     k = max(k, 0);
     mC.load(m.C, k, live - (long)k * TT);
     if (CARRY) return;
     mB.load(m.B, k, live - (long)k * TT);
-#pragma unroll
-    for (int j = 0; j < NS; ++j) m.h[j] = ck[((long)k * N + min(j, (int)N - 1 - at.n0)) * D];      // (states past N: any value in bounds)
+    load_h(m, ck0 + k * cktile);
   };
-  auto prepare = [&](const Rows& r, int k, int buf) {
-    const bool whole = live - (long)k * TT >= TT;
+  auto prepare = [&](const Rows& r, long left, int buf, auto whole) __attribute__((always_inline)) {        // left: steps before the end from the tile's first row on
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
@@ -474,7 +493,7 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
         dY *= z * sg;
         dg = dy * (sg * fmaf(z, 1.0f - sg, 1.0f));
       }
-      if (!at.on || (!whole && row + (long)k * TT >= live)) dl = du = dY = 0.0f;
+      if (!at.on || (!decltype(whole)::v && row >= left)) dl = du = dY = 0.0f;
       s_in[buf][row][ch] = make_float2(dl, du);
       s_dy[buf][row][ch] = dY;
       if (!CARRY) {
@@ -486,9 +505,12 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
   };
   const unsigned ostep = (unsigned)D * sizeof(IT), ooff = __umul24(at.row, ostep) + d * (unsigned)sizeof(IT);
   const long out0 = (b * T + at.t0) * D;
-  auto finish = [&](int k, int buf) {
+  auto finish = [&](int k, int buf, auto whole) __attribute__((always_inline)) {
     const long left = live - (long)k * TT, room = at.t1 - at.t0 - (long)k * TT;
-    const long tile = (long)k * TT * ostep;
+    const long tile = out0 * (long)sizeof(IT) + (long)k * TT * ostep;
+    char* const du = static_cast<char*>(a.g.du) + tile;
+    char* const ddelta = static_cast<char*>(a.g.ddelta) + tile;
+    char* const dz = static_cast<char*>(a.g.dz) + tile;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
@@ -500,91 +522,108 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
         s2 += s.y;
       }
       const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[0][row][ch];
-      const bool in = row < left && at.on, store = row < room && at.on;
+      const bool in = (decltype(whole)::v || row < left) && at.on, store = (decltype(whole)::v || row < room) && at.on;
       const float ddl = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
       dDk = fmaf(dY, in ? u : 0.0f, dDk);
       dbias += in ? ddl : 0.0f;
-      const long o = tile + (long)i * PS * ostep + ooff;
-      auto put = [&](void* p, float v) {
-        if (store) *reinterpret_cast<IT*>(reinterpret_cast<char*>(static_cast<IT*>(p) + out0) + o) = down<IT>(in ? v : 0.0f);
+      const long o = (long)i * PS * ostep;
+      auto put = [&](char* p, float v) __attribute__((always_inline)) {
+        if (store) *reinterpret_cast<IT*>(p + o + ooff) = down<IT>(in ? v : 0.0f);
       };
-      put(a.g.du, fmaf(dl, s1, Dk * dY));
-      put(a.g.ddelta, ddl);
+      put(du, fmaf(dl, s1, Dk * dY));
+      put(ddelta, ddl);
       if (gate) {
         float y = Dk * u;
 #pragma unroll
         for (int p = 0; p < PS; ++p) y += s_y[row][p][ch];
-        put(a.g.dz, y * s_own[2][row][ch]);
+        put(dz, y * s_own[2][row][ch]);
       }
     }
   };
 
   if (at.tiles > 0) {
-    const int p = last & 1;
-    // (the register sets are named by the tile's parity; at run time one of the two orders)
-    auto begin = [&](auto parity) {
+    // (the register sets are named by the tile's parity)
+    auto begin = [&](auto parity) __attribute__((always_inline)) {
       constexpr int P = decltype(parity)::v;
       load(rows[P], last);
       load(rows[P ^ 1], last - 1);
       load_maps(maps[P], last);
       load_maps(maps[P ^ 1], last - 1);
-      prepare(rows[P], last, P);
+      prepare(rows[P], live - (long)last * TT, P, Int<0>{});
       load(rows[P], last - 2);
     };
-    if (p) begin(Int<1>{});
+    if (last & 1) begin(Int<1>{});
     else begin(Int<0>{});
   }
   __syncthreads();
   const long part0 = ((at.blk * a.p.B + b) * T + at.t0) * N;
-  auto iteration = [&](int i, auto parity) {
+  // FAST: tiles i - 3 .. i exist and are whole
+  auto iteration = [&](int i, auto parity, auto fast) __attribute__((always_inline)) {
     constexpr int P = decltype(parity)::v;
+    constexpr bool FAST = decltype(fast)::v;
+    const long left = live - (long)i * TT;
     float B[Q], C[Q], h0[NS];
-    mC.widen(maps[P].C, C, live - (long)i * TT);
+    mC.template widen<FAST>(maps[P].C, C, left);
     if (!CARRY) {
-      mB.widen(maps[P].B, B, live - (long)i * TT);
+      mB.template widen<FAST>(maps[P].B, B, left);
 #pragma unroll
-      for (int j = 0; j < NS; ++j) h0[j] = at.n0 + j < N ? maps[P].h[j] : 0.0f;
+      for (int j = 0; j < NS; ++j) h0[j] = maps[P].h[j];
     }
-    load_maps(maps[P], i - 2);
+    if (FAST) {
+      mC.next(maps[P].C, -1);
+      if (!CARRY) {
+        mB.next(maps[P].B, -1);
+        load_h(maps[P], ck);
+        ck -= cktile;
+      }
+    } else {
+      load_maps(maps[P], i - 2);
+    }
+    auto ahead = [&]() __attribute__((always_inline)) {
+      prepare(rows[P ^ 1], FAST || i > 0 ? TT : 0, P ^ 1, fast);      // (before the first tile: not read)
+      if (FAST) {
+        su.next(rows[P ^ 1].u, -1);
+        sdl.next(rows[P ^ 1].dl, -1);
+        sdy.next(rows[P ^ 1].dy, -1);
+        sz.next(rows[P ^ 1].z, -1);
+      } else {
+        load(rows[P ^ 1], i - 3);
+      }
+    };
     if constexpr (CARRY) {
-      prepare(rows[P ^ 1], max(i - 1, 0), P ^ 1);         // (before the first tile: not read)
-      load(rows[P ^ 1], i - 3);
-      each_back<TT - 1>([&](auto tc) {
+      ahead();
+      each_back<TT - 1>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::v;
         const float dl = s_in[P][t][ch].x, dY = s_dy[P][t][ch];
         sum += dl;
-        each<NS>([&](auto jc) {
+        each<NS>([&](auto jc) __attribute__((always_inline)) {
           constexpr int j = decltype(jc)::v;
           lam[j] = exp2_hw(dl * A2[j]) * fmaf(bc<S, t, j>(C), dY, lam[j]);
         });
       });
     } else {
       float hh[TT][NS], aa[TT][NS];
-      each<TT>([&](auto tc) {
+      each<TT>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::v;
         const float2 in = s_in[P][t][ch];
-        each<NS>([&](auto jc) {
+        each<NS>([&](auto jc) __attribute__((always_inline)) {
           constexpr int j = decltype(jc)::v;
           aa[t][j] = exp2_hw(in.x * A2[j]);
           hh[t][j] = fmaf(aa[t][j], t ? hh[t ? t - 1 : 0][j] : h0[j], bc<S, t, j>(B) * in.y);
         });
-        if (gate) {
-          float y = 0.0f;
-          dot_bcast<S, t>(y, C, hh[t]);
-          s_y[t][part][ch] = y;
-        }
+        if (gate) s_y[t][part][ch] = dot_bcast<S, t>(C, hh[t]);
       });
       float tA[NS];
 #pragma unroll
       for (int j = 0; j < NS; ++j) tA[j] = 0.0f;
       ChannelSum<S> sums;
       const long room = at.t1 - at.t0 - (long)i * TT;
-      each_back<TT - 1>([&](auto tc) {
+      each_back<TT - 1>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::v;
         const float2 in = s_in[P][t][ch];
         const float dY = s_dy[P][t][ch];
-        float v[2 * NS], gg[NS], s1 = 0.0f, s2 = 0.0f;
-        each<NS>([&](auto jc) {
+        float v[2 * NS], gg[NS], s2 = 0.0f;
+        each<NS>([&](auto jc) __attribute__((always_inline)) {
           constexpr int j = decltype(jc)::v;
           const float g = fmaf(bc<S, t, j>(C), dY, lam[j]);
           gg[j] = g;
@@ -592,11 +631,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
           v[NS + j] = dY * hh[t][j];
           lam[j] = aa[t][j] * g;
           const float q = lam[j] * (t ? hh[t ? t - 1 : 0][j] : h0[j]);
-          s2 = fmaf(A2[j], q, s2);
+          s2 = j ? fmaf(A2[j], q, s2) : A2[j] * q;
           tA[j] = fmaf(q, in.x, tA[j]);
         });
-        dot_bcast<S, t>(s1, B, gg);
-        s_sum[t][part][ch] = make_float2(s1, s2);
+        s_sum[t][part][ch] = make_float2(dot_bcast<S, t>(B, gg), s2);
         using CS = ChannelSum<S>;
         float out[CS::K / CS::KG];
         if (sums.template add<t>(v, at.lane, out)) {
@@ -605,24 +643,31 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan_grad(const ScanArgs a) {
           for (int o = 0; o < CS::K / CS::KG; ++o) {
             const int k = o * CS::KG + CS::value_of(at.lane), n = at.n0 + k % NS;
             float* p = (k < NS ? a.partB : a.partC) + part0 + (long)i * TT * N;
-            if (ts < room && n < N) p[ts * (int)N + n] = out[o];
+            if ((FAST || ts < room) && n < N) p[ts * (int)N + n] = out[o];
           }
         }
       });
 #pragma unroll
       for (int j = 0; j < NS; ++j) dA[j] += tA[j];
       __syncthreads();
-      finish(i, P);
-      prepare(rows[P ^ 1], max(i - 1, 0), P ^ 1);
-      load(rows[P ^ 1], i - 3);
+      finish(i, P, fast);
+      ahead();
     }
     __syncthreads();
   };
-  int i = last;
-  if (i >= 0 && (i & 1)) iteration(i--, Int<1>{});
-  for (; i >= 0; i -= 2) {
-    iteration(i, Int<0>{});
-    if (i > 0) iteration(i - 1, Int<1>{});
+  for (int i = last; i >= 0;) {
+    if ((i & 1) && i >= 4 && i < at.full) {               // pairs (odd, even) of whole tiles
+      su.seek(i - 3), sdl.seek(i - 3), sdy.seek(i - 3), sz.seek(i - 3), mB.seek(i - 2), mC.seek(i - 2);
+      if (!CARRY) ck = ck0 + (i - 2) * cktile;
+      for (; i >= 4; i -= 2) {
+        iteration(i, Int<1>{}, Int<1>{});
+        iteration(i - 1, Int<0>{}, Int<1>{});
+      }
+    } else {
+      if (i & 1) iteration(i, Int<1>{}, Int<0>{});
+      else iteration(i, Int<0>{}, Int<0>{});
+      --i;
+    }
   }
   if constexpr (CARRY) {
     if (!at.on) return;
@@ -731,11 +776,6 @@ template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
   const long N = a.p.N;
   if (N > 32) return launch<IT, Shape<64, 8, 8, 8>>(what, a, st);
   if (N > 16) return launch<IT, Shape<64, 4, 8, 16>>(what, a, st);
-#ifdef NS4
-  if (N > 8) return launch<IT, Shape<64, 4, 4, 16>>(what, a, st);
-  if (N > 4) return launch<IT, Shape<64, 4, 2, 16>>(what, a, st);
-  return launch<IT, Shape<64, 4, 1, 16>>(what, a, st);
-#else
   if (a.ch == 32) {
     if (N > 8) return launch<IT, Shape<32, 2, 4, 16>>(what, a, st);
     if (N > 4) return launch<IT, Shape<32, 2, 2, 16>>(what, a, st);
@@ -743,9 +783,7 @@ template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
   }
   if (N > 8) return launch<IT, Shape<64, 2, 8, 16>>(what, a, st);
   if (N > 4) return launch<IT, Shape<64, 2, 4, 16>>(what, a, st);
-  if (N > 2) return launch<IT, Shape<64, 2, 2, 16>>(what, a, st);
-  return launch<IT, Shape<64, 2, 1, 16>>(what, a, st);
-#endif
+  return launch<IT, Shape<64, 2, 2, 16>>(what, a, st);
 }
 
 template <class IT> int launch_step(ScanArgs a, float* state, hipStream_t st) {
