@@ -125,9 +125,8 @@ extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_b
   float* ws = static_cast<float*>(workspace);
   a.hl = ws;
   a.sd = ws + (s.carry ? p->B * a.chunks * p->N * p->D : 0);
-  a.partB = ws + s.carry;
-  a.partC = a.partB + s.group;
-  a.partP = a.partC + s.group;
+  a.partBC = ws + s.carry;
+  a.partP = a.partBC + 2 * s.group;
   hipStream_t st = (hipStream_t)stream;
   const long n = p->B * p->T * p->G * p->N, groups = (n + 255) / 256;
   if (!grid_fits(groups, 256)) return LQG_ERR_ARG;

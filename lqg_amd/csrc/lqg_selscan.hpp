@@ -23,7 +23,7 @@ struct ScanArgs {
   long Dg, bpg, blocks, ch;      // channels of a group, blocks of `ch` of them, blocks in all
   long chunks, chunk, tiles;     // chunks of the time axis, their steps (a multiple of TT), tiles of TT steps in T
   float *hl, *sd;                // carries [B][chunks][N][D], sums of dl [B][chunks][D]
-  float *partB, *partC, *partP;  // gradients: [blocks][B][T][N] twice, [B * chunks][N + 2][D]
+  float *partBC, *partP;         // gradients: [blocks][B][T][2][N], [B * chunks][N + 2][D]
 };
 
 template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, long off) {
@@ -85,22 +85,38 @@ template <class S> __device__ inline void load_A2(const ScanArgs& a, const Place
 
 // Row t of a tile is read at a uniform pointer plus a 32-bit offset of the thread, in bytes (row strides are below 2^24 of them).  Loads
 // run two tiles ahead of their use and are never skipped, so that the counter of outstanding loads can be waited on exactly.
-template <class IT> __device__ inline IT at_byte(const char* p, unsigned off) { return *reinterpret_cast<const IT*>(p + off); }
+typedef __attribute__((address_space(1))) char gchar;          // in global memory, which a pinned pointer would no longer show
+// (the offset is made opaque where it is used: widened to 64 bits ahead of the loop, it would cost an addition an access and a second
+// register)
+template <class IT> __device__ __forceinline__ IT at_byte(const gchar* p, unsigned off) {
+  asm("" : "+v"(off));
+  return *(const __attribute__((address_space(1))) IT*)(p + off);
+}
+template <class IT> __device__ __forceinline__ void put_byte(gchar* p, unsigned off, IT v) {
+  asm("" : "+v"(off));
+  *(__attribute__((address_space(1))) IT*)(p + off) = v;
+}
+// keeps a uniform pointer in scalar registers: the optimiser would carry pointer + offset of every row along the loop, 64 bits a lane each
+template <class P> __device__ __forceinline__ void pin(P*& p) { asm("" : "+s"(p)); }
 
 // One sequence: R rows of the thread in each tile, PS apart.
 template <class IT, class S> struct Stream {
-  const char *p, *q;                          // the chunk's first row; the next tile of `next`
-  unsigned off, step;                         // the thread's first row and channel; bytes of a row
+  const gchar *p, *q;                         // the chunk's first row; the next tile of `next`
+  unsigned off[S::R], step;                   // the thread's rows and channel in a tile; bytes of a row
   __device__ Stream(const lqg_seq& s, const Place<S>& at)
-      : p(reinterpret_cast<const char*>(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st)), q(p),
-        off(__umul24(at.row, (unsigned)s.st * sizeof(IT)) + at.d * (unsigned)sizeof(IT)), step((unsigned)s.st * sizeof(IT)) {}
-  __device__ const char* tile(int k) const { return p + (long)k * S::TT * step; }
+      : p((const gchar*)(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st)), q(p),
+        step((unsigned)s.st * sizeof(IT)) {
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) off[i] = __umul24(at.row + i * S::PS, step) + at.d * (unsigned)sizeof(IT);
+  }
+  __device__ const gchar* tile(int k) const { return p + (long)k * S::TT * step; }
   __device__ void seek(int k) { q = tile(k); }
   // a whole tile, then on by `way` tiles
   __device__ void next(IT (&r)[S::R], int way) {
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) r[i] = at_byte<IT>(q + (long)i * S::PS * step, off);
+    for (int i = 0; i < S::R; ++i) r[i] = at_byte<IT>(q, off[i]);
     q += (long)way * S::TT * (int)step;
+    pin(q);
   }
   // tile k; left: steps before the end from its first row on (>= 1): rows behind the end repeat the last one
   __device__ void load(IT (&r)[S::R], int k, long left, const Place<S>& at) const {
@@ -114,23 +130,25 @@ template <class IT, class S> struct Stream {
 // a tile's B or C: value (t, j) of a lane's states in register (t NS + j) / 16, lane (t NS + j) % 16 of its row of 16
 template <class IT, class S> struct Maps {
   static constexpr int rows = 16 / S::NS;     // steps of a register
-  const char *p, *q;
-  unsigned off, step, n;
+  const gchar *p, *q;
+  unsigned off[S::Q], step, n;
   int t;
   bool ok;
   __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : step((unsigned)s.st * sizeof(IT)) {
     const int f = at.lane & 15, j = f % S::NS;
     t = f / S::NS;
-    p = q = reinterpret_cast<const char*>(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg);
+    p = q = (const gchar*)(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg);
     ok = at.n0 + j < a.p.N;
     n = (ok ? at.n0 + j : 0) * sizeof(IT);
-    off = __umul24(t, step) + n;
+#pragma unroll
+    for (int i = 0; i < S::Q; ++i) off[i] = __umul24(t + i * rows, step) + n;
   }
   __device__ void seek(int k) { q = p + (long)k * S::TT * step; }
   __device__ void next(IT (&r)[S::Q], int way) {
 #pragma unroll
-    for (int i = 0; i < S::Q; ++i) r[i] = at_byte<IT>(q + (long)i * rows * step, off);
+    for (int i = 0; i < S::Q; ++i) r[i] = at_byte<IT>(q, off[i]);
     q += (long)way * S::TT * (int)step;
+    pin(q);
   }
   __device__ void load(IT (&r)[S::Q], int k, long left) const {
     const int most = (int)min(left, (long)S::TT) - 1;
@@ -148,23 +166,58 @@ template <class S, int T, int J> __device__ inline float bc(const float (&r)[S::
   return row_bcast<(T * S::NS + J) % 16>(r[(T * S::NS + J) / 16]);
 }
 
-// sum_j bc(C)(t, j) h[j].  The broadcast is an operand modifier of the multiply-add, which the compiler folds into products only (it would
-// copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart from the broadcast's read.
-#define LQG_FMAC_BCAST(C, K, X) "v_fmac_f32_dpp %0, " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
-template <class S, int T> __device__ inline float dot_bcast(const float (&C)[S::Q], const float (&h)[S::NS]) {
+// y[g] = sum_j bc(C)(T + g, j) h[g][j] for GS steps.  The broadcast is an operand modifier of the multiply-add, which the compiler folds into
+// products only (it would copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart
+// from the broadcasts' reads; several steps in a block share them.
+template <class S> struct Group { static constexpr int GS = S::NS == 2 ? 4 : S::NS == 4 ? 2 : 1; };
+#define LQG_FMAC_BCAST(Y, C, K, X) "v_fmac_f32_dpp " Y ", " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
+template <class S, int T> __device__ __forceinline__ void dot_bcast(const float (&C)[S::Q], const float (&h)[Group<S>::GS][S::NS], float (&y)[Group<S>::GS]) {
   constexpr int f = T * S::NS, k = f % 16;
-  float y = row_bcast<k>(C[f / 16]) * h[0];
+  const float c = C[f / 16];
   if constexpr (S::NS == 2) {
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c3", "%2") : "+v"(y) : "v"(C[f / 16]), "v"(h[1]), "n"(k + 1));
+    y[0] = row_bcast<k>(c) * h[0][0], y[1] = row_bcast<k + 2>(c) * h[1][0], y[2] = row_bcast<k + 4>(c) * h[2][0], y[3] = row_bcast<k + 6>(c) * h[3][0];
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%4", "%c9", "%5") LQG_FMAC_BCAST("%1", "%4", "%c10", "%6")
+        LQG_FMAC_BCAST("%2", "%4", "%c11", "%7") LQG_FMAC_BCAST("%3", "%4", "%c12", "%8")
+        : "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3])
+        : "v"(c), "v"(h[0][1]), "v"(h[1][1]), "v"(h[2][1]), "v"(h[3][1]), "n"(k + 1), "n"(k + 3), "n"(k + 5), "n"(k + 7));
+  } else if constexpr (S::NS == 4) {
+    y[0] = row_bcast<k>(c) * h[0][0], y[1] = row_bcast<k + 4>(c) * h[1][0];
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%2", "%c9", "%3") LQG_FMAC_BCAST("%1", "%2", "%c12", "%6")
+        LQG_FMAC_BCAST("%0", "%2", "%c10", "%4") LQG_FMAC_BCAST("%1", "%2", "%c13", "%7")
+        LQG_FMAC_BCAST("%0", "%2", "%c11", "%5") LQG_FMAC_BCAST("%1", "%2", "%c14", "%8")
+        : "+v"(y[0]), "+v"(y[1])
+        : "v"(c), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[1][1]), "v"(h[1][2]), "v"(h[1][3]),
+          "n"(k + 1), "n"(k + 2), "n"(k + 3), "n"(k + 5), "n"(k + 6), "n"(k + 7));
   } else {
-    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c5", "%2") LQG_FMAC_BCAST("%1", "%c6", "%3") LQG_FMAC_BCAST("%1", "%c7", "%4")
-        : "+v"(y) : "v"(C[f / 16]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(k + 1), "n"(k + 2), "n"(k + 3));
-    if constexpr (S::NS == 8)
-      asm("s_nop 1\n\t" LQG_FMAC_BCAST("%1", "%c6", "%2") LQG_FMAC_BCAST("%1", "%c7", "%3") LQG_FMAC_BCAST("%1", "%c8", "%4")
-          LQG_FMAC_BCAST("%1", "%c9", "%5")
-          : "+v"(y) : "v"(C[f / 16]), "v"(h[4]), "v"(h[5]), "v"(h[6]), "v"(h[7]), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
+    y[0] = row_bcast<k>(c) * h[0][0];
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c9", "%2") LQG_FMAC_BCAST("%0", "%1", "%c10", "%3")
+        LQG_FMAC_BCAST("%0", "%1", "%c11", "%4") LQG_FMAC_BCAST("%0", "%1", "%c12", "%5") LQG_FMAC_BCAST("%0", "%1", "%c13", "%6")
+        LQG_FMAC_BCAST("%0", "%1", "%c14", "%7") LQG_FMAC_BCAST("%0", "%1", "%c15", "%8")
+        : "+v"(y[0])
+        : "v"(c), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[0][4]), "v"(h[0][5]), "v"(h[0][6]), "v"(h[0][7]),
+          "n"(k + 1), "n"(k + 2), "n"(k + 3), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
   }
-  return y;
+}
+// x[j] += bc(C)(T, j) f
+template <class S, int T> __device__ __forceinline__ void add_bcast(float (&x)[S::NS], const float (&C)[S::Q], float f) {
+  constexpr int at = T * S::NS, k = at % 16;
+  const float c = C[at / 16];
+  if constexpr (S::NS == 2) {
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%2", "%c4", "%3") LQG_FMAC_BCAST("%1", "%2", "%c5", "%3")
+        : "+v"(x[0]), "+v"(x[1]) : "v"(c), "v"(f), "n"(k), "n"(k + 1));
+  } else {
+#pragma unroll
+    for (int q = 0; q < S::NS; q += 4)
+      if (q == 0)
+        asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%4", "%c6", "%5") LQG_FMAC_BCAST("%1", "%4", "%c7", "%5")
+            LQG_FMAC_BCAST("%2", "%4", "%c8", "%5") LQG_FMAC_BCAST("%3", "%4", "%c9", "%5")
+            : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(c), "v"(f), "n"(k), "n"(k + 1), "n"(k + 2), "n"(k + 3));
+      else
+        asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%4", "%c6", "%5") LQG_FMAC_BCAST("%1", "%4", "%c7", "%5")
+            LQG_FMAC_BCAST("%2", "%4", "%c8", "%5") LQG_FMAC_BCAST("%3", "%4", "%c9", "%5")
+            : "+v"(x[4 % S::NS]), "+v"(x[5 % S::NS]), "+v"(x[6 % S::NS]), "+v"(x[7 % S::NS])
+            : "v"(c), "v"(f), "n"((k + 4) % 16), "n"((k + 5) % 16), "n"((k + 6) % 16), "n"((k + 7) % 16));
+  }
 }
 
 // compile-time loop: f(Int<I>) for I = 0 .. N-1, or downwards
@@ -246,8 +299,11 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     }
   };
   // Lanes past the end of the group repeat its last channel: they store the same values to the same places.
-  const unsigned ystep = (unsigned)a.p.y.st * sizeof(IT), yoff = __umul24(at.row, ystep) + d * (unsigned)sizeof(IT);
-  char* y = CARRY ? nullptr : reinterpret_cast<char*>(const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st);
+  const unsigned ystep = (unsigned)a.p.y.st * sizeof(IT);
+  unsigned yoff[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) yoff[i] = __umul24(at.row + i * PS, ystep) + d * (unsigned)sizeof(IT);
+  gchar* y = CARRY ? nullptr : (gchar*)(const_cast<IT*>(static_cast<const IT*>(a.p.y.ptr)) + b * a.p.y.sb + at.t0 * a.p.y.st);
   auto finish = [&](int buf, long left, long room, auto whole) __attribute__((always_inline)) {    // the tile at y; left: steps before the end, room: of the chunk
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -258,9 +314,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
       for (int p = 0; p < PS; ++p) v += s_y[buf][row][p][ch];
       v *= o.y;
       if (decltype(whole)::v || row < room)
-        *reinterpret_cast<IT*>(y + (long)i * PS * ystep + yoff) = down<IT>(decltype(whole)::v || row < left ? v : 0.0f);
+        put_byte(y, yoff[i], down<IT>(decltype(whole)::v || row < left ? v : 0.0f));
     }
     y += (long)TT * ystep;
+    pin(y);
   };
 
   if (at.tiles > 0) {
@@ -273,8 +330,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
   }
   __syncthreads();
   const bool keep = !CARRY && a.p.checkpoints;
-  char* ck = keep ? static_cast<char*>(a.p.checkpoints) + (b * a.tiles + at.t0 / TT) * S::NP * D * sizeof(float) : nullptr;
-  const unsigned ckoff = ((unsigned)at.n0 * (unsigned)D + d) * (unsigned)sizeof(float);
+  gchar* ck = keep ? (gchar*)a.p.checkpoints + (b * a.tiles + at.t0 / TT) * S::NP * D * sizeof(float) : nullptr;
+  unsigned ckoff[NS];
+#pragma unroll
+  for (int j = 0; j < NS; ++j) ckoff[j] = ((unsigned)(at.n0 + j) * (unsigned)D + d) * (unsigned)sizeof(float);
   // FAST: tiles i - 1 .. i + 3 exist and are whole
   auto iteration = [&](int i, auto parity, auto fast) __attribute__((always_inline)) {
     constexpr int P = decltype(parity)::v;
@@ -300,21 +359,31 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
     }
     if (!CARRY && keep) {
 #pragma unroll
-      for (int j = 0; j < NS; ++j) *reinterpret_cast<float*>(ck + (long)j * D * sizeof(float) + ckoff) = h[j];
+      for (int j = 0; j < NS; ++j) put_byte(ck, ckoff[j], h[j]);
       ck += (long)S::NP * D * sizeof(float);
+      pin(ck);
     }
     float2 in[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) in[t] = s_in[P][t][ch];
     __builtin_amdgcn_sched_barrier(0);                    // all of the tile's inputs on their way before the first is waited for
-    each<TT>([&](auto tc) __attribute__((always_inline)) {
-      constexpr int t = decltype(tc)::v;
-      each<NS>([&](auto jc) __attribute__((always_inline)) {
-        constexpr int j = decltype(jc)::v;
-        h[j] = fmaf(exp2_hw(in[t].x * A2[j]), h[j], bc<S, t, j>(B) * in[t].y);
+    constexpr int GS = Group<S>::GS;
+    each<TT / GS>([&](auto gc) __attribute__((always_inline)) {
+      constexpr int t0 = decltype(gc)::v * GS;
+      float hh[GS][NS], v[GS];
+      each<GS>([&](auto tc) __attribute__((always_inline)) {
+        constexpr int t = t0 + decltype(tc)::v;
+        each<NS>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::v;
+          hh[t - t0][j] = h[j] = fmaf(exp2_hw(in[t].x * A2[j]), h[j], bc<S, t, j>(B) * in[t].y);
+        });
+        if (CARRY) sum += in[t].x;
       });
-      if (CARRY) sum += in[t].x;
-      else s_y[P][t][part][ch] = dot_bcast<S, t>(C, h);
+      if (!CARRY) {
+        dot_bcast<S, t0>(C, hh, v);
+#pragma unroll
+        for (int k = 0; k < GS; ++k) s_y[P][t0 + k][part][ch] = v[k];
+      }
     });
     __syncthreads();
   };
@@ -343,7 +412,7 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
   if (last >= 0) finish(last & 1, live - (long)last * TT, at.t1 - at.t0 - (long)last * TT, Int<0>{});
   if (!at.on) return;
   for (long t = (long)at.tiles * TT + at.row; t < at.t1 - at.t0; t += PS, y += (long)PS * ystep)       // padding behind the last tile
-    *reinterpret_cast<IT*>(y + yoff) = down<IT>(0.0f);
+    put_byte(y, yoff[0], down<IT>(0.0f));
   if (a.p.state_out && at.c == a.chunks - 1) {
 #pragma unroll
     for (int j = 0; j < NS; ++j)
@@ -357,8 +426,10 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
 //   du = dl s1 + D dY;  d dl = s2 + u s1;  dA = sum q dl;  lambda <- a g.
 // A tile's states are recomputed from the checkpoint that the forward pass left at its start.
 
-// x and y reduced by halves: lanes whose bit BIT is 0 receive x's sum over that bit, the others y's.
-template <int BIT> __device__ inline float merge(float x, float y, int lane) {
+// x and y reduced by halves: lanes whose bit BIT is 0 receive x's sum over that bit, the others y's.  Bits 5 and 4: the halves change
+// places (one instruction) and are added.  Bits 3 and 2 name a group of 4 lanes in its row, which a DPP instruction can be masked by: x's
+// sum everywhere, y's over it where the bit is set.
+template <int BIT> __device__ __forceinline__ float merge(float x, float y, int lane) {
   if constexpr (BIT == 5) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
@@ -369,6 +440,30 @@ template <int BIT> __device__ inline float merge(float x, float y, int lane) {
     const bool hi = lane >> BIT & 1;
     const float keep = hi ? y : x, give = hi ? x : y;
     return keep + dpp<BIT == 3 ? DPP_ROR8 : BIT == 2 ? DPP_HALF_MIRROR : BIT == 1 ? DPP_XOR2 : DPP_XOR1>(give);
+  }
+}
+#define LQG_MERGE(O, X, Y, M, B) "v_add_f32_dpp " O ", " X ", " X " " M " row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp " O ", " Y ", " Y " " M " row_mask:0xf bank_mask:" B "\n\t"
+// M merges over bit BIT, in a block that waits once for what wrote its operands
+template <int BIT, int M> __device__ __forceinline__ void merge_all(float* x, const float* y, int lane) {
+  if constexpr (BIT >= 4 || BIT < 2 || M % 4) {
+#pragma unroll
+    for (int k = 0; k < M; ++k) x[k] = merge<BIT>(x[k], y[k], lane);
+  } else {
+#pragma unroll
+    for (int k = 0; k < M; k += 4) {
+      float o0, o1, o2, o3;
+      if constexpr (BIT == 3)
+        asm("s_nop 1\n\t" LQG_MERGE("%0", "%4", "%8", "row_ror:8", "0xc") LQG_MERGE("%1", "%5", "%9", "row_ror:8", "0xc")
+            LQG_MERGE("%2", "%6", "%10", "row_ror:8", "0xc") LQG_MERGE("%3", "%7", "%11", "row_ror:8", "0xc")
+            : "=&v"(o0), "=&v"(o1), "=&v"(o2), "=&v"(o3)
+            : "v"(x[k]), "v"(x[k + 1]), "v"(x[k + 2]), "v"(x[k + 3]), "v"(y[k]), "v"(y[k + 1]), "v"(y[k + 2]), "v"(y[k + 3]));
+      else
+        asm("s_nop 1\n\t" LQG_MERGE("%0", "%4", "%8", "row_half_mirror", "0xa") LQG_MERGE("%1", "%5", "%9", "row_half_mirror", "0xa")
+            LQG_MERGE("%2", "%6", "%10", "row_half_mirror", "0xa") LQG_MERGE("%3", "%7", "%11", "row_half_mirror", "0xa")
+            : "=&v"(o0), "=&v"(o1), "=&v"(o2), "=&v"(o3)
+            : "v"(x[k]), "v"(x[k + 1]), "v"(x[k + 2]), "v"(x[k + 3]), "v"(y[k]), "v"(y[k + 1]), "v"(y[k + 2]), "v"(y[k + 3]));
+      x[k] = o0, x[k + 1] = o1, x[k + 2] = o2, x[k + 3] = o3;
+    }
   }
 }
 constexpr int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
@@ -400,15 +495,13 @@ template <class S> struct ChannelSum {
       return false;
     } else {
       constexpr int BIT = log2_of(S::CH) - 1 - L;
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = merge<BIT>(v[k], held[L][k], lane);
+      merge_all<BIT, K>(v, held[L], lane);
       return level<T, L + 1>(v, lane, out);
     }
   }
   template <int M> __device__ static void values(float (&x)[KG], int lane) {
     if constexpr (M > 1) {
-#pragma unroll
-      for (int k = 0; k < M / 2; ++k) x[k] = merge<log2_of(M) - 1>(x[k], x[k + M / 2], lane);
+      merge_all<log2_of(M) - 1, M / 2>(x, x + M / 2, lane);
       values<M / 2>(x, lane);
     }
   }
@@ -440,7 +533,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     dA[j] = 0.0f;
-    lam[j] = !CARRY && a.g.dstate_out && at.n0 + j < N ? a.g.dstate_out[(b * D + d) * N + at.n0 + j] : 0.0f;
+    lam[j] = !CARRY && a.g.dstate_out && at.n0 + j < N && at.on ? a.g.dstate_out[(b * D + d) * N + at.n0 + j] : 0.0f;
   }
   if (!CARRY) {
     for (long c = a.chunks - 1; c > at.c; --c) {          // the chunks after this one
@@ -461,9 +554,11 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
   const int last = at.tiles - 1;
   const long live = at.len - at.t0;                       // steps before the end from the chunk's first on
   const long cktile = S::NP * D * (long)sizeof(float);
-  const char* const ck0 = CARRY ? nullptr : static_cast<const char*>(a.p.checkpoints) + (b * a.tiles + at.t0 / TT) * cktile;
-  const char* ck = ck0;
-  const unsigned ckoff = ((unsigned)at.n0 * (unsigned)D + d) * (unsigned)sizeof(float);
+  const gchar* const ck0 = CARRY ? nullptr : (const gchar*)a.p.checkpoints + (b * a.tiles + at.t0 / TT) * cktile;
+  const gchar* ck = ck0;
+  unsigned ckoff[NS];
+#pragma unroll
+  for (int j = 0; j < NS; ++j) ckoff[j] = ((unsigned)(at.n0 + j) * (unsigned)D + d) * (unsigned)sizeof(float);
   auto load = [&](Rows& r, int k) __attribute__((always_inline)) {
     k = max(k, 0);
     su.load(r.u, k, live - (long)k * TT, at);
@@ -471,9 +566,9 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
     sdy.load(r.dy, k, live - (long)k * TT, at);
     sz.load(r.z, k, live - (long)k * TT, at);
   };
-  auto load_h = [&](RawMaps& m, const char* p) __attribute__((always_inline)) {
+  auto load_h = [&](RawMaps& m, const gchar* p) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) m.h[j] = at_byte<float>(p + (long)j * D * sizeof(float), ckoff);
+    for (int j = 0; j < NS; ++j) m.h[j] = at_byte<float>(p, ckoff[j]);
   };
   auto load_maps = [&](RawMaps& m, int k) __attribute__((always_inline)) {
     k = max(k, 0);
@@ -503,14 +598,14 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
       }
     }
   };
-  const unsigned ostep = (unsigned)D * sizeof(IT), ooff = __umul24(at.row, ostep) + d * (unsigned)sizeof(IT);
+  const unsigned ostep = (unsigned)D * sizeof(IT);
+  unsigned ooff[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) ooff[i] = __umul24(at.row + i * PS, ostep) + d * (unsigned)sizeof(IT);
   const long out0 = (b * T + at.t0) * D;
   auto finish = [&](int k, int buf, auto whole) __attribute__((always_inline)) {
-    const long left = live - (long)k * TT, room = at.t1 - at.t0 - (long)k * TT;
-    const long tile = out0 * (long)sizeof(IT) + (long)k * TT * ostep;
-    char* const du = static_cast<char*>(a.g.du) + tile;
-    char* const ddelta = static_cast<char*>(a.g.ddelta) + tile;
-    char* const dz = static_cast<char*>(a.g.dz) + tile;
+    const int left = (int)min(live - (long)k * TT, (long)TT), room = (int)min(at.t1 - at.t0 - (long)k * TT, (long)TT);
+    float vu[R], vd[R], vz[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = at.row + i * PS;
@@ -522,21 +617,29 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
         s2 += s.y;
       }
       const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[0][row][ch];
-      const bool in = (decltype(whole)::v || row < left) && at.on, store = (decltype(whole)::v || row < room) && at.on;
-      const float ddl = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
-      dDk = fmaf(dY, in ? u : 0.0f, dDk);
-      dbias += in ? ddl : 0.0f;
-      const long o = (long)i * PS * ostep;
-      auto put = [&](char* p, float v) __attribute__((always_inline)) {
-        if (store) *reinterpret_cast<IT*>(p + o + ooff) = down<IT>(in ? v : 0.0f);
-      };
-      put(du, fmaf(dl, s1, Dk * dY));
-      put(ddelta, ddl);
+      vu[i] = fmaf(dl, s1, Dk * dY);
+      vd[i] = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
       if (gate) {
-        float y = Dk * u;
+        vz[i] = Dk * u;
 #pragma unroll
-        for (int p = 0; p < PS; ++p) y += s_y[row][p][ch];
-        put(dz, y * s_own[2][row][ch]);
+        for (int p = 0; p < PS; ++p) vz[i] += s_y[row][p][ch];
+        vz[i] *= s_own[2][row][ch];
+      }
+      const bool in = decltype(whole)::v || row < left;         // (lanes past the group's end have dY = 0, and their sums are not stored)
+      if (!in) vu[i] = vd[i] = vz[i] = 0.0f;
+      dDk = fmaf(dY, in ? u : 0.0f, dDk);
+      dbias += vd[i];
+    }
+    const long tile = out0 * (long)sizeof(IT) + (long)k * TT * ostep;
+    gchar *pu = (gchar*)a.g.du + tile, *pd = (gchar*)a.g.ddelta + tile, *pz = (gchar*)a.g.dz + tile;
+    pin(pu), pin(pd), pin(pz);
+    if (at.on) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (!decltype(whole)::v && at.row + i * PS >= room) break;
+        put_byte(pu, ooff[i], down<IT>(vu[i]));
+        put_byte(pd, ooff[i], down<IT>(vd[i]));
+        if (gate) put_byte(pz, ooff[i], down<IT>(vz[i]));
       }
     }
   };
@@ -556,7 +659,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
     else begin(Int<0>{});
   }
   __syncthreads();
-  const long part0 = ((at.blk * a.p.B + b) * T + at.t0) * N;
+  const long part0 = ((at.blk * a.p.B + b) * T + at.t0) * 2 * N;
   // FAST: tiles i - 3 .. i exist and are whole
   auto iteration = [&](int i, auto parity, auto fast) __attribute__((always_inline)) {
     constexpr int P = decltype(parity)::v;
@@ -575,6 +678,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
         mB.next(maps[P].B, -1);
         load_h(maps[P], ck);
         ck -= cktile;
+        pin(ck);
       }
     } else {
       load_maps(maps[P], i - 2);
@@ -611,9 +715,17 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
           aa[t][j] = exp2_hw(in.x * A2[j]);
           hh[t][j] = fmaf(aa[t][j], t ? hh[t ? t - 1 : 0][j] : h0[j], bc<S, t, j>(B) * in.y);
         });
-        if (gate) s_y[t][part][ch] = dot_bcast<S, t>(C, hh[t]);
       });
-      float tA[NS];
+      constexpr int GS = Group<S>::GS;
+      if (gate)
+        each<TT / GS>([&](auto gc) __attribute__((always_inline)) {
+          constexpr int t0 = decltype(gc)::v * GS;
+          float v[GS];
+          dot_bcast<S, t0>(C, reinterpret_cast<float(&)[GS][NS]>(hh[t0]), v);
+#pragma unroll
+          for (int k = 0; k < GS; ++k) s_y[t0 + k][part][ch] = v[k];
+        });
+      float tA[NS], gg[GS][NS], s2[GS];
 #pragma unroll
       for (int j = 0; j < NS; ++j) tA[j] = 0.0f;
       ChannelSum<S> sums;
@@ -622,19 +734,25 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
         constexpr int t = decltype(tc)::v;
         const float2 in = s_in[P][t][ch];
         const float dY = s_dy[P][t][ch];
-        float v[2 * NS], gg[NS], s2 = 0.0f;
+        constexpr int k = t % GS;
+        float v[2 * NS];
+        add_bcast<S, t>(lam, C, dY);                      // g
         each<NS>([&](auto jc) __attribute__((always_inline)) {
           constexpr int j = decltype(jc)::v;
-          const float g = fmaf(bc<S, t, j>(C), dY, lam[j]);
-          gg[j] = g;
-          v[j] = g * in.y;
+          gg[k][j] = lam[j];
+          v[j] = lam[j] * in.y;
           v[NS + j] = dY * hh[t][j];
-          lam[j] = aa[t][j] * g;
+          lam[j] = aa[t][j] * lam[j];
           const float q = lam[j] * (t ? hh[t ? t - 1 : 0][j] : h0[j]);
-          s2 = j ? fmaf(A2[j], q, s2) : A2[j] * q;
+          s2[k] = j ? fmaf(A2[j], q, s2[k]) : A2[j] * q;
           tA[j] = fmaf(q, in.x, tA[j]);
         });
-        s_sum[t][part][ch] = make_float2(dot_bcast<S, t>(B, gg), s2);
+        if constexpr (k == 0) {
+          float s1[GS];
+          dot_bcast<S, t>(B, gg, s1);
+#pragma unroll
+          for (int o = 0; o < GS; ++o) s_sum[t + o][part][ch] = make_float2(s1[o], s2[o]);
+        }
         using CS = ChannelSum<S>;
         float out[CS::K / CS::KG];
         if (sums.template add<t>(v, at.lane, out)) {
@@ -642,8 +760,9 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
 #pragma unroll
           for (int o = 0; o < CS::K / CS::KG; ++o) {
             const int k = o * CS::KG + CS::value_of(at.lane), n = at.n0 + k % NS;
-            float* p = (k < NS ? a.partB : a.partC) + part0 + (long)i * TT * N;
-            if ((FAST || ts < room) && n < N) p[ts * (int)N + n] = out[o];
+            gchar* p = (gchar*)(a.partBC + part0 + (long)i * TT * 2 * N);
+            pin(p);
+            if ((FAST || ts < room) && n < N) put_byte(p, (unsigned)((2 * ts + (k < NS ? 0 : 1)) * (int)N + n) * 4u, out[o]);
           }
         }
       });
@@ -711,9 +830,9 @@ template <class IT> __global__ __launch_bounds__(256) void k_scan_groups(const S
   float x = 0.0f, y = 0.0f;
   if (live)
     for (long k = g * a.bpg; k < (g + 1) * a.bpg; ++k) {
-      const long at = ((k * B + b) * T + t) * N + n;
-      x += a.partB[at];
-      y += a.partC[at];
+      const long at = ((k * B + b) * T + t) * 2 * N + n;
+      x += a.partBC[at];
+      y += a.partBC[at + N];
     }
   static_cast<IT*>(a.g.dBm)[e] = down<IT>(x);
   static_cast<IT*>(a.g.dCm)[e] = down<IT>(y);
