@@ -1,28 +1,43 @@
 // lqg_conv.hip — short causal convolution over each channel, its gradients and its single step (include/lqg_learn.h).
 //
-// y[t] = act(bias + sum_k w[k] xs[t - (W-1) + k]).  Memory bound: 2 W (+ 6 for silu) flops per element read and written.  One lane walks
-// one channel over a piece of the time axis with the last W rows in registers, so x is read once but for the W-1 rows before a piece.
+// y[t] = act(bias + sum_k w[k] xs[t - (W-1) + k]).  Memory bound: 2 W (+ 6 for silu) flops per element read and written.  One lane walks V
+// neighbouring channels over a piece of the time axis with the last W rows in registers: x is read once but for the W-1 rows before a
+// piece.  8 rows are requested before the first is used.  Vectors need no alignment beyond their elements' (the hardware takes global
+// accesses at any address), and the last vector of a row moves back to end with the row: channels that two lanes then hold get the
+// same values from both.
 #include "lqg_learn.hpp"
+
+#include <algorithm>
 
 using namespace lqg::learn;
 
 namespace {
 
 constexpr int WMAX = 8;
-constexpr int PIECE = 32;        // steps one lane walks (forward): (PIECE + W - 1) / PIECE rows read per row written
-constexpr int GPIECE = 128;      // backward: longer, since each piece leaves W + 1 partial sums per channel
+constexpr int AHEAD = 8;         // rows requested together
+constexpr int PIECE = 32;        // steps one lane walks: (PIECE + W - 1) / PIECE rows read per row written
+constexpr int MAX_GPIECE = 128;  // backward: up to this, since each piece leaves W + 1 partial sums per channel
 
 struct ConvArgs {
   lqg_conv p;
-  long pieces, blocks;           // pieces of the time axis, blocks of 256 channels
+  long pieces, piece, groups;    // pieces of the time axis, their steps; vectors of channels in a row
   lqg_seq dy;
   const void *dstate_out;
   void *dx, *dstate;
   float* part;                   // [B * pieces][(W + 1)][D]
 };
 
-template <class T> __device__ inline const T* row(const lqg_seq& s, long b, long t) {
-  return static_cast<const T*>(s.ptr) + b * s.sb + t * s.st;
+template <class T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
+template <class T, int V> __device__ inline void load_v(const T* p, float (&x)[V]) {
+  const Vec<T, V> r = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+  for (int c = 0; c < V; ++c) x[c] = up(r.v[c]);
+}
+template <class T, int V> __device__ inline void store_v(T* p, const float (&x)[V]) {
+  Vec<T, V> r;
+#pragma unroll
+  for (int c = 0; c < V; ++c) r.v[c] = down<T>(x[c]);
+  *reinterpret_cast<Vec<T, V>*>(p) = r;
 }
 
 __device__ inline long length_of(const int32_t* lengths, long b, long T) {
@@ -31,121 +46,227 @@ __device__ inline long length_of(const int32_t* lengths, long b, long T) {
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
+// where a thread is: neighbouring threads hold neighbouring channels
+template <int V> struct ConvPlace {
+  long b, piece, d, n, t0, t1;
+  bool any;
+  __device__ ConvPlace(const ConvArgs& a) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x, rest = id / a.groups;
+    any = rest < a.pieces * a.p.B;
+    d = (id - rest * a.groups) * V;
+    if (V > 1) d = min(d, a.p.D - V);
+    piece = rest % a.pieces;
+    b = rest / a.pieces;
+    t0 = piece * a.piece;
+    t1 = min(t0 + a.piece, a.p.T);
+    n = any ? length_of(a.p.lengths, b, a.p.T) : 0;
+  }
+};
+
 // row s of (state ++ x[:n]) counted from x's first step: state for s < 0
-template <class T> __device__ inline float line(const ConvArgs& a, long b, long s, long d) {
-  if (s >= 0) return up(row<T>(a.p.x, b, s)[d]);
-  if (!a.p.state) return 0.0f;
-  return up(static_cast<const T*>(a.p.state)[(b * (a.p.W - 1) + (s + a.p.W - 1)) * a.p.D + d]);
+template <class T, int V> __device__ inline void line(const ConvArgs& a, const T* x, long b, long s, long d, float (&r)[V]) {
+  if (s >= 0) return load_v<T, V>(x + s * a.p.x.st, r);
+  if (a.p.state) return load_v<T, V>(static_cast<const T*>(a.p.state) + (b * (a.p.W - 1) + (s + a.p.W - 1)) * a.p.D + d, r);
+#pragma unroll
+  for (int c = 0; c < V; ++c) r[c] = 0.0f;
 }
 
-template <class T, int W>
+template <class T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv(const ConvArgs a) {
-  const long blk = blockIdx.x % a.blocks, rest = blockIdx.x / a.blocks;
-  const long piece = rest % a.pieces, b = rest / a.pieces;
-  const long d = blk * 256 + threadIdx.x;
-  if (d >= a.p.D) return;
-  const long n = length_of(a.p.lengths, b, a.p.T);
-  const long t0 = piece * PIECE, t1 = min(t0 + PIECE, a.p.T);
-  float w[W], r[W];
+  const ConvPlace<V> at(a);
+  if (!at.any) return;
+  const long b = at.b, d = at.d, n = at.n;
+  float w[W][V], r[W][V], bias[V];                 // r: the last W - 1 rows, and the current one
 #pragma unroll
-  for (int k = 0; k < W; ++k) w[k] = load_param(a.p.w, d * W + k);
-  const float bias = a.p.bias.ptr ? load_param(a.p.bias, d) : 0.0f;
+  for (int c = 0; c < V; ++c) {
+    bias[c] = a.p.bias.ptr ? load_param(a.p.bias, d + c) : 0.0f;
 #pragma unroll
-  for (int k = 1; k < W; ++k) r[k] = t0 < n ? line<T>(a, b, t0 - W + k, d) : 0.0f;     // rows t0-(W-1) .. t0-1
-  T* y = static_cast<T*>(const_cast<void*>(a.p.y.ptr)) + b * a.p.y.sb + d;
-#pragma unroll 4
-  for (long t = t0; t < t1; ++t) {
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k) r[k] = r[k + 1];
-    const bool live = t < n;
-    r[W - 1] = live ? up(row<T>(a.p.x, b, t)[d]) : 0.0f;
-    float v = bias;
-#pragma unroll
-    for (int k = 0; k < W; ++k) v = fmaf(w[k], r[k], v);
-    if (a.p.silu) v *= sigmoid(v);
-    y[t * a.p.y.st] = down<T>(live ? v : 0.0f);
+    for (int k = 0; k < W; ++k) w[k][c] = load_param(a.p.w, (d + c) * W + k), r[k][c] = 0.0f;
   }
-  if (a.p.state_out && piece == 0) {
+  const T* x = static_cast<const T*>(a.p.x.ptr) + b * a.p.x.sb + d;
+  T* y = static_cast<T*>(const_cast<void*>(a.p.y.ptr)) + b * a.p.y.sb + d;
+  if (at.t0 < n)
+#pragma unroll
+    for (int k = 1; k < W; ++k) line<T, V>(a, x, b, at.t0 - W + k, d, r[k]);
+  auto step = [&](long t, const float (&now)[V], bool live) {
+    float v[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+#pragma unroll
+      for (int k = 0; k + 1 < W; ++k) r[k][c] = r[k + 1][c];
+      r[W - 1][c] = now[c];
+      v[c] = bias[c];
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[c] = fmaf(w[k][c], r[k][c], v[c]);
+      if (a.p.silu) v[c] *= sigmoid(v[c]);
+      if (!live) v[c] = 0.0f;
+    }
+    store_v<T, V>(y + t * a.p.y.st, v);
+  };
+  long t = at.t0;
+  for (; t + AHEAD <= min(at.t1, n); t += AHEAD) {
+    Vec<T, V> raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) raw[i] = *reinterpret_cast<const Vec<T, V>*>(x + (t + i) * a.p.x.st);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      float now[V];
+#pragma unroll
+      for (int c = 0; c < V; ++c) now[c] = up(raw[i].v[c]);
+      step(t + i, now, true);
+    }
+  }
+  for (; t < at.t1; ++t) {
+    float now[V] = {};
+    if (t < n) load_v<T, V>(x + t * a.p.x.st, now);
+    step(t, now, t < n);
+  }
+  if (a.p.state_out && at.piece == 0) {
     T* so = static_cast<T*>(a.p.state_out) + b * (W - 1) * a.p.D + d;
-    for (int k = 0; k + 1 < W; ++k) so[k * a.p.D] = down<T>(line<T>(a, b, n - (W - 1) + k, d));
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k) {
+      float s[V];
+      line<T, V>(a, x, b, n - (W - 1) + k, d, s);
+      store_v<T, V>(so + k * a.p.D, s);
+    }
   }
 }
 
 // e[t] = dy[t] act'(v[t]);  dx[s] = sum_k w[k] e[s + W-1-k];  dw[k] = sum_t e[t] xs[t - (W-1) + k];  dbias = sum_t e[t].
 // A lane recomputes v over its piece and the W-1 steps after it (whose e its last rows need), and finishes dx[t - (W-1)] at step t.
-template <class T, int W>
+template <class T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv_grad(const ConvArgs a) {
-  const long blk = blockIdx.x % a.blocks, rest = blockIdx.x / a.blocks;
-  const long piece = rest % a.pieces, b = rest / a.pieces;
-  const long d = blk * 256 + threadIdx.x, D = a.p.D;
-  if (d >= D) return;
-  const long n = length_of(a.p.lengths, b, a.p.T);
-  const long t0 = piece * GPIECE, t1 = min(t0 + GPIECE, a.p.T);
-  float w[W], r[W], e[W], dw[W], db = 0.0f;
+  const ConvPlace<V> at(a);
+  if (!at.any) return;
+  const long b = at.b, d = at.d, n = at.n, D = a.p.D;
+  float w[W][V], r[W][V], e[W][V], dw[W][V], db[V], bias[V];
 #pragma unroll
-  for (int k = 0; k < W; ++k) w[k] = load_param(a.p.w, d * W + k), e[k] = 0.0f, dw[k] = 0.0f;
-  const float bias = a.p.bias.ptr ? load_param(a.p.bias, d) : 0.0f;
+  for (int c = 0; c < V; ++c) {
+    bias[c] = a.p.bias.ptr ? load_param(a.p.bias, d + c) : 0.0f;
+    db[c] = 0.0f;
 #pragma unroll
-  for (int k = 1; k < W; ++k) r[k] = t0 < n ? line<T>(a, b, t0 - W + k, d) : 0.0f;
+    for (int k = 0; k < W; ++k) w[k][c] = load_param(a.p.w, (d + c) * W + k), r[k][c] = e[k][c] = dw[k][c] = 0.0f;
+  }
+  const T* x = static_cast<const T*>(a.p.x.ptr) + b * a.p.x.sb + d;
+  const T* dy = static_cast<const T*>(a.dy.ptr) + b * a.dy.sb + d;
   T* dx = static_cast<T*>(a.dx) + (b * a.p.T) * D + d;
   const T* so = static_cast<const T*>(a.dstate_out);
+  if (at.t0 < n)
+#pragma unroll
+    for (int k = 1; k < W; ++k) line<T, V>(a, x, b, at.t0 - W + k, d, r[k]);
+  // own: the step counts towards dw, dbias; the next W - 1 only finish rows
+  auto step = [&](const float (&now)[V], const float (&g0)[V], bool live, bool own, float (&out)[V]) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+#pragma unroll
+      for (int k = 0; k + 1 < W; ++k) r[k][c] = r[k + 1][c], e[k][c] = e[k + 1][c];
+      r[W - 1][c] = now[c];
+      float g = g0[c];
+      if (a.p.silu) {
+        float v = bias[c];
+#pragma unroll
+        for (int k = 0; k < W; ++k) v = fmaf(w[k][c], r[k][c], v);
+        const float sg = sigmoid(v);
+        g *= sg * fmaf(v, 1.0f - sg, 1.0f);
+      }
+      if (!live) g = 0.0f;
+      e[W - 1][c] = g;
+      if (own) {
+        db[c] += g;
+#pragma unroll
+        for (int k = 0; k < W; ++k) dw[k][c] = live ? fmaf(g, r[k][c], dw[k][c]) : dw[k][c];
+      }
+      out[c] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) out[c] = fmaf(w[k][c], e[W - 1 - k][c], out[c]);
+    }
+  };
   // rows before the piece belong to the piece before it; the first piece owns the state's rows
-  const long s0 = piece == 0 ? -(long)(W - 1) : t0;
-  for (long t = t0; t < t1 + W - 1; ++t) {
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k) r[k] = r[k + 1], e[k] = e[k + 1];
+  const long s0 = at.piece == 0 ? -(long)(W - 1) : at.t0;
+  auto one = [&](long t) {
     const bool live = t < n;
-    r[W - 1] = live ? up(row<T>(a.p.x, b, t)[d]) : 0.0f;
-    float g = live ? up(row<T>(a.dy, b, t)[d]) : 0.0f;
-    if (a.p.silu) {
-      float v = bias;
+    float now[V] = {}, g[V] = {}, v[V];
+    if (live) load_v<T, V>(x + t * a.p.x.st, now), load_v<T, V>(dy + t * a.dy.st, g);
+    step(now, g, live, t < at.t1, v);
+    const long s = t - (W - 1);                  // e[0] = e at s .. e[W-1] = e at s + W-1
+    if (s < s0) return;
+    if (so && s < n && s >= n - (W - 1)) {
+      float q[V];
+      load_v<T, V>(so + (b * (W - 1) + (s - (n - (W - 1)))) * D + d, q);
 #pragma unroll
-      for (int k = 0; k < W; ++k) v = fmaf(w[k], r[k], v);
-      const float sg = sigmoid(v);
-      g = live ? g * (sg * fmaf(v, 1.0f - sg, 1.0f)) : 0.0f;
+      for (int c = 0; c < V; ++c) v[c] += q[c];
     }
-    e[W - 1] = g;
-    if (t < t1 && live) {
-      db += g;
-#pragma unroll
-      for (int k = 0; k < W; ++k) dw[k] = fmaf(g, r[k], dw[k]);
-    }
-    const long s = t - (W - 1);                  // e[0] = e[s] .. e[W-1] = e[s + W-1]
-    if (s < s0) continue;
-    float v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) v = fmaf(w[k], e[W - 1 - k], v);
-    if (so && s < n && s >= n - (W - 1)) v += up(so[(b * (W - 1) + (s - (n - (W - 1)))) * D + d]);
     if (s < 0) {
-      if (a.dstate) static_cast<T*>(a.dstate)[(b * (W - 1) + s + W - 1) * D + d] = down<T>(v);
+      if (a.dstate) store_v<T, V>(static_cast<T*>(a.dstate) + (b * (W - 1) + s + W - 1) * D + d, v);
     } else {
-      dx[s * D] = down<T>(s < n ? v : 0.0f);
+      if (s >= n)
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] = 0.0f;
+      store_v<T, V>(dx + s * D, v);
+    }
+  };
+  long t = at.t0;
+  for (; t < at.t0 + (W - 1); ++t) one(t);
+  // whole runs of steps whose rows are plain ones of this piece: inside the trial and clear of what the final state's gradient touches
+  const long plain = min(at.t1, so ? n - (W - 1) : n);
+  for (; t + AHEAD <= plain; t += AHEAD) {
+    Vec<T, V> rx[AHEAD], rg[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      rx[i] = *reinterpret_cast<const Vec<T, V>*>(x + (t + i) * a.p.x.st);
+      rg[i] = *reinterpret_cast<const Vec<T, V>*>(dy + (t + i) * a.dy.st);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      float now[V], g[V], v[V];
+#pragma unroll
+      for (int c = 0; c < V; ++c) now[c] = up(rx[i].v[c]), g[c] = up(rg[i].v[c]);
+      step(now, g, true, true, v);
+      store_v<T, V>(dx + (t + i - (W - 1)) * D, v);
     }
   }
-  float* part = a.part + ((b * a.pieces + piece) * (W + 1)) * D + d;
+  for (; t < at.t1 + W - 1; ++t) one(t);
+  float* part = a.part + ((b * a.pieces + at.piece) * (W + 1)) * D + d;
 #pragma unroll
-  for (int k = 0; k < W; ++k) part[k * D] = dw[k];
-  part[W * D] = db;
+  for (int k = 0; k < W; ++k) store_v<float, V>(part + k * D, dw[k]);
+  store_v<float, V>(part + W * D, db);
 }
 
-template <class T, int W>
+// One lane per vector of channels of a trial.
+template <class T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv_step(const ConvArgs a) {
-  const long blk = blockIdx.x % a.blocks, b = blockIdx.x / a.blocks;
-  const long d = blk * 256 + threadIdx.x, D = a.p.D;
-  if (d >= D) return;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x, b = id / a.groups, D = a.p.D;
+  if (b >= a.p.B) return;
+  const long d = V > 1 ? min((id - b * a.groups) * V, D - V) : id - b * a.groups;
+  // (a vector moved back shares channels with the one before it: that one alone writes them)
+  const int first = (int)((id - b * a.groups) * V - d);
   T* st = static_cast<T*>(const_cast<void*>(a.p.state)) + b * (W - 1) * D + d;
-  const T* x = static_cast<const T*>(a.p.x.ptr) + b * a.p.x.sb;
-  T r[W];
+  Vec<T, V> r[W];
 #pragma unroll
-  for (int k = 0; k + 1 < W; ++k) r[k] = st[k * D];
-  r[W - 1] = x[d];
-  float v = a.p.bias.ptr ? load_param(a.p.bias, d) : 0.0f;
+  for (int k = 0; k + 1 < W; ++k) r[k] = *reinterpret_cast<const Vec<T, V>*>(st + k * D);
+  r[W - 1] = *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(a.p.x.ptr) + b * a.p.x.sb + d);
+  float v[V];
 #pragma unroll
-  for (int k = 0; k < W; ++k) v = fmaf(load_param(a.p.w, d * W + k), up(r[k]), v);
-  if (a.p.silu) v *= sigmoid(v);
-  static_cast<T*>(const_cast<void*>(a.p.y.ptr))[b * a.p.y.sb + d] = down<T>(v);
+  for (int c = 0; c < V; ++c) {
+    v[c] = a.p.bias.ptr ? load_param(a.p.bias, d + c) : 0.0f;
 #pragma unroll
-  for (int k = 0; k + 1 < W; ++k) st[k * D] = r[k + 1];
+    for (int k = 0; k < W; ++k) v[c] = fmaf(load_param(a.p.w, (d + c) * W + k), up(r[k].v[c]), v[c]);
+    if (a.p.silu) v[c] *= sigmoid(v[c]);
+  }
+  T* y = static_cast<T*>(const_cast<void*>(a.p.y.ptr)) + b * a.p.y.sb + d;
+  if (first == 0) {
+    store_v<T, V>(y, v);
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k) *reinterpret_cast<Vec<T, V>*>(st + k * D) = r[k + 1];
+  } else {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      if (c < first) continue;
+      y[c] = down<T>(v[c]);
+#pragma unroll
+      for (int k = 0; k + 1 < W; ++k) st[k * D + c] = r[k + 1].v[c];
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ sums over rows
@@ -185,38 +306,53 @@ __global__ __launch_bounds__(1024) void k_row_sum(const float* in, long rows, lo
   }
 }
 
-template <class T, int W>
-int launch(int what, const ConvArgs& a, long groups, hipStream_t st) {
-  if (what == 0) hipLaunchKernelGGL((k_conv<T, W>), dim3((unsigned)groups), dim3(256), 0, st, a);
-  else if (what == 1) hipLaunchKernelGGL((k_conv_grad<T, W>), dim3((unsigned)groups), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_conv_step<T, W>), dim3((unsigned)groups), dim3(256), 0, st, a);
+constexpr int VECTOR = 4;        // channels of a lane, where a row has that many
+
+template <class T, int W, int V>
+int launch(int what, ConvArgs a, hipStream_t st) {
+  a.groups = (a.p.D + V - 1) / V;
+  const long blocks = (a.groups * (what == 2 ? 1 : a.pieces) * a.p.B + 255) / 256;
+  if (!grid_fits(blocks, 256)) return LQG_ERR_ARG;
+  if (what == 0) hipLaunchKernelGGL((k_conv<T, W, V>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  else if (what == 1) hipLaunchKernelGGL((k_conv_grad<T, W, V>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_conv_step<T, W, V>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   return (int)last();
 }
 
-template <class T>
-int by_width(int what, const ConvArgs& a, long groups, hipStream_t st) {
+template <class T, int V>
+int by_width(int what, const ConvArgs& a, hipStream_t st) {
   switch (a.p.W) {
-    case 1: return launch<T, 1>(what, a, groups, st);
-    case 2: return launch<T, 2>(what, a, groups, st);
-    case 3: return launch<T, 3>(what, a, groups, st);
-    case 4: return launch<T, 4>(what, a, groups, st);
-    case 5: return launch<T, 5>(what, a, groups, st);
-    case 6: return launch<T, 6>(what, a, groups, st);
-    case 7: return launch<T, 7>(what, a, groups, st);
-    default: return launch<T, 8>(what, a, groups, st);
+    case 1: return launch<T, 1, V>(what, a, st);
+    case 2: return launch<T, 2, V>(what, a, st);
+    case 3: return launch<T, 3, V>(what, a, st);
+    case 4: return launch<T, 4, V>(what, a, st);
+    case 5: return launch<T, 5, V>(what, a, st);
+    case 6: return launch<T, 6, V>(what, a, st);
+    case 7: return launch<T, 7, V>(what, a, st);
+    default: return launch<T, 8, V>(what, a, st);
   }
 }
 
-int by_type(int what, const ConvArgs& a, long groups, hipStream_t st) {
-  if (!grid_fits(groups, 256)) return LQG_ERR_ARG;
-  if (a.p.type == LQG_T_F32) return by_width<float>(what, a, groups, st);
-  if (a.p.type == LQG_T_BF16) return by_width<bf16>(what, a, groups, st);
-  return by_width<f16>(what, a, groups, st);
+template <class T> int by_vector(int what, const ConvArgs& a, hipStream_t st) {
+  return a.p.D >= VECTOR ? by_width<T, VECTOR>(what, a, st) : by_width<T, 1>(what, a, st);
+}
+int by_type(int what, const ConvArgs& a, hipStream_t st) {
+  if (a.p.type == LQG_T_F32) return by_vector<float>(what, a, st);
+  if (a.p.type == LQG_T_BF16) return by_vector<bf16>(what, a, st);
+  return by_vector<f16>(what, a, st);
+}
+
+// Steps of a piece of the backward pass: halved while the card's SIMDs would not all have two waves.
+long gpiece(const lqg_conv* p) {
+  long s = MAX_GPIECE;
+  const long lanes = p->B * ((p->D + VECTOR - 1) / VECTOR);
+  while (s > 16 && lanes * ((p->T + s - 1) / s) < 2 * 1024 * 64) s /= 2;
+  return s;
 }
 
 int check(const lqg_conv* p, bool step) {
   if (!p) return LQG_ERR_NULL;
-  if (p->W < 1 || p->W > WMAX || p->B < 1 || p->T < 1 || p->D < 1 || (step && p->T != 1)) return LQG_ERR_ARG;
+  if (p->W < 1 || p->W > WMAX || p->B < 1 || p->T < 1 || p->D < 1 || p->D > (1 << 24) || (step && p->T != 1)) return LQG_ERR_ARG;
   if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
   for (const lqg_param* q : {&p->w, &p->bias})
     if (q->ptr && q->type != LQG_T_F32 && q->type != LQG_T_BF16 && q->type != LQG_T_F16) return LQG_ERR_ARG;
@@ -248,14 +384,14 @@ extern "C" int lqg_causal_conv(const lqg_conv* p, void* stream) {
   if (!p->y.ptr) return LQG_ERR_NULL;
   ConvArgs a{};
   a.p = *p;
+  a.piece = PIECE;
   a.pieces = (p->T + PIECE - 1) / PIECE;
-  a.blocks = (p->D + 255) / 256;
-  return by_type(0, a, a.blocks * a.pieces * p->B, (hipStream_t)stream);
+  return by_type(0, a, (hipStream_t)stream);
 }
 
 extern "C" size_t lqg_causal_conv_grad_workspace(const lqg_conv* p) {
   if (check(p, false)) return 0;
-  const long rows = p->B * ((p->T + GPIECE - 1) / GPIECE), cols = (p->W + 1) * p->D;
+  const long rows = p->B * ((p->T + gpiece(p) - 1) / gpiece(p)), cols = (p->W + 1) * p->D;
   return (size_t)(rows + row_sum_mid_rows(rows)) * cols * sizeof(float);
 }
 
@@ -266,14 +402,14 @@ extern "C" int lqg_causal_conv_grad(const lqg_conv* p, lqg_seq dy, const void* d
   if (workspace_bytes < lqg_causal_conv_grad_workspace(p)) return LQG_ERR_WORKSPACE;
   ConvArgs a{};
   a.p = *p;
-  a.pieces = (p->T + GPIECE - 1) / GPIECE;
-  a.blocks = (p->D + 255) / 256;
+  a.piece = gpiece(p);
+  a.pieces = (p->T + a.piece - 1) / a.piece;
   a.dy = dy;
   a.dstate_out = dstate_out;
   a.dx = dx;
   a.dstate = dstate;
   a.part = static_cast<float*>(workspace);
-  if (const int rc = by_type(1, a, a.blocks * a.pieces * p->B, (hipStream_t)stream)) return rc;
+  if (const int rc = by_type(1, a, (hipStream_t)stream)) return rc;
   if (!dw && !dbias) return 0;
   const long rows = p->B * a.pieces, cols = (p->W + 1) * p->D;
   RowSum s{a.part, rows, cols, a.part + rows * cols};
@@ -297,6 +433,5 @@ extern "C" int lqg_causal_conv_step(const lqg_conv* p, void* stream) {
   if (!p->y.ptr) return LQG_ERR_NULL;
   ConvArgs a{};
   a.p = *p;
-  a.blocks = (p->D + 255) / 256;
-  return by_type(2, a, a.blocks * p->B, (hipStream_t)stream);
+  return by_type(2, a, (hipStream_t)stream);
 }
