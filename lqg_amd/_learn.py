@@ -1,5 +1,7 @@
 """ctypes mirror of include/lqg_learn.h: the learned-filter operators (lqg_amd.belief.ssm) and the AdamW step (lqg_amd.optim)."""
+import contextlib
 import ctypes as C
+import struct
 
 import torch
 
@@ -11,31 +13,18 @@ TYPES = {torch.float32: T_F32, torch.bfloat16: T_BF16, torch.float16: T_F16, tor
 SEQ_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+# The operators' descriptions are packed into bytes, whose address is what the entry points take: the structs of the header field by
+# field, in native alignment (csrc/lqg_learn.hpp asserts the same sizes).  A ctypes.Structure costs a microsecond for every nested one.
+_SEQ, _PARAM = "Pqqq", "Pii"
+CONV = struct.Struct("@4i3q" + 2 * _SEQ + 2 * _PARAM + "3P")                   # lqg_conv
+SELSCAN = struct.Struct("@2i5q" + 6 * _SEQ + 3 * _PARAM + "4P2i")              # lqg_selscan
+SELSCAN_BARS = struct.Struct("@" + _SEQ + "10P")                               # lqg_selscan_bars
+SEQ = struct.Struct("@" + _SEQ)
+NO_SEQ, NO_PARAM = (0, 0, 0, 0), (0, 0, 0)
+
+
 class Seq(C.Structure):
     _fields_ = [("ptr", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sg", C.c_int64)]
-
-
-class Param(C.Structure):
-    _fields_ = [("ptr", C.c_void_p), ("type", C.c_int32), ("pad", C.c_int32)]
-
-
-class Conv(C.Structure):
-    _fields_ = [("type", C.c_int32), ("W", C.c_int32), ("silu", C.c_int32), ("pad", C.c_int32), ("B", C.c_int64), ("T", C.c_int64),
-                ("D", C.c_int64), ("x", Seq), ("y", Seq), ("w", Param), ("bias", Param), ("state", C.c_void_p),
-                ("state_out", C.c_void_p), ("lengths", C.c_void_p)]
-
-
-class SelScan(C.Structure):
-    _fields_ = [("type", C.c_int32), ("softplus", C.c_int32), ("B", C.c_int64), ("T", C.c_int64), ("D", C.c_int64), ("N", C.c_int64),
-                ("G", C.c_int64), ("u", Seq), ("delta", Seq), ("z", Seq), ("Bm", Seq), ("Cm", Seq), ("y", Seq), ("A", Param),
-                ("Dskip", Param), ("delta_bias", Param), ("state", C.c_void_p), ("state_out", C.c_void_p), ("lengths", C.c_void_p),
-                ("checkpoints", C.c_void_p), ("chunks", C.c_int32), ("channels", C.c_int32)]
-
-
-class SelScanBars(C.Structure):
-    _fields_ = [("dy", Seq), ("dstate_out", C.c_void_p), ("du", C.c_void_p), ("ddelta", C.c_void_p), ("dz", C.c_void_p),
-                ("dBm", C.c_void_p), ("dCm", C.c_void_p), ("dA", C.c_void_p), ("dD", C.c_void_p), ("ddelta_bias", C.c_void_p),
-                ("dstate", C.c_void_p)]
 
 
 class AdamW(C.Structure):
@@ -57,18 +46,18 @@ def load():
         if not hasattr(lib, "lqg_selective_scan"):
             raise LqgHipError(f"{_abi.LIB_PATH} holds no learned-filter operators: build it again "
                               "(python -c 'import __graft_entry__ as g; g.build()')")
-        V, Z, I = C.c_void_p, C.c_size_t, C.c_int
+        V, Z, I, P = C.c_void_p, C.c_size_t, C.c_int, C.c_char_p
         for name, args, res in (
-                ("causal_conv", [C.POINTER(Conv), V], I),
-                ("causal_conv_grad_workspace", [C.POINTER(Conv)], Z),
-                ("causal_conv_grad", [C.POINTER(Conv), Seq, V, V, V, V, V, V, Z, V], I),
-                ("causal_conv_step", [C.POINTER(Conv), V], I),
-                ("selscan_workspace", [C.POINTER(SelScan)], Z),
-                ("selscan_checkpoint_bytes", [C.POINTER(SelScan)], Z),
-                ("selscan_grad_workspace", [C.POINTER(SelScan)], Z),
-                ("selective_scan", [C.POINTER(SelScan), V, Z, V], I),
-                ("selective_scan_grad", [C.POINTER(SelScan), C.POINTER(SelScanBars), V, Z, V], I),
-                ("selective_scan_step", [C.POINTER(SelScan), V, V], I),
+                ("causal_conv", [P, V], I),
+                ("causal_conv_grad_workspace", [P], Z),
+                ("causal_conv_grad", [P, Seq, V, V, V, V, V, V, Z, V], I),
+                ("causal_conv_step", [P, V], I),
+                ("selscan_workspace", [P], Z),
+                ("selscan_checkpoint_bytes", [P], Z),
+                ("selscan_grad_workspace", [P], Z),
+                ("selective_scan", [P, V, Z, V], I),
+                ("selective_scan_grad", [P, P, V, Z, V], I),
+                ("selective_scan_step", [P, V, V], I),
                 ("adamw_step", [C.POINTER(AdamW), V], I),
                 ("adamw_advance", [V, C.c_double, C.c_double, V], I)):
             fn = getattr(lib, "lqg_" + name)
@@ -78,30 +67,39 @@ def load():
 
 
 def stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(device):
-    """`with` block in which `device` is the current one; free when it already is."""
-    return torch.cuda.device(device)
+    """`with` block in which `device` is the current one."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def seq(t):
-    """[B, T, D] or [B, T, G, N] (channel stride 1) -> its view."""
-    return Seq(None, 0, 0, 0) if t is None else Seq(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2) if t.dim() == 4 else 0)
+    """[B, T, D] or [B, T, G, N] (channel stride 1): pointer, trial, time and group strides."""
+    if t is None:
+        return NO_SEQ
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1], st[2] if len(st) == 4 else 0
 
 
 def row(t):
-    """[B, D] or [B, G, N]: one step -> its view."""
-    return Seq(None, 0, 0, 0) if t is None else Seq(t.data_ptr(), t.stride(0), 0, t.stride(1) if t.dim() == 3 else 0)
+    """[B, D] or [B, G, N]: the same of one step."""
+    if t is None:
+        return NO_SEQ
+    st = t.stride()
+    return t.data_ptr(), st[0], 0, st[1] if len(st) == 3 else 0
 
 
 def param(t):
-    return Param(None, 0, 0) if t is None else Param(t.data_ptr(), TYPES[t.dtype], 0)
+    return NO_PARAM if t is None else (t.data_ptr(), TYPES[t.dtype], 0)
 
 
 def scratch(nbytes, device):

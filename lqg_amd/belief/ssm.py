@@ -11,8 +11,6 @@ states of the scan, and all arithmetic, are float32.  Any trial / time strides a
 output); a channel stride other than 1 costs a copy.  `lengths` [trial] (int32 or int64, on the device) marks padded trials: outputs
 and gradients at and behind a trial's length are 0, its state is that after its last step, and what the padding holds — NaN included —
 is never used.  Lengths outside 0..T count as the nearer end.  Computation is on the GPU only; no call synchronises."""
-import ctypes as C
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -22,100 +20,103 @@ from lqg_amd._abi import LqgHipError
 MAX_WIDTH, MAX_STATES, MAX_STRIDE = 8, 64, (1 << 22) - 1
 
 
-def _need(ok, what):
-    if not ok:
-        raise LqgHipError(what)
+def _got(t):
+    return f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
 
 
 def _sequence(t, name, dims, like=None):
-    _need(isinstance(t, torch.Tensor) and t.dim() == dims, f"{name}: a tensor of {dims} dimensions is needed, got "
-          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
-    _need(t.dtype in _learn.SEQ_TYPES, f"{name}: float32, bfloat16 or float16 is needed, got {t.dtype}")
-    if like is not None:
-        _need(t.dtype == like.dtype and t.device == like.device,
-              f"{name}: {t.dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise LqgHipError(f"{name}: a tensor of {dims} dimensions is needed, got {_got(t)}")
+    if t.dtype not in _learn.SEQ_TYPES:
+        raise LqgHipError(f"{name}: float32, bfloat16 or float16 is needed, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise LqgHipError(f"{name}: {t.dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
     return t if _as_it_is(t) else t.contiguous()
 
 
 def _as_it_is(t):
     """Channels next to each other, and steps near enough for the kernels' 32-bit offsets inside a tile."""
-    return (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) <= MAX_STRIDE)
+    st = t.stride()
+    return (st[-1] == 1 or t.shape[-1] == 1) and (len(st) < 3 or st[1] <= MAX_STRIDE)
 
 
 def _on_gpu(t):
-    _need(t.device.type == "cuda", f"lqg_amd computes on MI355X only: tensors are on '{t.device}'; there is no CPU fallback")
+    if t.device.type != "cuda":
+        raise LqgHipError(f"lqg_amd computes on MI355X only: tensors are on '{t.device}'; there is no CPU fallback")
 
 
 def _parameter(t, name, shape, like):
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == shape, f"{name}: shape {shape} is needed, got "
-          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
-    _need(t.dtype in _learn.SEQ_TYPES and t.device == like.device,
-          f"{name}: float32, bfloat16 or float16 on {like.device} is needed, got {t.dtype} on {t.device}")
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
+        raise LqgHipError(f"{name}: shape {tuple(shape)} is needed, got {_got(t)}")
+    if t.dtype not in _learn.SEQ_TYPES or t.device != like.device:
+        raise LqgHipError(f"{name}: float32, bfloat16 or float16 on {like.device} is needed, got {t.dtype} on {t.device}")
     return t.contiguous()
 
 
 def _state(t, name, shape, dtype, like, in_place=False):
     if t is None:
+        if in_place:
+            raise LqgHipError(f"{name}: {dtype} {shape} is needed")
         return None
-    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype and t.device == like.device,
-          f"{name}: {dtype} {shape} on {like.device} is needed, got "
-          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t).__name__}")
-    if in_place:
-        _need(t.is_contiguous(), f"{name}: a contiguous tensor is needed, since the step moves it on in place")
-        return t
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != like.device:
+        raise LqgHipError(f"{name}: {dtype} {shape} on {like.device} is needed, got {_got(t)}")
+    if in_place and not t.is_contiguous():
+        raise LqgHipError(f"{name}: a contiguous tensor is needed, since the step moves it on in place")
     return t.contiguous()
 
 
 def _lengths(t, B, like):
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and tuple(t.shape) == (B,) and t.dtype in (torch.int32, torch.int64) and t.device == like.device,
-          f"lengths: int32 or int64 [{B}] on {like.device} is needed")
+    if not isinstance(t, torch.Tensor) or t.shape != (B,) or t.dtype not in (torch.int32, torch.int64) or t.device != like.device:
+        raise LqgHipError(f"lengths: int32 or int64 [{B}] on {like.device} is needed, got {_got(t)}")
     # (clamped before the narrowing, which would wrap)
     return (t.clamp(0, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t).contiguous()
 
 
+def _tracked(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 def _no_gradient(what, instead, *tensors):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if _tracked(*tensors):
         raise LqgHipError(f"{what} has no gradient (its state is moved on in place): call it under torch.no_grad(), or {instead}")
 
 
 def _separate(state, name, *others):
     """An in-place state must not be read through another argument while it is written."""
-    if state is None or not state.numel():
-        return
-    lo, hi = state.data_ptr(), state.data_ptr() + state.numel() * state.element_size()
+    lo = state.data_ptr()
+    hi = lo + state.numel() * state.element_size()
     for t in others:
-        if t is not None and t.numel():
-            a = t.data_ptr()
-            b = a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-            _need(b <= lo or a >= hi, f"{name}: it shares memory with another argument")
+        if t is not None and t.data_ptr() < hi:
+            end = t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            if end > lo and hi > lo and t.numel():
+                raise LqgHipError(f"{name}: it shares memory with another argument")
 
 
 # ------------------------------------------------------------------------------------------------ short causal convolution
 
-def _conv_args(x, w, bias, silu):
-    p = _learn.Conv()
-    p.type, p.W, p.silu = _learn.TYPES[x.dtype], w.shape[1], int(bool(silu))
-    p.w, p.bias = _learn.param(w), _learn.param(bias)
-    return p
+def _conv_desc(x, w, bias, silu, B, T, D, xv, yv, state, state_out, lengths):
+    return _learn.CONV.pack(_learn.TYPES[x.dtype], w.shape[1], silu, 0, B, T, D, *xv, *yv, *_learn.param(w), *_learn.param(bias),
+                            _learn.ptr(state), _learn.ptr(state_out), _learn.ptr(lengths))
+
+
+def _conv_forward(x, w, bias, state, lengths, silu, want_state):
+    B, T, D = x.shape
+    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    last = torch.empty((B, w.shape[1] - 1, D), dtype=x.dtype, device=x.device) if want_state else None
+    p = _conv_desc(x, w, bias, silu, B, T, D, _learn.seq(x), _learn.seq(y), state, last, lengths)
+    with _learn.on_device(x.device):
+        _abi.check(_learn.load().lqg_causal_conv(p, _learn.stream(x.device)), "lqg_causal_conv")
+    return y, last
 
 
 class _Conv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, state, lengths, silu, want_state):
-        B, T, D = x.shape
-        W = w.shape[1]
-        y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-        last = torch.empty((B, W - 1, D), dtype=x.dtype, device=x.device) if want_state else None
-        lib = _learn.load()
-        p = _conv_args(x, w, bias, silu)
-        p.B, p.T, p.D, p.x, p.y = B, T, D, _learn.seq(x), _learn.seq(y)
-        p.state, p.state_out, p.lengths = _learn.ptr(state), _learn.ptr(last), _learn.ptr(lengths)
-        with _learn.on_device(x.device):
-            _abi.check(lib.lqg_causal_conv(C.byref(p), _learn.stream(x.device)), "lqg_causal_conv")
+        y, last = _conv_forward(x, w, bias, state, lengths, silu, want_state)
         ctx.save_for_backward(x, w, bias, state, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -137,13 +138,11 @@ class _Conv(torch.autograd.Function):
         dw, dbias = torch.empty_like(w), None if bias is None else torch.empty_like(bias)
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
-        p = _conv_args(x, w, bias, ctx.silu)
-        p.B, p.T, p.D, p.x = B, T, D, _learn.seq(x)
-        p.state, p.lengths = _learn.ptr(state), _learn.ptr(lengths)
+        p = _conv_desc(x, w, bias, ctx.silu, B, T, D, _learn.seq(x), _learn.NO_SEQ, state, None, lengths)
         with _learn.on_device(dev):
-            n = lib.lqg_causal_conv_grad_workspace(C.byref(p))
+            n = lib.lqg_causal_conv_grad_workspace(p)
             ws = _learn.scratch(n, dev)
-            _abi.check(lib.lqg_causal_conv_grad(C.byref(p), _learn.seq(dy), _learn.ptr(dlast), _learn.ptr(dx), _learn.ptr(dstate),
+            _abi.check(lib.lqg_causal_conv_grad(p, _learn.Seq(*_learn.seq(dy)), _learn.ptr(dlast), _learn.ptr(dx), _learn.ptr(dstate),
                                                 _learn.ptr(dw), _learn.ptr(dbias), _learn.ptr(ws), n, _learn.stream(dev)),
                        "lqg_causal_conv_grad")
         return dx, dw, dbias, dstate, None, None, None
@@ -152,9 +151,9 @@ class _Conv(torch.autograd.Function):
 def _conv_check(x, weight, bias, dims):
     x = _sequence(x, "x", dims)
     D = x.shape[-1]
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] == D and 1 <= weight.shape[1] <= MAX_WIDTH,
-          f"weight: shape ({D}, 1 .. {MAX_WIDTH}) is needed")
-    return x, _parameter(weight, "weight", tuple(weight.shape), x), _parameter(bias, "bias", (D,), x)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] != D or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise LqgHipError(f"weight: shape ({D}, 1 .. {MAX_WIDTH}) is needed, got {_got(weight)}")
+    return x, _parameter(weight, "weight", weight.shape, x), _parameter(bias, "bias", (D,), x)
 
 
 def causal_conv(x, weight, bias=None, *, state=None, lengths=None, silu=False, return_state=False):
@@ -171,7 +170,8 @@ def causal_conv(x, weight, bias=None, *, state=None, lengths=None, silu=False, r
     _on_gpu(x)
     if not x.numel():
         return _empty_conv(x, w, bias, state, return_state)
-    y, last = _Conv.apply(x, w, bias, state, lengths, bool(silu), bool(return_state))
+    run = _Conv.apply if _tracked(x, w, bias, state) else _conv_forward
+    y, last = run(x, w, bias, state, lengths, int(bool(silu)), bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -196,50 +196,56 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False):
     x, w, bias = _conv_check(x, weight, bias, 2)
     B, D = x.shape
     W = w.shape[1]
-    _need(state is not None, f"state: {(B, W - 1, D)} is needed")
     state = _state(state, "state", (B, W - 1, D), x.dtype, x, in_place=True)
     _separate(state, "state", x, w, bias)
     _on_gpu(x)
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
     if not y.numel():
         return y
-    p = _conv_args(x, w, bias, silu)
-    p.B, p.T, p.D, p.x, p.y, p.state = B, 1, D, _learn.row(x), _learn.row(y), _learn.ptr(state)
+    p = _conv_desc(x, w, bias, int(bool(silu)), B, 1, D, _learn.row(x), _learn.row(y), state, None, None)
     with _learn.on_device(x.device):
-        _abi.check(_learn.load().lqg_causal_conv_step(C.byref(p), _learn.stream(x.device)), "lqg_causal_conv_step")
+        _abi.check(_learn.load().lqg_causal_conv_step(p, _learn.stream(x.device)), "lqg_causal_conv_step")
     torch.autograd.graph.increment_version(state)
     return y
 
 
 # ------------------------------------------------------------------------------------------------ selective scan
 
-def _scan_args(u, A, G, D, delta_bias, softplus):
-    p = _learn.SelScan()
-    p.type, p.softplus = _learn.TYPES[u.dtype], int(softplus)
-    p.D, p.N, p.G = u.shape[-1], A.shape[1], G
-    p.chunks, p.channels = options.get("SELSCAN_CHUNKS"), options.get("SELSCAN_CHANNELS")
-    p.A, p.Dskip, p.delta_bias = _learn.param(A), _learn.param(D), _learn.param(delta_bias)
-    return p
+def _scan_desc(u, A, G, D, delta_bias, softplus, B, T, seqs, state, last, lengths, checkpoints, chunks=0, channels=0):
+    u_, delta, z, Bm, Cm, y = seqs
+    return _learn.SELSCAN.pack(_learn.TYPES[u.dtype], softplus, B, T, u.shape[-1], A.shape[1], G, *u_, *delta, *z, *Bm, *Cm, *y,
+                               *_learn.param(A), *_learn.param(D), *_learn.param(delta_bias), _learn.ptr(state), _learn.ptr(last),
+                               _learn.ptr(lengths), _learn.ptr(checkpoints), chunks, channels)
+
+
+def _cuts():
+    return options.get("SELSCAN_CHUNKS"), options.get("SELSCAN_CHANNELS")
+
+
+def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
+    """y, the last state, the checkpoints (keep)."""
+    nB, T, nD = u.shape
+    N, G, dev = A.shape[1], Bm.shape[2], u.device
+    y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
+    last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
+    lib = _learn.load()
+    seqs, cuts = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], _cuts()
+    desc = lambda ck: _scan_desc(u, A, G, D, delta_bias, softplus, nB, T, seqs, state, last, lengths, ck, *cuts)  # noqa: E731
+    p, ck = desc(None), None
+    with _learn.on_device(dev):
+        if keep:
+            ck = _learn.scratch(lib.lqg_selscan_checkpoint_bytes(p), dev)
+            p = desc(ck)
+        n = lib.lqg_selscan_workspace(p)
+        ws = _learn.scratch(n, dev)
+        _abi.check(lib.lqg_selective_scan(p, _learn.ptr(ws), n, _learn.stream(dev)), "lqg_selective_scan")
+    return y, last, ck
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
-        nB, T, nD = u.shape
-        N, G, dev = A.shape[1], Bm.shape[2], u.device
-        y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
-        last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
-        lib = _learn.load()
-        p = _scan_args(u, A, G, D, delta_bias, softplus)
-        p.B, p.T = nB, T
-        p.u, p.delta, p.z, p.Bm, p.Cm, p.y = (_learn.seq(t) for t in (u, delta, z, Bm, Cm, y))
-        p.state, p.state_out, p.lengths = _learn.ptr(state), _learn.ptr(last), _learn.ptr(lengths)
-        with _learn.on_device(dev):
-            ck = _learn.scratch(lib.lqg_selscan_checkpoint_bytes(C.byref(p)), dev) if keep else None
-            p.checkpoints = _learn.ptr(ck)
-            n = lib.lqg_selscan_workspace(C.byref(p))
-            ws = _learn.scratch(n, dev)
-            _abi.check(lib.lqg_selective_scan(C.byref(p), _learn.ptr(ws), n, _learn.stream(dev)), "lqg_selective_scan")
+    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state):
+        y, last, ck = _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, True)
         ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -250,7 +256,7 @@ class _Scan(torch.autograd.Function):
     def backward(ctx, dy, dlast):
         u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck = ctx.saved_tensors
         if dy is None and dlast is None:
-            return (None,) * 13
+            return (None,) * 12
         nB, T, nD = u.shape
         N, G, dev = A.shape[1], Bm.shape[2], u.device
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
@@ -262,20 +268,14 @@ class _Scan(torch.autograd.Function):
         dD, dbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
-        p = _scan_args(u, A, G, D, delta_bias, ctx.softplus)
-        p.B, p.T = nB, T
-        p.u, p.delta, p.z, p.Bm, p.Cm = (_learn.seq(t) for t in (u, delta, z, Bm, Cm))
-        p.lengths, p.checkpoints = _learn.ptr(lengths), _learn.ptr(ck)
-        g = _learn.SelScanBars()
-        g.dy, g.dstate_out, g.dstate = _learn.seq(dy), _learn.ptr(dlast), _learn.ptr(dstate)
-        g.du, g.ddelta, g.dz, g.dBm, g.dCm = (_learn.ptr(t) for t in (du, ddelta, dz, dBm, dCm))
-        g.dA, g.dD, g.ddelta_bias = _learn.ptr(dA), _learn.ptr(dD), _learn.ptr(dbias)
+        seqs = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, None)]
+        p = _scan_desc(u, A, G, D, delta_bias, ctx.softplus, nB, T, seqs, None, None, lengths, ck, *_cuts())
+        g = _learn.SELSCAN_BARS.pack(*_learn.seq(dy), *(_learn.ptr(t) for t in (dlast, du, ddelta, dz, dBm, dCm, dA, dD, dbias, dstate)))
         with _learn.on_device(dev):
-            n = lib.lqg_selscan_grad_workspace(C.byref(p))
+            n = lib.lqg_selscan_grad_workspace(p)
             ws = _learn.scratch(n, dev)
-            _abi.check(lib.lqg_selective_scan_grad(C.byref(p), C.byref(g), _learn.ptr(ws), n, _learn.stream(dev)),
-                       "lqg_selective_scan_grad")
-        return du, ddelta, dA, dBm, dCm, dD, dz, dbias, dstate, None, None, None, None
+            _abi.check(lib.lqg_selective_scan_grad(p, g, _learn.ptr(ws), n, _learn.stream(dev)), "lqg_selective_scan_grad")
+        return du, ddelta, dA, dBm, dCm, dD, dz, dbias, dstate, None, None, None
 
 
 def _scan_check(u, delta, A, B, C_, D, z, delta_bias, dims):
@@ -284,20 +284,22 @@ def _scan_check(u, delta, A, B, C_, D, z, delta_bias, dims):
     delta = _sequence(delta, "delta", dims, u)
     z = None if z is None else _sequence(z, "z", dims, u)
     for t, name in ((delta, "delta"), (z, "z")):
-        _need(t is None or t.shape == u.shape, f"{name}: the shape of u, {tuple(u.shape)}, is needed")
-    _need(isinstance(A, torch.Tensor) and A.dim() == 2 and A.shape[0] == nD and 1 <= A.shape[1] <= MAX_STATES,
-          f"A: shape ({nD}, 1 .. {MAX_STATES}) is needed")
-    A = _parameter(A, "A", tuple(A.shape), u)
-    N = A.shape[1]
+        if t is not None and t.shape != u.shape:
+            raise LqgHipError(f"{name}: the shape of u, {tuple(u.shape)}, is needed, got {_got(t)}")
+    if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != nD or not 1 <= A.shape[1] <= MAX_STATES:
+        raise LqgHipError(f"A: shape ({nD}, 1 .. {MAX_STATES}) is needed, got {_got(A)}")
+    A = _parameter(A, "A", A.shape, u)
+    N, lead = A.shape[1], u.shape[:-1]
     maps = []
     for t, name in ((B, "B"), (C_, "C")):
         if isinstance(t, torch.Tensor) and t.dim() == dims:
             t = t.unsqueeze(-2)                    # one group
         t = _sequence(t, name, dims + 1, u)
-        _need(t.shape[:-2] == u.shape[:-1] and t.shape[-1] == N and t.shape[-2] >= 1 and nD % t.shape[-2] == 0,
-              f"{name}: shape {tuple(u.shape[:-1])} + (groups that divide {nD}, {N}) is needed, got {tuple(t.shape)}")
+        if t.shape[:-2] != lead or t.shape[-1] != N or t.shape[-2] < 1 or nD % t.shape[-2]:
+            raise LqgHipError(f"{name}: shape {tuple(lead)} + (groups that divide {nD}, {N}) is needed, got {_got(t)}")
         maps.append(t)
-    _need(maps[0].shape == maps[1].shape, "B and C: the same groups are needed")
+    if maps[0].shape != maps[1].shape:
+        raise LqgHipError("B and C: the same groups are needed")
     return u, delta, A, *maps, _parameter(D, "D", (nD,), u), z, _parameter(delta_bias, "delta_bias", (nD,), u)
 
 
@@ -316,12 +318,15 @@ def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softpl
     lengths = _lengths(lengths, nB, u)
     _on_gpu(u)
     inputs = (u, delta, A, Bm, Cm, D, z, delta_bias, state)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    keep = _tracked(*inputs)
     if not u.numel():
         y = u * 1 + _zero_like_sum(*inputs[1:]) if keep else u.clone()
         last = torch.zeros((nB, nD, A.shape[1]), dtype=torch.float32, device=u.device) if state is None else state.clone()
         return (y, last) if return_state else y
-    y, last = _Scan.apply(*inputs, lengths, bool(softplus), bool(return_state), keep)
+    if keep:
+        y, last = _Scan.apply(*inputs, lengths, int(bool(softplus)), bool(return_state))
+    else:
+        y, last, _ = _scan_forward(*inputs, lengths, int(bool(softplus)), bool(return_state), False)
     return (y, last) if return_state else y
 
 
@@ -331,18 +336,15 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, *, z=None, delta_bias=
     _no_gradient("selective_scan_step", "use selective_scan", u, delta, state, A, B, C, D, z, delta_bias)
     u, delta, A, Bm, Cm, D, z, delta_bias = _scan_check(u, delta, A, B, C, D, z, delta_bias, 2)
     nB, nD = u.shape
-    _need(state is not None, f"state: {(nB, nD, A.shape[1])} is needed")
     state = _state(state, "state", (nB, nD, A.shape[1]), torch.float32, u, in_place=True)
     _separate(state, "state", u, delta, A, Bm, Cm, D, z, delta_bias)
     _on_gpu(u)
     y = torch.empty((nB, nD), dtype=u.dtype, device=u.device)
     if not y.numel():
         return y
-    p = _scan_args(u, A, Bm.shape[1], D, delta_bias, softplus)
-    p.B, p.T = nB, 1
-    p.u, p.delta, p.z, p.Bm, p.Cm, p.y = (_learn.row(t) for t in (u, delta, z, Bm, Cm, y))
-    lib = _learn.load()
+    p = _scan_desc(u, A, Bm.shape[1], D, delta_bias, int(bool(softplus)), nB, 1, [_learn.row(t) for t in (u, delta, z, Bm, Cm, y)],
+                   None, None, None, None)
     with _learn.on_device(u.device):
-        _abi.check(lib.lqg_selective_scan_step(p, state.data_ptr(), _learn.stream(u.device)), "lqg_selective_scan_step")
+        _abi.check(_learn.load().lqg_selective_scan_step(p, state.data_ptr(), _learn.stream(u.device)), "lqg_selective_scan_step")
     torch.autograd.graph.increment_version(state)
     return y

@@ -6,6 +6,9 @@
 #include "../../include/lqg_hip.h"
 #include "../../include/lqg_learn.h"
 
+// (lqg_amd/_learn.py packs these field by field)
+static_assert(sizeof(lqg_conv) == 160 && sizeof(lqg_selscan) == 328 && sizeof(lqg_selscan_bars) == 112, "");
+
 namespace lqg {
 namespace learn {
 

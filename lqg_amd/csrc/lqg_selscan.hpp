@@ -839,40 +839,62 @@ template <class IT> __global__ __launch_bounds__(256) void k_scan_groups(const S
 }
 
 // ------------------------------------------------------------------------------------------------ one step
-// LPC lanes per channel, 4 states each: a wave moves whole lines of the state.
+// LPC lanes per channel, 4 states each (16 bytes of the state: a wave reads and writes 1 kB in a row).  Memory bound by the state.
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+template <class T> __device__ inline void load4(const T* p, bool whole, long left, float (&x)[4]) {
+  if (whole) {
+    const Four<T> r = *reinterpret_cast<const Four<T>*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = up(r.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = j < left ? up(p[j]) : 0.0f;
+  }
+}
+
 template <class IT, int LPC>
 __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* state) {
-  const long N = a.p.N, D = a.p.D, per = 256 / LPC;
-  const long blk = blockIdx.x % a.blocks, b = blockIdx.x / a.blocks;
+  const long N = a.p.N, D = a.p.D;
+  constexpr int per = 256 / LPC;
+  const long blk = blockIdx.x % (unsigned)a.blocks, b = blockIdx.x / (unsigned)a.blocks;
   const long d = blk * per + threadIdx.x / LPC;
   const int q = threadIdx.x % LPC;
   if (d >= D) return;                                 // whole channels: their LPC lanes leave together
-  const long grp = d / a.Dg;
+  const long n = q * 4, left = N - n;
+  const bool whole = left >= 4;
+  float* hp = state + (b * D + d) * N + n;
+  float h[4], A[4], B[4], C[4];
+  load4(hp, whole, left, h);
+  if (a.p.A.type == LQG_T_F32) load4(static_cast<const float*>(a.p.A.ptr) + d * N + n, whole, left, A);
+  else
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A[j] = j < left ? load_param(a.p.A, d * N + n + j) : 0.0f;
+  const unsigned grp = (unsigned)d / (unsigned)a.Dg;
+  load4(seq<IT>(a.p.Bm, b, grp * a.p.Bm.sg + n), whole, left, B);
+  load4(seq<IT>(a.p.Cm, b, grp * a.p.Cm.sg + n), whole, left, C);
   const float u = up(seq<IT>(a.p.u, b, d)[0]);
+  const float z = a.p.z.ptr ? up(seq<IT>(a.p.z, b, d)[0]) : 0.0f;
   float dl = up(seq<IT>(a.p.delta, b, d)[0]);
   if (a.p.delta_bias.ptr) dl += load_param(a.p.delta_bias, d);
   dl = step_size(a, dl);
-  const IT* B = seq<IT>(a.p.Bm, b, grp * a.p.Bm.sg);
-  const IT* C = seq<IT>(a.p.Cm, b, grp * a.p.Cm.sg);
-  float* h = state + (b * D + d) * N;
   float y = 0.0f;
-  for (long n = q * 4; n < N; n += LPC * 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (n + j >= N) break;
-      const float v = fmaf(exp2_hw(dl * (load_param(a.p.A, d * N + n + j) * LOG2E)), h[n + j], dl * u * up(B[n + j]));
-      h[n + j] = v;
-      y = fmaf(up(C[n + j]), v, y);
-    }
+  for (int j = 0; j < 4; ++j) {
+    h[j] = fmaf(exp2_hw(dl * (A[j] * LOG2E)), h[j], dl * u * B[j]);
+    if (j < left) y = fmaf(C[j], h[j], y);
+  }
+  if (whole) {
+    *reinterpret_cast<Four<float>*>(hp) = Four<float>{{h[0], h[1], h[2], h[3]}};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) hp[j] = h[j];
   }
 #pragma unroll
   for (int k = 1; k < LPC; k <<= 1) y += __shfl_xor(y, k);
   if (q) return;
   if (a.p.Dskip.ptr) y = fmaf(load_param(a.p.Dskip, d), u, y);
-  if (a.p.z.ptr) {
-    const float z = up(seq<IT>(a.p.z, b, d)[0]);
-    y *= z * sigmoid(z);
-  }
+  if (a.p.z.ptr) y *= z * sigmoid(z);
   const_cast<IT*>(seq<IT>(a.p.y, b, d))[0] = down<IT>(y);
 }
 

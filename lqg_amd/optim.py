@@ -206,14 +206,15 @@ class AdamW:
                 g = p.grad
                 if g is None:
                     continue
-                if g.is_sparse or g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
-                    raise LqgHipError(f"AdamW.step: a dense gradient of {p.dtype} {tuple(p.shape)} is needed, got {g.dtype} {tuple(g.shape)}")
-                if (p.dtype, p.device, p.numel()) != self._sizes[i] or not p.is_contiguous():
+                dtype, device, size = self._sizes[i]
+                if p.dtype != dtype or p.device != device or p.numel() != size or not p.is_contiguous():
                     raise LqgHipError("AdamW.step: a tensor's type, device, size or order is not what it was")
+                if g.is_sparse or g.dtype != dtype or g.device != device or g.numel() != size:
+                    raise LqgHipError(f"AdamW.step: a dense gradient of {dtype} {tuple(p.shape)} is needed, got {g.dtype} {tuple(g.shape)}")
                 if not g.is_contiguous():
                     g = g.contiguous()
                     kept.append(g)
-                params[n], grads[n], numel[n], offset[n] = p.data_ptr(), g.data_ptr(), p.numel(), self.offsets[i]
+                params[n], grads[n], numel[n], offset[n] = p.data_ptr(), g.data_ptr(), size, self.offsets[i]
                 moved.append(p)
                 n += 1
             call.count = n
