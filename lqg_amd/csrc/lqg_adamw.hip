@@ -2,8 +2,9 @@
 //
 // Memory bound: an element of a float tensor moves 28 bytes (p, m, v read and written, g read), 16 with 8-bit moments.  One launch
 // walks up to TENSORS tensors: their table travels in the kernel's arguments, so that no table has to be copied to the device and kept
-// alive; a workgroup finds its tensor by bisection in uniform (scalar) registers.  This file is compiled with -ffp-contract=off: every
-// operation rounds by itself, so a step gives the bits that the same formula gives written operation by operation.
+// alive; a workgroup finds its tensor by bisection in uniform (scalar) registers.  Vectors need no alignment beyond their elements'
+// (the hardware takes global accesses at any address).  This file is compiled with -ffp-contract=off: with 32-bit states every operation
+// rounds by itself, so a step gives the bits that the same formula gives written operation by operation.
 #include "lqg_learn.hpp"
 
 #include <cmath>
@@ -13,8 +14,8 @@ using namespace lqg::learn;
 namespace {
 
 constexpr int TENSORS = 96;      // 3.5 kB of arguments
-constexpr int CHUNK = 2048;      // elements of a workgroup: 256 lanes x 2 vectors of 4
-constexpr int BLOCK = 256;       // elements that share a scale (8 bits): a wave, 4 per lane
+constexpr int CHUNK = 2048;      // elements of a workgroup: 256 lanes x 2 vectors of 4 (32 bits), x 8 (8 bits)
+constexpr int BLOCK = 256;       // elements that share a scale (8 bits): half a wave, 8 per lane
 constexpr float F8_MAX = 448.0f, TINY = 1e-30f, LEAST = 0x1p-9f;
 
 struct Table {
@@ -30,7 +31,7 @@ template <class S> struct Hyper {
   const double* state;                              // {t, inv1, inv2} or NULL
 };
 
-template <class T> struct alignas(4 * sizeof(T)) Vec4 { T v[4]; };
+template <class T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
 
 template <class S> __device__ inline S root(S x);
 template <> __device__ inline float root(float x) { return sqrtf(x); }
@@ -55,137 +56,148 @@ __device__ inline int tensor_of(const Table& t, int chunk) {
   return lo;
 }
 
-// four elements at i, of which `left` exist; whole: the pointer is aligned for a vector
-template <class T> __device__ inline Vec4<T> load4(const T* p, bool whole, long left) {
-  if (whole && left >= 4) return *reinterpret_cast<const Vec4<T>*>(p);
-  Vec4<T> r;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) r.v[k] = k < left ? p[k] : (T)0.0f;
-  return r;
-}
-template <class T> __device__ inline void store4(T* p, const Vec4<T>& r, bool whole, long left) {
-  if (whole && left >= 4) {
-    *reinterpret_cast<Vec4<T>*>(p) = r;
+// V elements, of which `left` exist (WHOLE: all)
+template <bool WHOLE, class T, int V> __device__ inline void load(const T* p, long left, Vec<T, V>& r) {
+  if (WHOLE || left >= V) {
+    r = *reinterpret_cast<const Vec<T, V>*>(p);
     return;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < V; ++k) r.v[k] = k < left ? p[k] : (T)0.0f;
+}
+template <bool WHOLE, class T, int V> __device__ inline void store(T* p, long left, const Vec<T, V>& r) {
+  if (WHOLE || left >= V) {
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k)
     if (k < left) p[k] = r.v[k];
 }
 
 // T: tensors' type, S: type of the moments and of the arithmetic
-template <class T, class S>
-__global__ __launch_bounds__(256) void k_adamw(const Table tab, const Hyper<S> h, S* ms, S* vs) {
-  const int i = tensor_of(tab, (int)blockIdx.x);
-  const long at = (long)((int)blockIdx.x - tab.start[i]) * CHUNK + threadIdx.x * 4, n = tab.n[i];
-  T* p = static_cast<T*>(tab.p[i]);
-  const T* g = static_cast<const T*>(tab.g[i]);
-  const bool whole = (((uintptr_t)p | (uintptr_t)g) & (sizeof(T) * 4 - 1)) == 0;
-  S* m = ms + tab.off[i];
-  S* v = vs + tab.off[i];
-  const S inv1 = h.state ? (S)h.state[1] : h.inv1, inv2 = h.state ? (S)h.state[2] : h.inv2;
-  Vec4<T> pv[2], gv[2];
-  Vec4<S> mv[2], vv[2];
+template <bool WHOLE, class T, class S>
+__device__ inline void step32(const Hyper<S>& h, T* p, const T* g, S* m, S* v, long left, S inv1, S inv2) {
+  Vec<T, 4> pv[2], gv[2];
+  Vec<S, 4> mv[2], vv[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const long e = at + q * 1024, left = n - e;
-    if (left <= 0) continue;
-    pv[q] = load4(p + e, whole, left);
-    gv[q] = load4(g + e, whole, left);
-    mv[q] = load4(m + e, true, left);
-    vv[q] = load4(v + e, true, left);
+    if (!WHOLE && left <= q * 1024) continue;
+    load<WHOLE>(p + q * 1024, left - q * 1024, pv[q]);
+    load<WHOLE>(g + q * 1024, left - q * 1024, gv[q]);
+    mv[q] = *reinterpret_cast<const Vec<S, 4>*>(m + q * 1024);       // (states reach to a multiple of 256)
+    vv[q] = *reinterpret_cast<const Vec<S, 4>*>(v + q * 1024);
   }
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const long e = at + q * 1024, left = n - e;
-    if (left <= 0) continue;
+    if (!WHOLE && left <= q * 1024) continue;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       moments<S>(h, (S)gv[q].v[k], mv[q].v[k], vv[q].v[k]);
       pv[q].v[k] = (T)moved<S>(h, inv1, inv2, (S)pv[q].v[k], mv[q].v[k], vv[q].v[k]);
     }
-    store4(p + e, pv[q], whole, left);
-    store4(m + e, mv[q], true, left);
-    store4(v + e, vv[q], true, left);
+    store<WHOLE>(p + q * 1024, left - q * 1024, pv[q]);
+    store<WHOLE>(m + q * 1024, left - q * 1024, mv[q]);
+    store<WHOLE>(v + q * 1024, left - q * 1024, vv[q]);
   }
 }
 
-// largest of the bit patterns of |x| over the wave: orders magnitudes, and puts a NaN above them all
-__device__ inline uint32_t wave_top(uint32_t x) {
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, k));
-  return x;
+template <class T, class S>
+__global__ __launch_bounds__(256) void k_adamw(const Table tab, const Hyper<S> h, S* ms, S* vs) {
+  const int i = tensor_of(tab, (int)blockIdx.x);
+  const long first = (long)((int)blockIdx.x - tab.start[i]) * CHUNK, n = tab.n[i], at = first + threadIdx.x * 4;
+  T* p = static_cast<T*>(tab.p[i]) + at;
+  const T* g = static_cast<const T*>(tab.g[i]) + at;
+  S *m = ms + tab.off[i] + at, *v = vs + tab.off[i] + at;
+  const S inv1 = h.state ? (S)h.state[1] : h.inv1, inv2 = h.state ? (S)h.state[2] : h.inv2;
+  if (first + CHUNK <= n) step32<true>(h, p, g, m, v, CHUNK, inv1, inv2);
+  else step32<false>(h, p, g, m, v, n - at, inv1, inv2);
 }
-__device__ inline uint32_t top4(const float (&x)[4]) {
+
+// largest of the bit patterns of |x| over half a wave: orders magnitudes, and puts a NaN above them all
+template <int CTRL> __device__ inline uint32_t max_dpp(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+__device__ inline float top(const float (&x)[8]) {
   uint32_t t = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) t = max(t, __float_as_uint(x[k]) & 0x7fffffffu);
-  return wave_top(t);
+  for (int k = 0; k < 8; ++k) t = max(t, __float_as_uint(x[k]) & 0x7fffffffu);
+  t = max_dpp<DPP_ROR8>(max_dpp<DPP_HALF_MIRROR>(max_dpp<DPP_XOR2>(max_dpp<DPP_XOR1>(t))));       // the row of 16
+  const auto a = __builtin_amdgcn_permlane16_swap(t, t, false, false);
+  return __uint_as_float(max((uint32_t)a[0], (uint32_t)a[1]));
 }
-__device__ inline void unpack(uint32_t c, float scale, float (&x)[4]) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-  x[0] = lo[0] * scale, x[1] = lo[1] * scale, x[2] = hi[0] * scale, x[3] = hi[1] * scale;
+struct __attribute__((packed, aligned(4))) Codes { uint32_t c[2]; };
+__device__ inline void unpack(const Codes& q, float scale, float (&x)[8]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.c[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.c[k], true);
+    x[4 * k] = lo[0] * scale, x[4 * k + 1] = lo[1] * scale, x[4 * k + 2] = hi[0] * scale, x[4 * k + 3] = hi[1] * scale;
+  }
 }
-__device__ inline uint32_t pack(const float (&x)[4]) {
-  int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
+__device__ inline Codes pack(const float (&x)[8]) {
+  Codes q;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k], x[4 * k + 1], 0, false);
+    q.c[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k + 2], x[4 * k + 3], c, true);
+  }
+  return q;
+}
+
+// Half a wave is a block of 256 elements, 8 a lane: one sequence of cross-lane maxima serves two blocks.  The root of v, which is stored,
+// serves the update as well: sqrt(v inv2) = sqrt(v) sqrt(inv2).  Roots and quotients are the hardware's approximations (1 ulp each): with the
+// exact ones, of a dozen instructions each, the arithmetic took longer than the bytes.
+template <bool WHOLE, class T>
+__device__ inline void step8(const Hyper<float>& h, T* p, const T* g, uint32_t* mc, uint32_t* rc, float* m_scale, float* r_scale, long left,
+                             float inv1, float inv2) {
+  Vec<T, 8> pv, gv;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) pv.v[k] = gv.v[k] = (T)0.0f;
+  if (WHOLE || left > 0) {
+    load<WHOLE>(p, left, pv);
+    load<WHOLE>(g, left, gv);
+  }
+  float m[8], r[8];
+  unpack(*reinterpret_cast<const Codes*>(mc), *m_scale, m);
+  unpack(*reinterpret_cast<const Codes*>(rc), *r_scale, r);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float gk = (float)gv.v[k];
+    m[k] = fmaf(h.b1, m[k], h.a1 * gk);
+    r[k] = __builtin_amdgcn_sqrtf(fmaf(h.b2, r[k] * r[k], (h.a2 * gk) * gk));
+    pv.v[k] = (T)fmaf(-(m[k] * inv1), rcp_hw(fmaf(r[k], inv2, h.eps)), (float)pv.v[k] * h.decay);
+    if (!WHOLE && k >= left) m[k] = r[k] = 0.0f;             // behind the tensor's end
+  }
+  if (WHOLE || left > 0) store<WHOLE>(p, left, pv);
+  const float mt = top(m), rt = top(r);
+  const bool mz = mt < TINY, rz = rt < TINY;                 // (false for a NaN, which then reaches the codes)
+  const float mi = mz ? 0.0f : F8_MAX * rcp_hw(mt), ri = rz ? 0.0f : F8_MAX * rcp_hw(rt);
+  const float least = rz ? 0.0f : LEAST;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float q = r[k] * ri;
+    m[k] *= mi;
+    r[k] = r[k] > 0.0f && q < least ? least : q;             // (half of it and less would round to 0)
+  }
+  *reinterpret_cast<Codes*>(mc) = pack(m);
+  *reinterpret_cast<Codes*>(rc) = pack(r);
+  if ((threadIdx.x & 31) == 0) {
+    *m_scale = mz ? 0.0f : mt * (1.0f / F8_MAX);
+    *r_scale = rz ? 0.0f : rt * (1.0f / F8_MAX);
+  }
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void k_adamw8(const Table tab, const Hyper<float> h, uint32_t* ms, uint32_t* rs, float* m_scale,
                                                 float* r_scale) {
   const int i = tensor_of(tab, (int)blockIdx.x);
-  const long n = tab.n[i];
-  T* p = static_cast<T*>(tab.p[i]);
-  const T* g = static_cast<const T*>(tab.g[i]);
-  const bool whole = (((uintptr_t)p | (uintptr_t)g) & (sizeof(T) * 4 - 1)) == 0;
-  const float inv1 = h.state ? (float)h.state[1] : h.inv1, inv2 = h.state ? (float)h.state[2] : h.inv2;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long first = (long)((int)blockIdx.x - tab.start[i]) * CHUNK;
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const long e0 = first + (q * 4 + wave) * BLOCK;          // the wave's block; uniform in the wave
-    if (e0 >= n) continue;
-    const long e = e0 + lane * 4, left = n - e, o = tab.off[i] + e;
-    const long sc = (tab.off[i] + e0) / BLOCK;
-    float m[4], r[4], v[4], pf[4];
-    unpack(ms[o / 4], m_scale[sc], m);
-    unpack(rs[o / 4], r_scale[sc], r);
-    Vec4<T> pv, gv;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) pv.v[k] = (T)0.0f, gv.v[k] = (T)0.0f;
-    if (left > 0) {
-      pv = load4(p + e, whole, left);
-      gv = load4(g + e, whole, left);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = r[k] * r[k];
-      moments<float>(h, (float)gv.v[k], m[k], v[k]);
-      pf[k] = moved<float>(h, inv1, inv2, (float)pv.v[k], m[k], v[k]);
-      r[k] = sqrtf(v[k]);
-      if (k >= left) m[k] = 0.0f, r[k] = 0.0f;               // behind the tensor's end
-      pv.v[k] = (T)pf[k];
-    }
-    const float mt = __uint_as_float(top4(m)), rt = __uint_as_float(top4(r));
-    const bool mz = mt < TINY, rz = rt < TINY;               // (false for a NaN, which then reaches the codes)
-    const float mi = mz ? 0.0f : F8_MAX / mt, ri = rz ? 0.0f : F8_MAX / rt;
-    float mc[4], rc[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      mc[k] = m[k] * mi;
-      rc[k] = r[k] * ri;
-      // (half the least value, ties to even: what is at most that rounds to 0)
-      if (r[k] > 0.0f && rc[k] < LEAST && !rz) rc[k] = LEAST;
-    }
-    if (left > 0) store4(p + e, pv, whole, left);
-    ms[o / 4] = pack(mc);
-    rs[o / 4] = pack(rc);
-    if (lane == 0) {
-      m_scale[sc] = mz ? 0.0f : mt / F8_MAX;
-      r_scale[sc] = rz ? 0.0f : rt / F8_MAX;
-    }
-  }
+  const long first = (long)((int)blockIdx.x - tab.start[i]) * CHUNK, n = tab.n[i], at = first + threadIdx.x * 8;
+  T* p = static_cast<T*>(tab.p[i]) + at;
+  const T* g = static_cast<const T*>(tab.g[i]) + at;
+  const long o = tab.off[i] + at, sc = o / BLOCK;
+  const float inv1 = h.lr * (h.state ? (float)h.state[1] : h.inv1), inv2 = sqrtf(h.state ? (float)h.state[2] : h.inv2);
+  if (first + CHUNK <= n) step8<true>(h, p, g, ms + o / 4, rs + o / 4, m_scale + sc, r_scale + sc, CHUNK, inv1, inv2);
+  else if (at - (threadIdx.x & 31) * 8 < n) step8<false>(h, p, g, ms + o / 4, rs + o / 4, m_scale + sc, r_scale + sc, n - at, inv1, inv2);
 }
 
 __global__ void k_advance(double* s, double b1, double b2) {
