@@ -63,7 +63,7 @@ typedef struct lqg_selscan {
   float* state_out;
   const int32_t* lengths;
   void* checkpoints;
-  int32_t chunks, channels;            /* pieces the time axis is cut into, channels of a workgroup: 0 = the rules, else 1 .. 64; 32, 64 */
+  int32_t chunks, pad;                 /* pieces the time axis is cut into: 0 = the rule, else 1 .. 64 */
 } lqg_selscan;
 size_t lqg_selscan_workspace(const lqg_selscan* p);
 size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p);

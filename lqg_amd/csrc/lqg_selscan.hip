@@ -35,7 +35,7 @@ int check(const lqg_selscan* p) {
   if (!p) return LQG_ERR_NULL;
   if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
   if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > MAX_STRIDE || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
-  if (p->chunks < 0 || p->chunks > 64 || (p->channels != 0 && p->channels != 32 && p->channels != 64)) return LQG_ERR_ARG;
+  if (p->chunks < 0 || p->chunks > 64) return LQG_ERR_ARG;
   for (const lqg_seq* q : {&p->u, &p->delta, &p->z, &p->Bm, &p->Cm, &p->y})
     if (q->st < 0 || q->st > MAX_STRIDE) return LQG_ERR_ARG;
   for (const lqg_param* q : {&p->A, &p->Dskip, &p->delta_bias})
@@ -47,19 +47,25 @@ int check(const lqg_selscan* p) {
 long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
 int tile_of(long N) { return N > 32 ? 8 : 16; }
 
-ScanArgs describe(const lqg_selscan* p) {
+// Waves on the 1024 SIMDs decide whether the time axis is cut.  A cut costs the pass that leaves the chunks' carries (forward 0.7 of the
+// main pass, backward a third of it) and pays while SIMDs are empty, or, where registers let two waves share a SIMD, while one waits
+// alone.  Measured at 2048 steps, bfloat16 (us, uncut / cut; waves uncut):  forward N = 16: 185 / 287 (2048), 132 / 167 (1024), 129 / 93
+// in 4 (512); N = 4: 208 / 176 in 2 (512).  Backward N = 16: 620 / 860 (2048), 404 / 353 in 2 (1024); N = 8: 545 / 581 (1024), 440 / 300
+// in 4 (512); N = 24: 590 / 730 (1024), 565 / 377 in 2 (512).  So: below 0.75 waves a SIMD (backward with 9 to 16 states: below 1.5) into
+// as many pieces as fill the SIMDs, twice where registers allow it (not with one wave a workgroup, N <= 4, nor backward beyond 16
+// states); a piece is 8 tiles at least.
+ScanArgs describe(const lqg_selscan* p, bool grad) {
   ScanArgs a{};
   a.p = *p;
   const long TT = tile_of(p->N);
   a.Dg = p->D / p->G;
-  a.ch = p->N > 16 ? 64 : p->channels ? p->channels : 32;
-  a.bpg = (a.Dg + a.ch - 1) / a.ch;
+  a.bpg = (a.Dg + CHANNELS - 1) / CHANNELS;
   a.blocks = a.bpg * p->G;
   a.tiles = (p->T + TT - 1) / TT;
-  // Waves enough for two on each of the 1024 SIMDs; a chunk is at least 8 tiles.
-  const long waves = a.blocks * p->B * (p->N > 16 ? 8 : p->N > 8 ? 4 : p->N > 4 ? 2 : 1);
-  a.chunks = p->chunks ? p->chunks : std::min(std::min(64L, (a.tiles + 7) / 8), (2048 + waves - 1) / waves);
-  if (a.chunks > a.tiles) a.chunks = a.tiles;
+  const long waves = a.blocks * p->B * (p->N > 8 ? 4 : p->N > 4 ? 2 : 1);
+  const long enough = grad && p->N > 8 && p->N <= 16 ? 1536 : 768, room = p->N > 4 && !(grad && p->N > 16) ? 2048 : 1024;
+  a.chunks = waves >= enough ? 1 : std::min({64L, (a.tiles + 7) / 8, (room + waves - 1) / waves});
+  if (p->chunks) a.chunks = std::min((long)p->chunks, a.tiles);
   const long per = (a.tiles + a.chunks - 1) / a.chunks;
   a.chunk = per * TT;
   a.chunks = (a.tiles + per - 1) / per;               // no empty chunk
@@ -91,19 +97,19 @@ GradSpace grad_space(const ScanArgs& a) {
 }  // namespace
 
 extern "C" size_t lqg_selscan_workspace(const lqg_selscan* p) {
-  return check(p) ? 0 : (size_t)carry_floats(describe(p)) * sizeof(float);
+  return check(p) ? 0 : (size_t)carry_floats(describe(p, false)) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p) {
-  return check(p) ? 0 : (size_t)(p->B * describe(p).tiles * room_of(p->N) * p->D) * sizeof(float);
+  return check(p) ? 0 : (size_t)(p->B * describe(p, false).tiles * room_of(p->N) * p->D) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_grad_workspace(const lqg_selscan* p) {
-  return check(p) ? 0 : (size_t)grad_space(describe(p)).total * sizeof(float);
+  return check(p) ? 0 : (size_t)grad_space(describe(p, true)).total * sizeof(float);
 }
 
 extern "C" int lqg_selective_scan(const lqg_selscan* p, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check(p)) return rc;
   if (!have(p) || !p->y.ptr) return LQG_ERR_NULL;
-  ScanArgs a = describe(p);
+  ScanArgs a = describe(p, false);
   const long carry = carry_floats(a);
   if (carry && !workspace) return LQG_ERR_NULL;
   if (workspace_bytes < carry * sizeof(float)) return LQG_ERR_WORKSPACE;
@@ -118,7 +124,7 @@ extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_b
   if (!g || !have(p) || !p->checkpoints || !workspace) return LQG_ERR_NULL;
   if (g->dy.st < 0 || g->dy.st > MAX_STRIDE) return LQG_ERR_ARG;
   if (!g->dy.ptr || !g->du || !g->ddelta || !g->dBm || !g->dCm || (p->z.ptr && !g->dz)) return LQG_ERR_NULL;
-  ScanArgs a = describe(p);
+  ScanArgs a = describe(p, true);
   a.g = *g;
   const GradSpace s = grad_space(a);
   if (workspace_bytes < s.total * sizeof(float)) return LQG_ERR_WORKSPACE;
@@ -128,7 +134,7 @@ extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_b
   a.partBC = ws + s.carry;
   a.partP = a.partBC + 2 * s.group;
   hipStream_t st = (hipStream_t)stream;
-  const long n = p->B * p->T * p->G * p->N, groups = (n + 255) / 256;
+  const long n = p->B * p->T * p->G * 2 * p->N, groups = (n + 255) / 256;
   if (!grid_fits(groups, 256)) return LQG_ERR_ARG;
   if (const int rc = by_type(1, a, st)) return rc;
   const int rc = p->type == LQG_T_F32 ? ScanOf<float>::groups(a, groups, st)
@@ -147,7 +153,7 @@ extern "C" int lqg_selective_scan_step(const lqg_selscan* p, float* state, void*
   if (const int rc = check(p)) return rc;
   if (p->T != 1) return LQG_ERR_ARG;
   if (!have(p) || !p->y.ptr || !state) return LQG_ERR_NULL;
-  ScanArgs a = describe(p);
+  ScanArgs a = describe(p, false);
   hipStream_t st = (hipStream_t)stream;
   if (p->type == LQG_T_F32) return ScanOf<float>::step(a, state, st);
   if (p->type == LQG_T_BF16) return ScanOf<bf16>::step(a, state, st);

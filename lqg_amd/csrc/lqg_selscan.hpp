@@ -3,12 +3,14 @@
 //   dl = softplus(delta + delta_bias),  h_t = exp(dl_t A) h_{t-1} + dl_t B_t u_t,  y_t = (sum_n C_t h_t + D u_t) silu(z_t)
 //
 // B x D x N scalar recurrences; per step of one of them one exponential and four float operations, and B_t, C_t are shared by all
-// channels of a group.  Mapping: a lane is a channel, a wave holds NS of the N states of 64 channels in registers, the NW = N / NS
-// waves of a workgroup share those 64 channels.  The time axis is walked in tiles of TT steps: each wave prepares TT / NW rows
-// (softplus, dl u) for all of them through LDS, runs the tile's TT steps on its states, and leaves its part of sum_n C h in LDS, where
-// the waves finish TT / NW rows each.  B_t and C_t of a tile sit one value per lane in rows of 16 and reach the arithmetic as DPP row
-// broadcasts: an operand modifier, no load and no instruction.  Few channels: the time axis is cut into chunks; one pass leaves each
-// chunk's end state from zero and its sum of dl, the second enters with exp(A sum dl) h + end state over the chunks before it.
+// channels of a group: bound by the vector units (and their exponential) from N = 8 or so on, by memory below.  Mapping: a workgroup is 32
+// channels with all their states; a wave is those 32 channels twice, each half with NS of the N states in registers, so NW waves hold
+// 2 NS NW states.  The time axis is walked in tiles of TT steps: the threads prepare the tile's TT x 32 elements (softplus, dl u, silu)
+// once for all states through LDS, every wave runs the TT steps on its states and leaves its part of sum_n C h in LDS, and the threads
+// finish the elements they prepared.  B_t and C_t of a tile sit one value per lane in rows of 16 and reach the arithmetic as DPP row
+// broadcasts: an operand modifier, no load and no instruction.  Whole tiles (all but the last) run without bounds checks, their loads two
+// tiles ahead.  Few channels: the time axis is cut into chunks; one pass leaves each chunk's end state from zero and its sum of dl, the
+// second enters with exp(A sum dl) h + end state over the chunks before it.
 #pragma once
 #include "lqg_learn.hpp"
 
@@ -16,11 +18,12 @@ namespace lqg {
 namespace learn {
 
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int CHANNELS = 32;     // of a workgroup
 
 struct ScanArgs {
   lqg_selscan p;
   lqg_selscan_bars g;
-  long Dg, bpg, blocks, ch;      // channels of a group, blocks of `ch` of them, blocks in all
+  long Dg, bpg, blocks;          // channels of a group, blocks of CHANNELS of them, blocks in all
   long chunks, chunk, tiles;     // chunks of the time axis, their steps (a multiple of TT), tiles of TT steps in T
   float *hl, *sd;                // carries [B][chunks][N][D], sums of dl [B][chunks][D]
   float *partBC, *partP;         // gradients: [blocks][B][T][2][N], [B * chunks][N + 2][D]
@@ -31,8 +34,9 @@ template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, lo
 }
 
 // The shape of a workgroup: CH channels x NS NW 64 / CH states, TT steps a tile.
-template <int CH_, int NS_, int NW_, int TT_> struct Shape {
-  static constexpr int CH = CH_, NS = NS_, NW = NW_, TT = TT_;
+template <int NS_, int NW_, int TT_> struct Shape {
+  static constexpr int CH = CHANNELS, NS = NS_, NW = NW_, TT = TT_;
+  static constexpr int GRAD_WAVES = NS == 2 && NW > 1 ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
   static constexpr int LS = 64 / CH;          // groups of NS states in a wave
   static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
   static constexpr int NP = NS * PS;          // states it has room for
@@ -517,7 +521,7 @@ template <class S> struct ChannelSum {
 
 // CARRY: leave each chunk's carry (lambda at its start from 0 at its end) and its sum of dl.
 template <class IT, class S, bool CARRY>
-__global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
+__global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const ScanArgs a) {
   constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
   __shared__ float2 s_in[2][TT][CH];                      // dl, dl u
   __shared__ float s_dy[2][TT][CH];                       // dY
@@ -821,21 +825,27 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_scan_grad(const ScanArgs a) {
   }
 }
 
-// dB, dC [B][T][G][N]: the blocks of a group summed, 0 in the padding
+// dB, dC [B][T][G][N]: the blocks of a group summed, 0 in the padding.  A thread per value, eight loads on their way at a time.
 template <class IT> __global__ __launch_bounds__(256) void k_scan_groups(const ScanArgs a) {
   const long e = (long)blockIdx.x * 256 + threadIdx.x, N = a.p.N, G = a.p.G, T = a.p.T, B = a.p.B;
-  if (e >= B * T * G * N) return;
-  const long n = e % N, g = e / N % G, t = e / (N * G) % T, b = e / (N * G * T);
-  const bool live = !a.p.lengths || t < a.p.lengths[b];
+  if (e >= B * T * G * 2 * N) return;
+  const unsigned n2 = (unsigned)(e % (2 * N));
+  const long btg = e / (2 * N), g = btg % G, bt = btg / G, t = bt % T, b = bt / T;
   float x = 0.0f, y = 0.0f;
-  if (live)
-    for (long k = g * a.bpg; k < (g + 1) * a.bpg; ++k) {
-      const long at = ((k * B + b) * T + t) * 2 * N + n;
-      x += a.partBC[at];
-      y += a.partBC[at + N];
+  if (!a.p.lengths || t < a.p.lengths[b]) {
+    const long step = B * T * 2 * N;
+    const float* p = a.partBC + g * a.bpg * step + bt * 2 * N + n2;
+    long k = 0;
+    for (; k + 8 <= a.bpg; k += 8) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = p[(k + q) * step];
+#pragma unroll
+      for (int q = 0; q < 8; q += 2) x += v[q], y += v[q + 1];
     }
-  static_cast<IT*>(a.g.dBm)[e] = down<IT>(x);
-  static_cast<IT*>(a.g.dCm)[e] = down<IT>(y);
+    for (; k < a.bpg; ++k) x += p[k * step];
+  }
+  static_cast<IT*>(n2 < N ? a.g.dBm : a.g.dCm)[btg * N + (n2 < N ? n2 : n2 - N)] = down<IT>(x + y);
 }
 
 // ------------------------------------------------------------------------------------------------ one step
@@ -915,16 +925,11 @@ template <class IT, class S> int launch(int what, const ScanArgs& a, hipStream_t
 
 template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
   const long N = a.p.N;
-  if (N > 32) return launch<IT, Shape<64, 8, 8, 8>>(what, a, st);
-  if (N > 16) return launch<IT, Shape<64, 4, 8, 16>>(what, a, st);
-  if (a.ch == 32) {
-    if (N > 8) return launch<IT, Shape<32, 2, 4, 16>>(what, a, st);
-    if (N > 4) return launch<IT, Shape<32, 2, 2, 16>>(what, a, st);
-    return launch<IT, Shape<32, 2, 1, 16>>(what, a, st);
-  }
-  if (N > 8) return launch<IT, Shape<64, 2, 8, 16>>(what, a, st);
-  if (N > 4) return launch<IT, Shape<64, 2, 4, 16>>(what, a, st);
-  return launch<IT, Shape<64, 2, 2, 16>>(what, a, st);
+  if (N > 32) return launch<IT, Shape<8, 4, 8>>(what, a, st);
+  if (N > 16) return launch<IT, Shape<4, 4, 16>>(what, a, st);
+  if (N > 8) return launch<IT, Shape<2, 4, 16>>(what, a, st);
+  if (N > 4) return launch<IT, Shape<2, 2, 16>>(what, a, st);
+  return launch<IT, Shape<2, 1, 16>>(what, a, st);
 }
 
 template <class IT> int launch_step(ScanArgs a, float* state, hipStream_t st) {
