@@ -14,6 +14,7 @@ derivative-free population evaluation of BASELINE config 3 (thousands of candida
 import torch
 
 from lqg_amd.infer.models import get_model_params, log_likelihood_objective
+from lqg_amd.optim import AdamW
 from lqg_amd.tracking import BoundedActor
 
 GUARD_EVERY = 64        # steps between two read-backs of the graphed loop's NaN guard (max_likelihood)
@@ -43,8 +44,8 @@ def max_likelihood(x, model=BoundedActor, numpyro_fn=None, process_noise=1.0, dt
     names = [k for k in get_model_params(model) if k not in fixed]
     P = len(names)
     z = torch.log(torch.tensor([float(get_model_params(model)[k]) for k in names], dtype=torch.float64, device=x.device))
-    m1, m2 = torch.zeros_like(z), torch.zeros_like(z)
-    b1, b2, eps = 0.9, 0.999, 1e-8
+    opt = AdamW(z, lr=abs(step_size), betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0) if steps else None     # (one launch a step)
+    held = lambda: (z.clone(), {k: v.clone() if k != "step" else v for k, v in opt.state_dict().items()})  # noqa: E731
     eye = torch.eye(P, dtype=torch.float64, device=x.device)
     losses = torch.empty(steps, dtype=torch.float64, device=x.device)     # (kept on the device: no synchronisation per step)
     if method not in ("fd", "adjoint"):
@@ -57,7 +58,7 @@ def max_likelihood(x, model=BoundedActor, numpyro_fn=None, process_noise=1.0, dt
     # the path: the replay then returns NaN.  The loop never synchronises per step; every GUARD_EVERY steps (one read-back) it
     # checks the losses since the last verified state and, on a NaN, resumes from THAT state on the eager path, which
     # re-decides per evaluation (round 3 refitted all `steps` iterations from scratch).
-    it, verified = 0, (0, z, m1, m2)
+    it, verified = 0, (0, held()) if steps else None
     while it < steps:
         if method == "adjoint":
             from lqg_amd.infer.gradient import value_and_grad
@@ -76,15 +77,16 @@ def max_likelihood(x, model=BoundedActor, numpyro_fn=None, process_noise=1.0, dt
             loss = -obj[0]
             grad = -(obj[1:P + 1] - obj[P + 1:]) / (2 * fd_step)
         losses[it] = loss
-        m1 = b1 * m1 + (1 - b1) * grad
-        m2 = b2 * m2 + (1 - b2) * grad * grad
-        z = z - step_size * (m1 / (1 - b1 ** (it + 1))) / (torch.sqrt(m2 / (1 - b2 ** (it + 1))) + eps)
+        z.grad = grad if step_size >= 0 else -grad
+        opt.step()
         it += 1
         if ev is not None and (it % GUARD_EVERY == 0 or it == steps):
             if bool(torch.isnan(losses[verified[0]:it]).any()):
-                it, z, m1, m2 = verified                      # back to the last state no replay had poisoned
+                it, (z0, state) = verified                    # back to the last state no replay had poisoned
+                z.copy_(z0)
+                opt.load_state_dict(state)
                 ev = None                                     # ... and on from there on the eager path
             else:
-                verified = (it, z, m1, m2)
+                verified = (it, held())
     params = {k: float(v) for k, v in zip(names, torch.exp(z).cpu())}
     return params, losses.cpu()

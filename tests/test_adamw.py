@@ -96,6 +96,32 @@ def test_the_bits_of_the_formula():
         assert torch.equal(p.detach(), z), step
 
 
+@gpu
+@pytest.mark.parametrize("step_size", (0.05, -0.01))
+def test_max_likelihood_steps_with_it(step_size):
+    """The losses and parameters of the loop written in torch operations, bit for bit."""
+    import lqg_amd
+    from lqg_amd import options
+    from lqg_amd.infer import get_model_params, log_likelihood_objective, max_likelihood
+    x = lqg_amd.BoundedActor(T=60, device="cuda", dtype=F64, sigma_target=10.0).simulate(5, n=10)
+    fixed = dict(action_cost=0.5, sigma_cursor=1.0)
+    with options.override(GRAPH=0):
+        params, losses = max_likelihood(x, lqg_amd.BoundedActor, steps=8, step_size=step_size, **fixed)
+        names = [k for k in get_model_params(lqg_amd.BoundedActor) if k not in fixed]
+        z = torch.log(torch.tensor([float(get_model_params(lqg_amd.BoundedActor)[k]) for k in names], dtype=F64, device="cuda"))
+        m, v, eye, h = torch.zeros_like(z), torch.zeros_like(z), torch.eye(len(names), dtype=F64, device="cuda"), 1e-4
+        for t in range(1, 9):
+            Z = torch.cat([z[None], z[None] + h * eye, z[None] - h * eye])
+            obj = log_likelihood_objective(x, lqg_amd.BoundedActor, {k: torch.exp(Z[:, i]) for i, k in enumerate(names)},
+                                           process_noise=1.0, dt=1.0 / 60, **fixed)
+            assert float(losses[t - 1]) == -float(obj[0])
+            g = -(obj[1:len(names) + 1] - obj[len(names) + 1:]) / (2 * h)
+            m = 0.9 * m + (1 - 0.9) * g
+            v = 0.999 * v + (1 - 0.999) * g * g
+            z = z - step_size * (m / (1 - 0.9 ** t)) / (torch.sqrt(v / (1 - 0.999 ** t)) + 1e-8)
+    assert params == {k: float(e) for k, e in zip(names, torch.exp(z).cpu())}
+
+
 def check8(opt, params, before, was, grads, step, dtype):
     """One 8-bit step: the parameters and scales to rounding; each held value is the nearest e4m3 value of the exact quotient, or, where
     that quotient is within the arithmetic's rounding of the middle between two values, the other one.  (A value that is not the nearest is
