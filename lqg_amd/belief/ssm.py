@@ -27,17 +27,19 @@ def _got(t):
 def _sequence(t, name, dims, like=None):
     if not isinstance(t, torch.Tensor) or t.dim() != dims:
         raise LqgHipError(f"{name}: a tensor of {dims} dimensions is needed, got {_got(t)}")
-    if t.dtype not in _learn.SEQ_TYPES:
-        raise LqgHipError(f"{name}: float32, bfloat16 or float16 is needed, got {t.dtype}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise LqgHipError(f"{name}: {t.dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
-    return t if _as_it_is(t) else t.contiguous()
+    dtype = t.dtype
+    if dtype not in _learn.SEQ_TYPES:
+        raise LqgHipError(f"{name}: float32, bfloat16 or float16 is needed, got {dtype}")
+    if like is not None and (dtype is not like.dtype or t.device != like.device):
+        raise LqgHipError(f"{name}: {dtype} on {t.device}, where the first sequence is {like.dtype} on {like.device}")
+    st = t.stride()
+    return t if st[-1] == 1 and (dims < 3 or st[1] <= MAX_STRIDE) else _as_it_is(t)
 
 
 def _as_it_is(t):
-    """Channels next to each other, and steps near enough for the kernels' 32-bit offsets inside a tile."""
+    """t, or its copy where channels are not next to each other or steps too far apart for the kernels' 32-bit offsets in a tile."""
     st = t.stride()
-    return (st[-1] == 1 or t.shape[-1] == 1) and (len(st) < 3 or st[1] <= MAX_STRIDE)
+    return t if (st[-1] == 1 or t.shape[-1] == 1) and (len(st) < 3 or st[1] <= MAX_STRIDE) else t.contiguous()
 
 
 def _on_gpu(t):
@@ -52,7 +54,7 @@ def _parameter(t, name, shape, like):
         raise LqgHipError(f"{name}: shape {tuple(shape)} is needed, got {_got(t)}")
     if t.dtype not in _learn.SEQ_TYPES or t.device != like.device:
         raise LqgHipError(f"{name}: float32, bfloat16 or float16 on {like.device} is needed, got {t.dtype} on {t.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _state(t, name, shape, dtype, like, in_place=False):
@@ -77,7 +79,11 @@ def _lengths(t, B, like):
 
 
 def _tracked(*tensors):
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_gradient(what, instead, *tensors):
@@ -87,12 +93,12 @@ def _no_gradient(what, instead, *tensors):
 
 def _separate(state, name, *others):
     """An in-place state must not be read through another argument while it is written."""
-    lo = state.data_ptr()
-    hi = lo + state.numel() * state.element_size()
+    storage = state.untyped_storage()._cdata
     for t in others:
-        if t is not None and t.data_ptr() < hi:
-            end = t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-            if end > lo and hi > lo and t.numel():
+        if t is not None and t.untyped_storage()._cdata == storage and t.numel():
+            lo, a = state.data_ptr(), t.data_ptr()
+            end = a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            if end > lo and a < lo + state.numel() * state.element_size():
                 raise LqgHipError(f"{name}: it shares memory with another argument")
 
 
@@ -131,7 +137,7 @@ class _Conv(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 7
         dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else dy
-        dy = dy if _as_it_is(dy) else dy.contiguous()
+        dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
         dev = x.device
         dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
@@ -192,11 +198,11 @@ def _empty_conv(x, w, bias, state, return_state):
 def causal_conv_step(x, state, weight, bias=None, *, silu=False):
     """One step of `causal_conv`: x [trial, channel] -> y [trial, channel]; state [trial, W-1, channel] (contiguous, type of x) is moved
     on IN PLACE.  No gradient."""
-    _no_gradient("causal_conv_step", "use causal_conv", x, state, weight, bias)
     x, w, bias = _conv_check(x, weight, bias, 2)
     B, D = x.shape
     W = w.shape[1]
     state = _state(state, "state", (B, W - 1, D), x.dtype, x, in_place=True)
+    _no_gradient("causal_conv_step", "use causal_conv", x, state, w, bias)
     _separate(state, "state", x, w, bias)
     _on_gpu(x)
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
@@ -256,7 +262,7 @@ class _Scan(torch.autograd.Function):
         nB, T, nD = u.shape
         N, G, dev = A.shape[1], Bm.shape[2], u.device
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
-        dy = dy if _as_it_is(dy) else dy.contiguous()
+        dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
         new = lambda *shape: torch.empty(shape, dtype=u.dtype, device=dev)  # noqa: E731
         du, ddelta, dz = new(nB, T, nD), new(nB, T, nD), None if z is None else new(nB, T, nD)
@@ -329,10 +335,10 @@ def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softpl
 def selective_scan_step(u, delta, state, A, B, C, D=None, *, z=None, delta_bias=None, softplus=False):
     """One step of `selective_scan`: u, delta, z [trial, channel], B, C [trial, N] or [trial, group, N] -> y [trial, channel]; state
     [trial, channel, N] (float32, contiguous) is moved on IN PLACE.  No gradient."""
-    _no_gradient("selective_scan_step", "use selective_scan", u, delta, state, A, B, C, D, z, delta_bias)
     u, delta, A, Bm, Cm, D, z, delta_bias = _scan_check(u, delta, A, B, C, D, z, delta_bias, 2)
     nB, nD = u.shape
     state = _state(state, "state", (nB, nD, A.shape[1]), torch.float32, u, in_place=True)
+    _no_gradient("selective_scan_step", "use selective_scan", u, delta, state, A, Bm, Cm, D, z, delta_bias)
     _separate(state, "state", u, delta, A, Bm, Cm, D, z, delta_bias)
     _on_gpu(u)
     y = torch.empty((nB, nD), dtype=u.dtype, device=u.device)

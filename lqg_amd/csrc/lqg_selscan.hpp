@@ -90,15 +90,18 @@ template <class S> __device__ inline void load_A2(const ScanArgs& a, const Place
 // Row t of a tile is read at a uniform pointer plus a 32-bit offset of the thread, in bytes (row strides are below 2^24 of them).  Loads
 // run two tiles ahead of their use and are never skipped, so that the counter of outstanding loads can be waited on exactly.
 typedef __attribute__((address_space(1))) char gchar;          // in global memory, which a pinned pointer would no longer show
-// (the offset is made opaque where it is used: widened to 64 bits ahead of the loop, it would cost an addition an access and a second
-// register)
+// (as buffer accesses, which add a 32-bit offset of the lane to a uniform base: of a global access the compiler would widen the offset ahead
+// of the loop and add 64 bits an access)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const gchar* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, -1, 0x27000);
+}
 template <class IT> __device__ __forceinline__ IT at_byte(const gchar* p, unsigned off) {
-  asm("" : "+v"(off));
-  return *(const __attribute__((address_space(1))) IT*)(p + off);
+  if constexpr (sizeof(IT) == 2) return __builtin_bit_cast(IT, __builtin_amdgcn_raw_buffer_load_b16(buffer(p), (int)off, 0, 0));
+  else return __builtin_bit_cast(IT, __builtin_amdgcn_raw_buffer_load_b32(buffer(p), (int)off, 0, 0));
 }
 template <class IT> __device__ __forceinline__ void put_byte(gchar* p, unsigned off, IT v) {
-  asm("" : "+v"(off));
-  *(__attribute__((address_space(1))) IT*)(p + off) = v;
+  if constexpr (sizeof(IT) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), buffer(p), (int)off, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), buffer(p), (int)off, 0, 0);
 }
 // keeps a uniform pointer in scalar registers: the optimiser would carry pointer + offset of every row along the loop, 64 bits a lane each
 template <class P> __device__ __forceinline__ void pin(P*& p) { asm("" : "+s"(p)); }
@@ -137,12 +140,12 @@ template <class IT, class S> struct Maps {
   const gchar *p, *q;
   unsigned off[S::Q], step, n;
   int t;
-  bool ok;
+  bool ok, all;                               // the lane's state exists; every state that there is room for does
   __device__ Maps(const lqg_seq& s, const ScanArgs& a, const Place<S>& at) : step((unsigned)s.st * sizeof(IT)) {
     const int f = at.lane & 15, j = f % S::NS;
     t = f / S::NS;
     p = q = (const gchar*)(static_cast<const IT*>(s.ptr) + at.b * s.sb + at.t0 * s.st + at.grp * s.sg);
-    ok = at.n0 + j < a.p.N;
+    ok = at.n0 + j < a.p.N, all = a.p.N == S::NP;
     n = (ok ? at.n0 + j : 0) * sizeof(IT);
 #pragma unroll
     for (int i = 0; i < S::Q; ++i) off[i] = __umul24(t + i * rows, step) + n;
@@ -161,6 +164,11 @@ template <class IT, class S> struct Maps {
   }
   // past N, and behind the end of a tile that is not whole: 0
   template <bool WHOLE> __device__ void widen(const IT (&r)[S::Q], float (&v)[S::Q], long left) const {
+    if (WHOLE && all) {
+#pragma unroll
+      for (int i = 0; i < S::Q; ++i) v[i] = up(r[i]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < S::Q; ++i) v[i] = ok && (WHOLE || t + i * rows < left) ? up(r[i]) : 0.0f;
   }
