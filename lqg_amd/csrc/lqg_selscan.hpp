@@ -528,18 +528,20 @@ template <class S> struct ChannelSum {
 };
 
 // CARRY: leave each chunk's carry (lambda at its start from 0 at its end) and its sum of dl.
+// Iteration i (downwards): finish tile i+1, prepare tile i-1, request tile i-3's rows and tile i-2's maps, walk tile i up and down; one
+// barrier.  The halves of a wave add their sums before they go to LDS, each for every other step.
 template <class IT, class S, bool CARRY>
 __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const ScanArgs a) {
-  constexpr int CH = S::CH, NS = S::NS, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
+  constexpr int CH = S::CH, NS = S::NS, NW = S::NW, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
   __shared__ float2 s_in[2][TT][CH];                      // dl, dl u
   __shared__ float s_dy[2][TT][CH];                       // dY
-  __shared__ float s_own[3][CARRY ? 1 : TT][CH];          // u, d dl / d delta, dy silu'(z): read by the thread that wrote them
-  __shared__ float2 s_sum[CARRY ? 1 : TT][PS][CH];        // s1, s2
-  __shared__ float s_y[CARRY ? 1 : TT][PS][CH];
+  __shared__ float s_own[2][3][CARRY ? 1 : TT][CH];       // u, d dl / d delta, dy silu'(z): read by the thread that wrote them
+  __shared__ float2 s_sum[2][CARRY ? 1 : TT][NW][CH];     // s1, s2
+  __shared__ float s_y[2][CARRY ? 1 : TT][NW][CH];
   const Place<S> at(a);
   const long D = a.p.D, N = a.p.N, T = a.p.T, b = at.b;
   const unsigned d = at.d;
-  const int ch = at.ch, part = at.row;
+  const int ch = at.ch, w = at.row / S::LS, half = at.row % S::LS;
   float A2[NS], lam[NS], dA[NS], sum = 0.0f, dDk = 0.0f, dbias = 0.0f;
   load_A2<S>(a, at, A2);
 #pragma unroll
@@ -604,9 +606,9 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
       s_in[buf][row][ch] = make_float2(dl, du);
       s_dy[buf][row][ch] = dY;
       if (!CARRY) {
-        s_own[0][row][ch] = u;
-        s_own[1][row][ch] = a.p.softplus ? sigmoid(raw) : 1.0f;
-        s_own[2][row][ch] = dg;
+        s_own[buf][0][row][ch] = u;
+        s_own[buf][1][row][ch] = a.p.softplus ? sigmoid(raw) : 1.0f;
+        s_own[buf][2][row][ch] = dg;
       }
     }
   };
@@ -623,19 +625,19 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
       const int row = at.row + i * PS;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-      for (int p = 0; p < PS; ++p) {
-        const float2 s = s_sum[row][p][ch];
+      for (int p = 0; p < NW; ++p) {
+        const float2 s = s_sum[buf][row][p][ch];
         s1 += s.x;
         s2 += s.y;
       }
-      const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[0][row][ch];
+      const float dl = s_in[buf][row][ch].x, dY = s_dy[buf][row][ch], u = s_own[buf][0][row][ch];
       vu[i] = fmaf(dl, s1, Dk * dY);
-      vd[i] = fmaf(u, s1, LN2 * s2) * s_own[1][row][ch];
+      vd[i] = fmaf(u, s1, LN2 * s2) * s_own[buf][1][row][ch];
       if (gate) {
         vz[i] = Dk * u;
 #pragma unroll
-        for (int p = 0; p < PS; ++p) vz[i] += s_y[row][p][ch];
-        vz[i] *= s_own[2][row][ch];
+        for (int p = 0; p < NW; ++p) vz[i] += s_y[buf][row][p][ch];
+        vz[i] *= s_own[buf][2][row][ch];
       }
       const bool in = decltype(whole)::v || row < left;         // (lanes past the group's end have dY = 0, and their sums are not stored)
       if (!in) vu[i] = vd[i] = vz[i] = 0.0f;
@@ -672,11 +674,21 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
   }
   __syncthreads();
   const long part0 = ((at.blk * a.p.B + b) * T + at.t0) * 2 * N;
-  // FAST: tiles i - 3 .. i exist and are whole
+  // FAST: tiles i - 3 .. i + 1 exist and are whole
   auto iteration = [&](int i, auto parity, auto fast) __attribute__((always_inline)) {
     constexpr int P = decltype(parity)::v;
     constexpr bool FAST = decltype(fast)::v;
     const long left = live - (long)i * TT;
+    if (!CARRY && (FAST || i < last)) finish(i + 1, P ^ 1, fast);
+    prepare(rows[P ^ 1], FAST || i > 0 ? TT : 0, P ^ 1, fast);          // (before the first tile: not read)
+    if (FAST) {
+      su.next(rows[P ^ 1].u, -1);
+      sdl.next(rows[P ^ 1].dl, -1);
+      sdy.next(rows[P ^ 1].dy, -1);
+      sz.next(rows[P ^ 1].z, -1);
+    } else {
+      load(rows[P ^ 1], i - 3);
+    }
     float B[Q], C[Q], h0[NS];
     mC.template widen<FAST>(maps[P].C, C, left);
     if (!CARRY) {
@@ -695,19 +707,7 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
     } else {
       load_maps(maps[P], i - 2);
     }
-    auto ahead = [&]() __attribute__((always_inline)) {
-      prepare(rows[P ^ 1], FAST || i > 0 ? TT : 0, P ^ 1, fast);      // (before the first tile: not read)
-      if (FAST) {
-        su.next(rows[P ^ 1].u, -1);
-        sdl.next(rows[P ^ 1].dl, -1);
-        sdy.next(rows[P ^ 1].dy, -1);
-        sz.next(rows[P ^ 1].z, -1);
-      } else {
-        load(rows[P ^ 1], i - 3);
-      }
-    };
     if constexpr (CARRY) {
-      ahead();
       each_back<TT - 1>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::v;
         const float dl = s_in[P][t][ch].x, dY = s_dy[P][t][ch];
@@ -729,13 +729,24 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
         });
       });
       constexpr int GS = Group<S>::GS;
+      // steps come singly (GS = 1) or in even groups; the halves' sums of a pair of steps: the lower half takes the even step
+      float ky = 0.0f, k1 = 0.0f, k2 = 0.0f;
+      auto put_y = [&](auto tc, const float (&v)[GS]) __attribute__((always_inline)) {
+        constexpr int t = decltype(tc)::v;
+        if constexpr (GS == 1) {
+          if constexpr (t & 1) s_y[P][t - 1 + half][w][ch] = merge<5>(ky, v[0], at.lane);
+          else ky = v[0];
+        } else {
+#pragma unroll
+          for (int k = 0; k < GS; k += 2) s_y[P][t + k + half][w][ch] = merge<5>(v[k], v[k + 1], at.lane);
+        }
+      };
       if (gate)
         each<TT / GS>([&](auto gc) __attribute__((always_inline)) {
           constexpr int t0 = decltype(gc)::v * GS;
           float v[GS];
           dot_bcast<S, t0>(C, reinterpret_cast<float(&)[GS][NS]>(hh[t0]), v);
-#pragma unroll
-          for (int k = 0; k < GS; ++k) s_y[t0 + k][part][ch] = v[k];
+          put_y(Int<t0>{}, v);
         });
       float tA[NS], gg[GS][NS], s2[GS];
 #pragma unroll
@@ -762,8 +773,14 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
         if constexpr (k == 0) {
           float s1[GS];
           dot_bcast<S, t>(B, gg, s1);
+          if constexpr (GS == 1) {
+            if constexpr (t & 1) k1 = s1[0], k2 = s2[0];
+            else s_sum[P][t + half][w][ch] = make_float2(merge<5>(s1[0], k1, at.lane), merge<5>(s2[0], k2, at.lane));
+          } else {
 #pragma unroll
-          for (int o = 0; o < GS; ++o) s_sum[t + o][part][ch] = make_float2(s1[o], s2[o]);
+            for (int o = 0; o < GS; o += 2)
+              s_sum[P][t + o + half][w][ch] = make_float2(merge<5>(s1[o], s1[o + 1], at.lane), merge<5>(s2[o], s2[o + 1], at.lane));
+          }
         }
         using CS = ChannelSum<S>;
         float out[CS::K / CS::KG];
@@ -780,14 +797,11 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
       });
 #pragma unroll
       for (int j = 0; j < NS; ++j) dA[j] += tA[j];
-      __syncthreads();
-      finish(i, P, fast);
-      ahead();
     }
     __syncthreads();
   };
   for (int i = last; i >= 0;) {
-    if ((i & 1) && i >= 4 && i < at.full) {               // pairs (odd, even) of whole tiles
+    if ((i & 1) && i >= 4 && i + 1 < at.full) {           // pairs (odd, even) of whole tiles
       su.seek(i - 3), sdl.seek(i - 3), sdy.seek(i - 3), sz.seek(i - 3), mB.seek(i - 2), mC.seek(i - 2);
       if (!CARRY) ck = ck0 + (i - 2) * cktile;
       for (; i >= 4; i -= 2) {
@@ -800,6 +814,7 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
       --i;
     }
   }
+  if (!CARRY && last >= 0) finish(0, 0, Int<0>{});
   if constexpr (CARRY) {
     if (!at.on) return;
     float* hl = a.hl + ((b * a.chunks + at.c) * N + at.n0) * D + d;
@@ -813,7 +828,9 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
       static_cast<IT*>(a.g.ddelta)[out0 + t * D + d] = down<IT>(0.0f);
       if (gate) static_cast<IT*>(a.g.dz)[out0 + t * D + d] = down<IT>(0.0f);
     }
-    s_sum[0][part][ch] = make_float2(dDk, dbias);
+    __syncthreads();
+    float2* const s_end = &s_sum[0][0][0][0];             // [PS][CH]
+    s_end[at.row * CH + ch] = make_float2(dDk, dbias);
     __syncthreads();
     if (!at.on) return;
     float* out = a.partP + (b * a.chunks + at.c) * (N + 2) * D + d;
@@ -826,7 +843,7 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
     if (at.row == 0) {
       float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int k = 0; k < PS; ++k) s.x += s_sum[0][k][ch].x, s.y += s_sum[0][k][ch].y;
+      for (int k = 0; k < PS; ++k) s.x += s_end[k * CH + ch].x, s.y += s_end[k * CH + ch].y;
       out[N * D] = s.x;
       out[(N + 1) * D] = s.y;
     }
