@@ -36,7 +36,7 @@ template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, lo
 // The shape of a workgroup: CH channels x NS NW 64 / CH states, TT steps a tile.
 template <int NS_, int NW_, int TT_> struct Shape {
   static constexpr int CH = CHANNELS, NS = NS_, NW = NW_, TT = TT_;
-  static constexpr int GRAD_WAVES = NS == 2 && NW > 1 ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
+  static constexpr int GRAD_WAVES = NS == 2 && NW > 2 ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
   static constexpr int LS = 64 / CH;          // groups of NS states in a wave
   static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
   static constexpr int NP = NS * PS;          // states it has room for
