@@ -109,7 +109,7 @@ class AdamW:
 
     Tensors are contiguous leaves on one GPU; float32, bfloat16 and float16 may be mixed, float64 ones take an optimiser of their own.
     Arithmetic is float32 (float64 for float64 tensors), every operation rounded by itself; a narrower tensor is rounded once when it is
-    written.  Tensors whose `.grad` is None are left as they are, states included.
+    written.  Tensors whose `.grad` is None are left as they are, states included (t counts the steps of the optimiser).
 
     state_bits=32: moments in float32 (float64 for float64 tensors).  state_bits=8: m and sqrt(v) as e4m3 values in units of one float32
     scale for every 256 elements of a tensor, the block's largest magnitude being 448 units (the root, since an 8-bit float spans 18
@@ -131,7 +131,7 @@ class AdamW:
             raise LqgHipError(f"state_bits must be 8 or 32, got {state_bits!r}")
         if not self.params:
             raise LqgHipError("AdamW: no tensors to step")
-        seen, wide = set(), [p.dtype == torch.float64 for p in self.params]
+        wide = [p.dtype == torch.float64 for p in self.params]
         dev = self.params[0].device
         for p in self.params:
             if p.dtype not in _learn.TYPES:
@@ -142,9 +142,9 @@ class AdamW:
                 raise LqgHipError("AdamW: a tensor is not a leaf: its gradient is not kept")
             if not p.is_contiguous():
                 raise LqgHipError(f"AdamW: a contiguous tensor is needed, got strides {tuple(p.stride())} for {tuple(p.shape)}")
-            if p.numel() and p.data_ptr() in seen:
-                raise LqgHipError("AdamW: the same tensor twice")
-            seen.add(p.data_ptr())
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise LqgHipError("AdamW: the same tensor twice, or two that share memory")
         if any(wide) and not all(wide):
             raise LqgHipError("AdamW: float64 tensors take an optimiser of their own")
         if any(wide) and state_bits == 8:

@@ -21,6 +21,7 @@ def test_adamw_refuses():
             (lambda: AdamW([t], lr=float("nan")), "lr"), (lambda: AdamW([t], betas=(1.0, 0.9)), "betas"),
             (lambda: AdamW([t], eps=-1e-8), "eps"), (lambda: AdamW({"a": [t, 3.0]}), "a tensor is needed, got float"),
             (lambda: AdamW([t.int()]), "unsupported dtype"), (lambda: AdamW([t, t]), "same tensor twice"),
+            (lambda: AdamW([t[:3], t[2:]]), "share memory"),
             (lambda: AdamW([torch.zeros(3, 4).t()]), "contiguous"), (lambda: AdamW([leaf * 2]), "not a leaf"),
             (lambda: AdamW([t, t.double()]), "of their own"), (lambda: AdamW([t.double()], state_bits=8), "32-bit or wider"),
             (lambda: AdamW([t, torch.zeros(3, device="meta")]), "one device"), (lambda: AdamW(iter([t])), "no CPU fallback")):
@@ -384,6 +385,20 @@ def test_other_stream():
     torch.cuda.current_stream().wait_stream(side)
     B.step()
     assert torch.equal(p.detach(), q.detach())
+
+
+@gpu
+def test_more_than_2_to_31_elements():
+    n = 2 ** 31 + 700
+    p = torch.zeros(n, dtype=BF16, device="cuda")
+    p.grad = torch.zeros(n, dtype=BF16, device="cuda")
+    tail = tensors(BF16, ((1000,),), seed=7)[0]
+    p.grad[-1000:] = tail
+    opt = AdamW(p, lr=0.5, weight_decay=0.0, state_bits=8)
+    opt.step()
+    assert not p[:-1000].any() and torch.equal(p[-1000:].float().sign(), -tail.float().sign())
+    # the first step is lr in each direction: m / (1 - b1) over sqrt(v / (1 - b2)), 10 roundings of float, one of bfloat16
+    assert float((p[-1000:].float().abs() - 0.5).abs().max()) <= 0.5 * (O.half(BF16) + 2.0 ** -20)
 
 
 # ------------------------------------------------------------------------------------------------ together

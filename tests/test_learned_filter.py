@@ -232,6 +232,10 @@ SCAN = [  # B, T, D, N, G, dtype, gate, softplus, state, D skip, delta bias, len
     (2, 100, 64, 4, 1, F32, False, False, True, False, False, (99, 100)), (4, 35, 63, 8, 1, F16, True, True, True, True, True, (35, 1, 0, 17)),
     (2, 31, 33, 2, 33, F32, True, True, True, True, True, None), (2, 150, 80, 16, 1, BF16, True, True, True, True, True, (150, 77)),
     (70, 3, 8, 5, 2, F32, True, True, True, True, True, None),
+    # long enough for the loops over whole tiles, each shape of a workgroup
+    (2, 200, 40, 16, 1, F32, True, True, True, True, True, (200, 131)), (2, 150, 72, 20, 3, F32, True, True, True, True, True, (97, 150)),
+    (3, 130, 33, 6, 1, BF16, False, True, True, True, True, (130, 128, 5)), (1, 90, 70, 40, 2, F16, True, True, False, True, True, None),
+    (2, 176, 40, 3, 2, F32, True, True, True, True, True, None), (1, 128, 64, 13, 1, F32, False, True, False, False, True, None),
 ]
 KEYS = ("gate", "softplus", "state", "skip", "bias", "lengths")
 
@@ -524,3 +528,66 @@ def test_extremes():
     y = ssm.selective_scan(u, torch.full_like(u, 0.5), A, one.expand(1, 20, 1), one.expand(1, 20, 1))
     assert torch.equal(y[0, :, 0], torch.full((20,), 0.5, device="cuda")) and torch.equal(y[0, :, 3], torch.ones(20, device="cuda"))
     assert not torch.isfinite(y[0, :, 1:3]).any()
+
+
+@gpu
+def test_far_apart_steps():
+    """Time strides at and beyond what the kernels address without a copy."""
+    A = -torch.rand(8, 4, device="cuda")
+    for stride in ((1 << 22) - 1, 1 << 22):
+        base = torch.empty(18 * stride, dtype=BF16, device="cuda")
+        u = base.as_strided((1, 18, 8), (18 * stride, stride, 1))
+        u.copy_(torch.randn(1, 18, 8, device="cuda"))
+        m = u[..., :4]
+        flat = u.contiguous()
+        outs = []
+        for v, k in ((u, m), (flat, m.contiguous())):
+            # (a leaf for each use: of one leaf autograd would add the uses' bfloat16 gradients, in an order that a copy's node changes)
+            x, dl, z, xc = (t.detach().requires_grad_() for t in (v, v.abs() * 0.3, v, v))
+            y = ssm.selective_scan(x, dl, A, k, k, z=z)
+            c = ssm.causal_conv(xc, A, silu=True)
+            outs.append((y, c, *torch.autograd.grad((y, c), (x, dl, z, xc), (flat, flat))))
+        for p, q in zip(*outs):
+            assert torch.equal(p, q)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows are those of the same channels alone."""
+    T, D = 70000, 32768
+    u = torch.randn(1, T, D, dtype=BF16, device="cuda")
+    few = slice(D - 40, D)
+    A, m = -torch.rand(D, 1, device="cuda"), torch.randn(1, T, 1, dtype=BF16, device="cuda")
+    w = torch.randn(D, 3, dtype=BF16, device="cuda")
+    last = torch.tensor([T - 3], device="cuda", dtype=torch.int32)
+    with options.override(SELSCAN_CHUNKS=1):
+        y, h = ssm.selective_scan(u, u, A, m, m, softplus=True, lengths=last, return_state=True)
+        v = u[..., few].contiguous()
+        y2, h2 = ssm.selective_scan(v, v, A[few].contiguous(), m, m, softplus=True, lengths=last, return_state=True)
+    assert torch.equal(y[..., few], y2) and torch.equal(h[:, few], h2)
+    del y
+    c, s = ssm.causal_conv(u, w, silu=True, lengths=last, return_state=True)
+    c2, s2 = ssm.causal_conv(v, w[few].contiguous(), silu=True, lengths=last, return_state=True)
+    assert torch.equal(c[..., few], c2) and torch.equal(s[..., few], s2)
+
+
+@gpu
+def test_inference_mode_and_refused_gradients():
+    i, kw = scan_case(2, 3, 8, 4, 1, F32, softplus=True)
+    with torch.inference_mode():
+        y, h = ssm.selective_scan(**i, **kw, return_state=True)
+        one = {k: (v[:, 0] if k in ("u", "delta", "B", "C") else v) for k, v in i.items() if k in ("u", "delta", "A", "B", "C")}
+        ssm.selective_scan_step(**one, state=h, **kw)
+        x, s = ssm.causal_conv(i["u"], i["A"], return_state=True)
+        ssm.causal_conv_step(i["u"][:, 0], s, i["A"])
+    assert torch.isfinite(h).all() and torch.isfinite(s).all()
+    u = i["u"].detach().requires_grad_()
+    g, = torch.autograd.grad(ssm.selective_scan(**{**i, "u": u}, **kw).sum(), u, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), u)              # once differentiable
+    st = torch.zeros(2, 8, 4, device="cuda")
+    y = ssm.selective_scan(**{**i, "u": u, "state": st}, **kw)
+    with torch.no_grad():
+        ssm.selective_scan_step(**one, state=st, **kw)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
