@@ -47,14 +47,13 @@ template <int NS_, int NW_, int TT_> struct Shape {
 
 // where a thread is
 template <class S> struct Place {
-  int lane, tid, ch, n0, row, tiles, full;    // ch: its channel in the block (as lane and as thread: the same); row: its first row
+  int lane, ch, n0, row, tiles, full;         // ch: its channel in the block; row: its first row of a tile
   long b, c, blk, grp, t0, t1, len;
   unsigned d;                                 // its channel, repeated past the end of the group (`on` false: nothing is stored)
   bool on;
   __device__ Place(const ScanArgs& a) {
     lane = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
-    tid = w * 64 + lane;
     ch = lane % S::CH;
     n0 = (w * S::LS + lane / S::CH) * S::NS;
     row = w * S::LS + lane / S::CH;
@@ -180,10 +179,11 @@ template <class S, int T, int J> __device__ inline float bc(const float (&r)[S::
 
 // y[g] = sum_j bc(C)(T + g, j) h[g][j] for GS steps.  The broadcast is an operand modifier of the multiply-add, which the compiler folds into
 // products only (it would copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart
-// from the broadcasts' reads; several steps in a block share them.
+// from the broadcasts' reads; several steps in a block share them.  SWAP: y goes into a swap of lanes, which must not read it in the
+// two wait states after its write; the compiler keeps its own instructions apart, and does not see these.
 template <class S> struct Group { static constexpr int GS = S::NS == 2 ? 4 : S::NS == 4 ? 2 : 1; };
 #define LQG_FMAC_BCAST(Y, C, K, X) "v_fmac_f32_dpp " Y ", " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
-template <class S, int T> __device__ __forceinline__ void dot_bcast(const float (&C)[S::Q], const float (&h)[Group<S>::GS][S::NS], float (&y)[Group<S>::GS]) {
+template <class S, int T, bool SWAP> __device__ __forceinline__ void dot_bcast(const float (&C)[S::Q], const float (&h)[Group<S>::GS][S::NS], float (&y)[Group<S>::GS]) {
   constexpr int f = T * S::NS, k = f % 16;
   const float c = C[f / 16];
   if constexpr (S::NS == 2) {
@@ -208,6 +208,11 @@ template <class S, int T> __device__ __forceinline__ void dot_bcast(const float 
         : "+v"(y[0])
         : "v"(c), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[0][4]), "v"(h[0][5]), "v"(h[0][6]), "v"(h[0][7]),
           "n"(k + 1), "n"(k + 2), "n"(k + 3), "n"(k + 4), "n"(k + 5), "n"(k + 6), "n"(k + 7));
+  }
+  if constexpr (SWAP) {
+    if constexpr (S::NS == 2) asm("s_nop 1" : "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3]));
+    else if constexpr (S::NS == 4) asm("s_nop 1" : "+v"(y[0]), "+v"(y[1]));
+    else asm("s_nop 1" : "+v"(y[0]));
   }
 }
 // x[j] += bc(C)(T, j) f
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(64 * S::NW) void k_scan(const ScanArgs a) {
         if (CARRY) sum += in[t].x;
       });
       if (!CARRY) {
-        dot_bcast<S, t0>(C, hh, v);
+        dot_bcast<S, t0, false>(C, hh, v);
 #pragma unroll
         for (int k = 0; k < GS; ++k) s_y[P][t0 + k][part][ch] = v[k];
       }
@@ -449,18 +454,20 @@ template <int BIT> __device__ __forceinline__ float merge(float x, float y, int 
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
   } else {
+    static_assert(BIT < 2, "merge_all's");
     const bool hi = lane >> BIT & 1;
     const float keep = hi ? y : x, give = hi ? x : y;
-    return keep + dpp<BIT == 3 ? DPP_ROR8 : BIT == 2 ? DPP_HALF_MIRROR : BIT == 1 ? DPP_XOR2 : DPP_XOR1>(give);
+    return keep + dpp<BIT == 1 ? DPP_XOR2 : DPP_XOR1>(give);
   }
 }
 #define LQG_MERGE(O, X, Y, M, B) "v_add_f32_dpp " O ", " X ", " X " " M " row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp " O ", " Y ", " Y " " M " row_mask:0xf bank_mask:" B "\n\t"
 // M merges over bit BIT, in a block that waits once for what wrote its operands
 template <int BIT, int M> __device__ __forceinline__ void merge_all(float* x, const float* y, int lane) {
-  if constexpr (BIT >= 4 || BIT < 2 || M % 4) {
+  if constexpr (BIT >= 4 || BIT < 2) {
 #pragma unroll
     for (int k = 0; k < M; ++k) x[k] = merge<BIT>(x[k], y[k], lane);
   } else {
+    static_assert(M % 4 == 0, "");
 #pragma unroll
     for (int k = 0; k < M; k += 4) {
       float o0, o1, o2, o3;
@@ -484,9 +491,9 @@ constexpr int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 // of the step on the upper ones, bits of the value on the lower, so that one sum ends in each lane: 2 instructions a value and not 12.
 template <class S> struct ChannelSum {
   static constexpr int K = 2 * S::NS, KG = K < 8 ? K : 8;                   // values of a step, of a group that ends together
-  static constexpr int TB = log2_of(S::CH) - log2_of(KG), TG = 1 << TB;     // bits of the step in the tree, steps of a tree
+  static constexpr int TB = log2_of(S::CH) - log2_of(KG);                   // bits of the step in the tree: 1 << TB steps
   float held[TB][K];
-  // v: the values of step T (steps come downwards); true when the tree of steps T .. T + TG - 1 is whole: out has K / KG sums
+  // v: the values of step T (steps come downwards); true when the tree of the 1 << TB steps from T on is whole: out has K / KG sums
   template <int T> __device__ bool add(float (&v)[K], int lane, float (&out)[K / KG]) {
     return level<T, 0>(v, lane, out);
   }
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
         each<TT / GS>([&](auto gc) __attribute__((always_inline)) {
           constexpr int t0 = decltype(gc)::v * GS;
           float v[GS];
-          dot_bcast<S, t0>(C, reinterpret_cast<float(&)[GS][NS]>(hh[t0]), v);
+          dot_bcast<S, t0, true>(C, reinterpret_cast<float(&)[GS][NS]>(hh[t0]), v);
           put_y(Int<t0>{}, v);
         });
       float tA[NS], gg[GS][NS], s2[GS];
@@ -772,7 +779,7 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
         });
         if constexpr (k == 0) {
           float s1[GS];
-          dot_bcast<S, t>(B, gg, s1);
+          dot_bcast<S, t, true>(B, gg, s1);
           if constexpr (GS == 1) {
             if constexpr (t & 1) k1 = s1[0], k2 = s2[0];
             else s_sum[P][t + half][w][ch] = make_float2(merge<5>(s1[0], k1, at.lane), merge<5>(s2[0], k2, at.lane));
