@@ -52,7 +52,7 @@ int lqg_causal_conv_step(const lqg_conv* p, void* stream);
  *   y_t = (sum_n C_t h_t + D u_t) [* silu(z_t)]
  * A [D][N]; B, C [batch][time][G][N], group g serves channels g D/G ..; state [B][D][N] float or NULL (zeros).
  * D and time strides below 2^22.  Padding as above: y is 0 and h stays.  state_out [B][D][N] float or NULL.
- * checkpoints (or NULL): lqg_scan_checkpoint_bytes of memory that lqg_selective_scan_grad reads.
+ * checkpoints (or NULL): lqg_selscan_checkpoint_bytes of memory that lqg_selective_scan_grad reads.
  */
 typedef struct lqg_selscan {
   int32_t type, softplus;

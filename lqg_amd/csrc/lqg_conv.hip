@@ -369,7 +369,7 @@ hipError_t row_sum(const RowSum& s, const RowSumOut& out, hipStream_t stream) {
   const long blocks = (s.cols + 63) / 64;
   const float* in = s.in;
   long rows = s.rows;
-  if (const long mid = row_sum_mid_rows(rows)) {
+  if (const long mid = row_sum_mid_rows(rows, s.cols)) {
     hipLaunchKernelGGL(k_row_sum_mid, dim3((unsigned)(blocks * mid)), dim3(64, 16), 0, stream, in, rows, s.cols, mid, s.mid);
     in = s.mid;
     rows = mid;
@@ -393,7 +393,7 @@ extern "C" int lqg_causal_conv(const lqg_conv* p, void* stream) {
 extern "C" size_t lqg_causal_conv_grad_workspace(const lqg_conv* p) {
   if (check(p, false)) return 0;
   const long piece = piece_of(p, MAX_GPIECE), rows = p->B * ((p->T + piece - 1) / piece), cols = (p->W + 1) * p->D;
-  return (size_t)(rows + row_sum_mid_rows(rows)) * cols * sizeof(float);
+  return (size_t)(rows + row_sum_mid_rows(rows, cols)) * cols * sizeof(float);
 }
 
 extern "C" int lqg_causal_conv_grad(const lqg_conv* p, lqg_seq dy, const void* dstate_out, void* dx, void* dstate, void* dw,

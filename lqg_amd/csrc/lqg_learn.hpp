@@ -64,11 +64,12 @@ constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_ROR
 inline bool grid_fits(long groups, int threads) { return groups > 0 && groups <= 0x7fffffffL && groups * (long)threads < (1L << 32); }
 
 // out[o][c] = sum over the rows r = o, o + outs, .. of in[r][c], in double, in a fixed order; outs = 1: stored as `type` to final[c's
-// place].  Two launches (rows -> 64 -> 1) when rows are many.  Defined in lqg_conv.hip.
+// place].  Two launches (rows -> 64 -> 1) when rows are many and columns are not: a million columns fill the card with one pass (16384
+// workgroups of 16 waves), and 64 times their workgroups are more than a launch may have from 4 million on.  Defined in lqg_conv.hip.
 struct RowSum {
   const float* in;         // [rows][cols]
   long rows, cols;
-  float* mid;              // [min(rows, 64)][cols] workspace
+  float* mid;              // [row_sum_mid_rows(rows, cols)][cols] workspace
 };
 // column c of the sum goes to seg[s] with begin[s] <= c < begin[s + 1], at place perm(c - begin[s]): [cols / inner][inner] -> transposed
 struct RowSumOut {
@@ -78,7 +79,8 @@ struct RowSumOut {
   long major[3], minor[3];     // column c' of segment s is (c' / minor, c' % minor) -> stored at (c' % minor) * major + c' / minor
 };
 hipError_t row_sum(const RowSum& s, const RowSumOut& out, hipStream_t stream);
-inline long row_sum_mid_rows(long rows) { return rows > 256 ? 64 : 0; }
+inline long row_sum_mid_rows(long rows, long cols) { return rows > 256 && cols <= 1 << 20 ? 64 : 0; }
+inline bool row_sum_fits(long cols) { return grid_fits((cols + 63) / 64, 1024); }
 
 inline hipError_t last() { return hipGetLastError(); }
 

@@ -89,7 +89,7 @@ GradSpace grad_space(const ScanArgs& a) {
   s.group = a.blocks * a.p.B * a.p.T * a.p.N;
   s.rows = a.p.B * a.chunks;
   s.cols = (a.p.N + 2) * a.p.D;
-  s.mid = row_sum_mid_rows(s.rows) * s.cols;
+  s.mid = row_sum_mid_rows(s.rows, s.cols) * s.cols;
   s.total = s.carry + 2 * s.group + s.rows * s.cols + s.mid;
   return s;
 }
@@ -135,7 +135,7 @@ extern "C" int lqg_selective_scan_grad(const lqg_selscan* p, const lqg_selscan_b
   a.partP = a.partBC + 2 * s.group;
   hipStream_t st = (hipStream_t)stream;
   const long n = p->B * p->T * p->G * 2 * p->N, groups = (n + 255) / 256;
-  if (!grid_fits(groups, 256)) return LQG_ERR_ARG;
+  if (!grid_fits(groups, 256) || !row_sum_fits(s.cols)) return LQG_ERR_ARG;
   if (const int rc = by_type(1, a, st)) return rc;
   const int rc = p->type == LQG_T_F32 ? ScanOf<float>::groups(a, groups, st)
                  : p->type == LQG_T_BF16 ? ScanOf<bf16>::groups(a, groups, st) : ScanOf<f16>::groups(a, groups, st);

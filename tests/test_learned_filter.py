@@ -591,3 +591,24 @@ def test_inference_mode_and_refused_gradients():
         ssm.selective_scan_step(**one, state=st, **kw)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@gpu
+def test_gradient_sums_of_many_trials_and_wide_rows():
+    """Sums over trials where rows are many and so are columns."""
+    B, D, N = 257, 262144, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    u = torch.randn(B, 1, D, dtype=BF16, device="cuda", generator=g)
+    m = torch.randn(B, 1, N, dtype=BF16, device="cuda", generator=g)
+    A, skip = -torch.rand(D, N, device="cuda", generator=g), torch.randn(D, device="cuda", generator=g)
+    h = torch.randn(B, D, N, device="cuda", generator=g)
+    A.requires_grad_(), skip.requires_grad_()
+    delta = u.abs() * 0.25
+    dA, dD = torch.autograd.grad(ssm.selective_scan(u, delta, A, m, m, skip, state=h).float().sum(), (A, skip))
+    # one step: dA = sum_b C dl exp(dl A) h, dD = sum_b u; relative to the terms' magnitudes each is a few roundings to float
+    for few in (slice(0, 500), slice(D - 500, D)):
+        dl, C = d64(delta[:, 0, few]), d64(m[:, 0])
+        terms = C[:, None, :] * dl[..., None] * torch.exp(dl[..., None] * d64(A[few].detach())) * d64(h[:, few])
+        assert float((d64(dA[few]) - terms.sum(0)).abs().max() / terms.abs().sum(0).max()) < 16 * 2.0 ** -24
+        x = d64(u[:, 0, few])
+        assert float((d64(dD[few]) - x.sum(0)).abs().max() / x.abs().sum(0).max()) < 16 * 2.0 ** -24
