@@ -19,7 +19,6 @@ _SEQ, _PARAM = "Pqqq", "Pii"
 CONV = struct.Struct("@4i3q" + 2 * _SEQ + 2 * _PARAM + "3P")                   # lqg_conv
 SELSCAN = struct.Struct("@2i5q" + 6 * _SEQ + 3 * _PARAM + "4P2i")              # lqg_selscan
 SELSCAN_BARS = struct.Struct("@" + _SEQ + "10P")                               # lqg_selscan_bars
-SEQ = struct.Struct("@" + _SEQ)
 NO_SEQ, NO_PARAM = (0, 0, 0, 0), (0, 0, 0)
 
 
@@ -83,11 +82,12 @@ def ptr(t):
 
 
 def seq(t):
-    """[B, T, D] or [B, T, G, N] (channel stride 1): pointer, trial, time and group strides."""
+    """[B, T, D] or [B, T, G, N] (channel stride 1): pointer, trial, time and group strides.  (The time stride of a single step means
+    nothing, and may be as large as it likes.)"""
     if t is None:
         return NO_SEQ
     st = t.stride()
-    return t.data_ptr(), st[0], st[1], st[2] if len(st) == 4 else 0
+    return t.data_ptr(), st[0], st[1] if t.shape[1] > 1 else 0, st[2] if len(st) == 4 else 0
 
 
 def row(t):

@@ -102,6 +102,25 @@ def _separate(state, name, *others):
                 raise LqgHipError(f"{name}: it shares memory with another argument")
 
 
+# Autograd adds up a leaf's gradient in a node that lives as long as any graph which holds it, on the stream it was made on.  A backward
+# pass under capture must not meet one of the default stream: the wait between the two streams breaks the capture and ends the process.
+_LEAF = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+
+
+def _note_leaves(fn, device):
+    """Marks the leaves' nodes that an eager call on the default stream holds."""
+    if _learn.stream(device) == 0:
+        for node, _ in fn.next_functions:
+            if type(node) is _LEAF:
+                node.metadata["lqg_default_stream"] = True
+
+
+def _capture_check(fn, what):
+    if torch.cuda.is_current_stream_capturing() and any(type(n) is _LEAF and "lqg_default_stream" in n.metadata for n, _ in fn.next_functions):
+        raise LqgHipError(f"{what}: this backward pass is captured while a graph of an earlier call on the default stream, with the same "
+                          "leaves, is alive: drop that call's outputs before the capture (or make it on another stream)")
+
+
 # ------------------------------------------------------------------------------------------------ short causal convolution
 
 def _conv_desc(x, w, bias, silu, B, T, D, xv, yv, state, state_out, lengths):
@@ -131,6 +150,7 @@ class _Conv(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
+        _capture_check(ctx, "causal_conv")
         x, w, bias, state, lengths = ctx.saved_tensors
         B, T, D = x.shape
         W = w.shape[1]
@@ -176,8 +196,10 @@ def causal_conv(x, weight, bias=None, *, state=None, lengths=None, silu=False, r
     _on_gpu(x)
     if not x.numel():
         return _empty_conv(x, w, bias, state, return_state)
-    run = _Conv.apply if _tracked(x, w, bias, state) else _conv_forward
-    y, last = run(x, w, bias, state, lengths, int(bool(silu)), bool(return_state))
+    keep = _tracked(x, w, bias, state)
+    y, last = (_Conv.apply if keep else _conv_forward)(x, w, bias, state, lengths, int(bool(silu)), bool(return_state))
+    if keep:
+        _note_leaves(y.grad_fn, x.device)
     return (y, last) if return_state else y
 
 
@@ -256,6 +278,7 @@ class _Scan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
+        _capture_check(ctx, "selective_scan")
         u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck = ctx.saved_tensors
         if dy is None and dlast is None:
             return (None,) * 12
@@ -327,6 +350,7 @@ def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softpl
         return (y, last) if return_state else y
     if keep:
         y, last = _Scan.apply(*inputs, lengths, int(bool(softplus)), bool(return_state))
+        _note_leaves(y.grad_fn, u.device)
     else:
         y, last, _ = _scan_forward(*inputs, lengths, int(bool(softplus)), bool(return_state), False)
     return (y, last) if return_state else y

@@ -1,4 +1,6 @@
 """lqg_amd.belief.ssm: the short causal convolution and the selective state-space scan, against float64 step by step."""
+import gc
+
 import pytest
 import torch
 
@@ -612,3 +614,51 @@ def test_gradient_sums_of_many_trials_and_wide_rows():
         assert float((d64(dA[few]) - terms.sum(0)).abs().max() / terms.abs().sum(0).max()) < 16 * 2.0 ** -24
         x = d64(u[:, 0, few])
         assert float((d64(dD[few]) - x.sum(0)).abs().max() / x.abs().sum(0).max()) < 16 * 2.0 ** -24
+
+
+def test_a_single_step_has_no_time_stride():
+    from lqg_amd import _learn
+    x = torch.zeros(4, 8).as_strided((4, 1, 8), (8, 1 << 23, 1))
+    assert _learn.seq(ssm._sequence(x, "x", 3))[2] == 0
+
+
+@gpu
+def test_single_steps_far_apart():
+    """One step of trials that are laid out time first: its time stride, beyond what a tile addresses, is not used."""
+    i, kw = scan_case(3, 1, 8, 4, 1, F32, softplus=True)
+    far = {k: (t.as_strided(t.shape, (t.stride(0), 1 << 23, *t.stride()[2:])) if k in ("u", "delta", "B", "C") else t) for k, t in i.items()}
+    leaf = lambda v: {k: (t.detach().requires_grad_() if k == "u" else t) for k, t in v.items()}  # noqa: E731
+    a, b = leaf(i), leaf(far)
+    b["u"] = far["u"].detach().requires_grad_()
+    ya, yb = ssm.selective_scan(**a, **kw), ssm.selective_scan(**b, **kw)
+    assert torch.equal(ya, yb)
+    for p, q in zip(torch.autograd.grad(ya, a["u"], i["u"]), torch.autograd.grad(yb, b["u"], far["u"])):
+        assert torch.equal(p, q)
+    assert torch.equal(ssm.causal_conv(i["u"], i["A"]), ssm.causal_conv(far["u"], i["A"]))
+
+
+@gpu
+def test_capture_beside_a_living_eager_graph_is_refused():
+    i, kw = scan_case(2, 5, 8, 4, 1, F32, softplus=True)
+    A = i["A"].detach().requires_grad_()
+    calls = {"selective_scan": lambda: ssm.selective_scan(**{**i, "A": A}, **kw), "causal_conv": lambda: ssm.causal_conv(i["u"], A)}
+    for name, call in calls.items():
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()                               # (a forward pass alone may be captured)
+            with pytest.raises(LqgHipError, match=name + ".*drop that call's outputs"):
+                torch.autograd.grad(y, A, i["u"])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive)
+        want, = torch.autograd.grad(alive, A, i["u"])
+        del alive, y
+        gc.collect()                                 # (what the error's traceback held)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(call(), A, i["u"])
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
