@@ -3,6 +3,7 @@
 #include "lqg_selscan.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace lqg::learn;
 
@@ -47,13 +48,36 @@ int check(const lqg_selscan* p) {
 long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
 int tile_of(long N) { return N > 32 ? 8 : 16; }
 
-// Waves on the 1024 SIMDs decide whether the time axis is cut.  A cut costs the pass that leaves the chunks' carries (forward 0.7 of the
-// main pass, backward a third of it) and pays while SIMDs are empty, or, where registers let two waves share a SIMD, while one waits
-// alone.  Measured at 2048 steps, bfloat16 (us, uncut / cut; waves uncut):  forward N = 16: 185 / 287 (2048), 132 / 167 (1024), 129 / 93
-// in 4 (512); N = 4: 208 / 176 in 2 (512).  Backward N = 16: 620 / 860 (2048), 404 / 353 in 2 (1024); N = 8: 545 / 581 (1024), 440 / 300
-// in 4 (512); N = 24: 590 / 730 (1024), 565 / 377 in 2 (512).  So: below 0.75 waves a SIMD (backward with 9 to 16 states: below 1.5) into
-// as many pieces as fill the SIMDs, twice where registers allow it (not with one wave a workgroup, N <= 4, nor backward beyond 16
-// states); a piece is 8 tiles at least.
+// Time of a pass of w waves over the whole axis, in units of one that half fills the 1024 SIMDs: as many rounds as fill them, and a tenth
+// more when every SIMD is taken.  Forward with 5 to 8 states workgroups of two waves share SIMDs early, and backward with 9 to 16 states
+// registers let two waves share one, so that one alone, which waits by itself, leaves time unused (in both 1.3).
+double pass_time(long N, bool grad, long w) {
+  const double q = w / 1024.0;
+  const bool shared = grad ? N > 8 && N <= 16 : N > 4 && N <= 8;
+  if (q <= 0.5) return 1.0;
+  if (q <= 1.0) return shared ? 1.3 : 1.1;
+  if (shared && !grad) return q <= 2.0 ? 1.6 : 0.96 * q;
+  return std::ceil(q);
+}
+
+// Pieces of the time axis.  A cut into c adds the pass that leaves the carries of c - 1 of them (0.55 of the main pass's time forward, 0.2
+// backward), 3 tiles a piece before its loads are under way, and a launch (6 tiles): the c with the least sum.  Measured, bfloat16 with
+// gate, us uncut / in 2 / 4 / 8 at 2048 steps:  forward N = 16: 126 / 115 / 88 / 88 (512 waves uncut), 128 / 138 / 135 / 143 (1024);
+// N = 8: 149 / 151 / 98 / 107 (512), 192 / 179 / 170 / 198 (1024).  Backward N = 16: 366 / 258 / 188 / 198 (512), 379 / 325 / 333 / 367
+// (1024), 516 / 598 / 630 / 700 (2048); N = 24: 572 / 393 / 392 / 439 (512), 592 / 689 / 734 / 841 (1024), 1144 / 1026 / 934 / 979 (1100).
+// Over 164 such rows (N = 4 .. 64, 512 to 6000 steps, 64 to 2048 waves) the choice is 1.3 % slower than the best cut (geometric mean, 25 %
+// at most); filling the SIMDs up to a threshold of waves was 6.8 % (54 %).
+long pieces(long N, bool grad, long waves, long tiles) {
+  long best = 1;
+  double least = pass_time(N, grad, waves);
+  for (long c = 2; c <= std::min(64L, tiles / 8); ++c) {
+    const double t = (pass_time(N, grad, waves * c) + (grad ? 0.2 : 0.55) * pass_time(N, grad, waves * (c - 1))) * (1.0 / c + 3.0 / tiles) +
+                     6.0 / tiles;
+    if (t < least) least = t, best = c;
+  }
+  return best;
+}
+
 ScanArgs describe(const lqg_selscan* p, bool grad) {
   ScanArgs a{};
   a.p = *p;
@@ -63,9 +87,7 @@ ScanArgs describe(const lqg_selscan* p, bool grad) {
   a.blocks = a.bpg * p->G;
   a.tiles = (p->T + TT - 1) / TT;
   const long waves = a.blocks * p->B * (p->N > 8 ? 4 : p->N > 4 ? 2 : 1);
-  const long enough = grad && p->N > 8 && p->N <= 16 ? 1536 : 768, room = p->N > 4 && !(grad && p->N > 16) ? 2048 : 1024;
-  a.chunks = waves >= enough ? 1 : std::min({64L, (a.tiles + 7) / 8, (room + waves - 1) / waves});
-  if (p->chunks) a.chunks = std::min((long)p->chunks, a.tiles);
+  a.chunks = p->chunks ? std::min((long)p->chunks, a.tiles) : pieces(p->N, grad, waves, a.tiles);
   const long per = (a.tiles + a.chunks - 1) / a.chunks;
   a.chunk = per * TT;
   a.chunks = (a.tiles + per - 1) / per;               // no empty chunk

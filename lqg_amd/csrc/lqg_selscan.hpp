@@ -25,6 +25,7 @@ struct ScanArgs {
   lqg_selscan_bars g;
   long Dg, bpg, blocks;          // channels of a group, blocks of CHANNELS of them, blocks in all
   long chunks, chunk, tiles;     // chunks of the time axis, their steps (a multiple of TT), tiles of TT steps in T
+  long run, first;               // chunks of this launch, the first of them
   float *hl, *sd;                // carries [B][chunks][N][D], sums of dl [B][chunks][D]
   float *partBC, *partP;         // gradients: [blocks][B][T][2][N], [B * chunks][N + 2][D]
 };
@@ -62,8 +63,8 @@ template <class S> struct Place {
     const unsigned id = x * q + min(x, r) + blockIdx.x / 8;
     blk = id % (unsigned)a.blocks;
     const unsigned rest = id / (unsigned)a.blocks;
-    c = rest % (unsigned)a.chunks;
-    b = rest / (unsigned)a.chunks;
+    c = a.first + rest % (unsigned)a.run;
+    b = rest / (unsigned)a.run;
     grp = (unsigned)blk / (unsigned)a.bpg;
     const long in = (blk - grp * a.bpg) * S::CH + ch;
     on = in < a.Dg;
@@ -894,6 +895,10 @@ template <class T> __device__ inline void load4(const T* p, bool whole, long lef
   }
 }
 
+// The state is read and written past the caches (it comes back after every other layer of a model): 1024 x 4096 x 16: 149 -> 124 us = 4.3
+// TB/s; 256 x 4096 x 16, which the last cache holds: 33 -> 32.  Several trials or several fours of states a lane, for more loads on their
+// way: 2 to 70 % slower.
+typedef float StateVec __attribute__((ext_vector_type(4), aligned(4)));
 template <class IT, int LPC>
 __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* state) {
   const long N = a.p.N, D = a.p.D;
@@ -906,7 +911,13 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* stat
   const bool whole = left >= 4;
   float* hp = state + (b * D + d) * N + n;
   float h[4], A[4], B[4], C[4];
-  load4(hp, whole, left, h);
+  if (whole) {
+    const StateVec r = __builtin_nontemporal_load(reinterpret_cast<const StateVec*>(hp));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = r[j];
+  } else {
+    load4(hp, false, left, h);
+  }
   if (a.p.A.type == LQG_T_F32) load4(static_cast<const float*>(a.p.A.ptr) + d * N + n, whole, left, A);
   else
 #pragma unroll
@@ -917,8 +928,9 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* stat
   const float u = up(seq<IT>(a.p.u, b, d)[0]);
   const float z = a.p.z.ptr ? up(seq<IT>(a.p.z, b, d)[0]) : 0.0f;
   float dl = up(seq<IT>(a.p.delta, b, d)[0]);
-  if (a.p.delta_bias.ptr) dl += load_param(a.p.delta_bias, d);
-  dl = step_size(a, dl);
+  const float bias = a.p.delta_bias.ptr ? load_param(a.p.delta_bias, d) : 0.0f;
+  const float Dk = a.p.Dskip.ptr ? load_param(a.p.Dskip, d) : 0.0f;
+  dl = step_size(a, dl + bias);
   float y = 0.0f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -926,7 +938,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* stat
     if (j < left) y = fmaf(C[j], h[j], y);
   }
   if (whole) {
-    *reinterpret_cast<Four<float>*>(hp) = Four<float>{{h[0], h[1], h[2], h[3]}};
+    __builtin_nontemporal_store(StateVec{h[0], h[1], h[2], h[3]}, reinterpret_cast<StateVec*>(hp));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -935,21 +947,34 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs a, float* stat
 #pragma unroll
   for (int k = 1; k < LPC; k <<= 1) y += __shfl_xor(y, k);
   if (q) return;
-  if (a.p.Dskip.ptr) y = fmaf(load_param(a.p.Dskip, d), u, y);
+  if (a.p.Dskip.ptr) y = fmaf(Dk, u, y);
   if (a.p.z.ptr) y *= z * sigmoid(z);
   const_cast<IT*>(seq<IT>(a.p.y, b, d))[0] = down<IT>(y);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-template <class IT, class S> int launch(int what, const ScanArgs& a, hipStream_t st) {
+template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
   const long groups = a.blocks * a.chunks * a.p.B;
   if (!grid_fits(groups, 64 * S::NW)) return LQG_ERR_ARG;
-  const dim3 g((unsigned)groups), t(64, S::NW);
+  const dim3 t(64, S::NW);
+  auto grid = [&](long run, long first) {
+    a.run = run, a.first = first;
+    return dim3((unsigned)(a.blocks * run * a.p.B));
+  };
+  // (nothing enters from the last chunk forward, nor from the first backward: their carries are not asked for)
   if (what == 0) {
-    if (a.chunks > 1) hipLaunchKernelGGL((k_scan<IT, S, true>), g, t, 0, st, a);
+    if (a.chunks > 1) {
+      const dim3 g = grid(a.chunks - 1, 0);
+      hipLaunchKernelGGL((k_scan<IT, S, true>), g, t, 0, st, a);
+    }
+    const dim3 g = grid(a.chunks, 0);
     hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
   } else {
-    if (a.chunks > 1) hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
+    if (a.chunks > 1) {
+      const dim3 g = grid(a.chunks - 1, 1);
+      hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
+    }
+    const dim3 g = grid(a.chunks, 0);
     hipLaunchKernelGGL((k_scan_grad<IT, S, false>), g, t, 0, st, a);
   }
   return (int)last();
