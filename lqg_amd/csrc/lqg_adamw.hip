@@ -1,6 +1,7 @@
 // lqg_adamw.hip — one AdamW step over many tensors, moments in float / double or in 8 bits (include/lqg_learn.h).
 //
-// Memory bound: an element of a float tensor moves 28 bytes (p, m, v read and written, g read), 16 with 8-bit moments.  One launch
+// Memory bound: an element of a float tensor moves 28 bytes (p, m, v read and written, g read), 16 with 8-bit moments.  66.7 M elements in
+// 100 tensors: float32 351 us, bfloat16 with 8-bit moments (10 bytes an element) 122 us, 5.3 TB/s both.  One launch
 // walks up to TENSORS tensors: their table travels in the kernel's arguments, so that no table has to be copied to the device and kept
 // alive; a workgroup finds its tensor by bisection in uniform (scalar) registers.  Vectors need no alignment beyond their elements'
 // (the hardware takes global accesses at any address).  This file is compiled with -ffp-contract=off: with 32-bit states every operation
