@@ -662,3 +662,34 @@ def test_capture_beside_a_living_eager_graph_is_refused():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+def selscan_spaces(B, T, D, N, chunks=0):
+    """Bytes of workspace forward and backward, of a call described by its sizes alone."""
+    from lqg_amd import _learn
+    p = _learn.SELSCAN.pack(_learn.T_F32, 1, B, T, D, N, 1, *(6 * _learn.NO_SEQ), *(3 * _learn.NO_PARAM), 0, 0, 0, 0, chunks, 0)
+    lib = _learn.load()
+    return lib.lqg_selscan_workspace(p), lib.lqg_selscan_grad_workspace(p)
+
+
+def test_the_time_axis_is_cut_where_waves_are_few():
+    for B, T, D, N, forward, backward in ((1, 2048, 2048, 16, True, True), (8, 2048, 2048, 16, False, False), (4, 2048, 2048, 16, False, True),
+                                          (1, 64, 2048, 16, False, False), (1, 16384, 1024, 4, True, True), (1, 100000, 32, 64, True, True)):
+        ws, gws = selscan_spaces(B, T, D, N)
+        _, gws1 = selscan_spaces(B, T, D, N, 1)
+        assert (ws > 0) is forward and (gws > gws1) is backward, (B, T, D, N)
+        # a carry for each state and a sum of step sizes for each channel of a piece, 64 at most
+        assert ws % (4 * B * (N + 1) * D) == 0 and ws // (4 * B * (N + 1) * D) in range(0, 65)
+
+
+LONG = [(1, 2100, 40, 16, 1, F32, True, True, True, True, True, None), (2, 1700, 33, 6, 1, BF16, True, True, True, False, True, (1700, 600)),
+        (1, 1500, 64, 3, 2, F32, False, True, False, True, True, (1333,)), (2, 1300, 40, 24, 1, F32, True, True, True, True, True, (200, 1290)),
+        (1, 900, 33, 50, 1, F16, True, True, True, True, True, None)]
+
+
+@gpu
+@pytest.mark.parametrize("case", LONG, ids=str)
+def test_scan_cut_by_the_rule(case):
+    assert min(selscan_spaces(*case[:4])) > 0
+    test_scan_forward_and_state(case, 0)
+    test_scan_gradients(case, 0)
