@@ -249,7 +249,7 @@ def _scan_desc(u, A, G, D, delta_bias, softplus, B, T, seqs, state, last, length
 def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
     """y, the last state, the checkpoints (keep)."""
     nB, T, nD = u.shape
-    N, G, dev = A.shape[1], Bm.shape[2], u.device
+    N, G, dev = A.shape[1], _groups(Bm, 2), u.device
     y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
     last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
     lib = _learn.load()
@@ -283,13 +283,13 @@ class _Scan(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 12
         nB, T, nD = u.shape
-        N, G, dev = A.shape[1], Bm.shape[2], u.device
+        N, G, dev = A.shape[1], _groups(Bm, 2), u.device
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
         dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
         new = lambda *shape: torch.empty(shape, dtype=u.dtype, device=dev)  # noqa: E731
         du, ddelta, dz = new(nB, T, nD), new(nB, T, nD), None if z is None else new(nB, T, nD)
-        dBm, dCm, dA = new(nB, T, G, N), new(nB, T, G, N), torch.empty_like(A)
+        dBm, dCm, dA = new(*Bm.shape), new(*Cm.shape), torch.empty_like(A)
         dD, dbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
@@ -303,6 +303,10 @@ class _Scan(torch.autograd.Function):
         return du, ddelta, dA, dBm, dCm, dD, dz, dbias, dstate, None, None, None
 
 
+def _groups(Bm, lead):
+    return Bm.shape[lead] if Bm.dim() == lead + 2 else 1
+
+
 def _scan_check(u, delta, A, B, C_, D, z, delta_bias, dims):
     u = _sequence(u, "u", dims)
     nD = u.shape[-1]
@@ -314,16 +318,17 @@ def _scan_check(u, delta, A, B, C_, D, z, delta_bias, dims):
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != nD or not 1 <= A.shape[1] <= MAX_STATES:
         raise LqgHipError(f"A: shape ({nD}, 1 .. {MAX_STATES}) is needed, got {_got(A)}")
     A = _parameter(A, "A", A.shape, u)
-    N, lead = A.shape[1], u.shape[:-1]
-    maps = []
+    N, lead, maps, groups = A.shape[1], u.shape[:-1], [], []
     for t, name in ((B, "B"), (C_, "C")):
-        if isinstance(t, torch.Tensor) and t.dim() == dims:
-            t = t.unsqueeze(-2)                    # one group
-        t = _sequence(t, name, dims + 1, u)
-        if t.shape[:-2] != lead or t.shape[-1] != N or t.shape[-2] < 1 or nD % t.shape[-2]:
-            raise LqgHipError(f"{name}: shape {tuple(lead)} + (groups that divide {nD}, {N}) is needed, got {_got(t)}")
+        grouped = isinstance(t, torch.Tensor) and t.dim() == dims + 1
+        t = _sequence(t, name, dims + grouped, u)
+        shape = t.shape
+        G = shape[-2] if grouped else 1
+        if shape[:dims - 1] != lead or shape[-1] != N or G < 1 or nD % G:
+            raise LqgHipError(f"{name}: shape {tuple(lead)} + ({N},) or {tuple(lead)} + (groups that divide {nD}, {N}) is needed, got {_got(t)}")
         maps.append(t)
-    if maps[0].shape != maps[1].shape:
+        groups.append(G)
+    if groups[0] != groups[1]:
         raise LqgHipError("B and C: the same groups are needed")
     return u, delta, A, *maps, _parameter(D, "D", (nD,), u), z, _parameter(delta_bias, "delta_bias", (nD,), u)
 
@@ -368,7 +373,7 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, *, z=None, delta_bias=
     y = torch.empty((nB, nD), dtype=u.dtype, device=u.device)
     if not y.numel():
         return y
-    p = _scan_desc(u, A, Bm.shape[1], D, delta_bias, int(bool(softplus)), nB, 1, [_learn.row(t) for t in (u, delta, z, Bm, Cm, y)],
+    p = _scan_desc(u, A, _groups(Bm, 1), D, delta_bias, int(bool(softplus)), nB, 1, [_learn.row(t) for t in (u, delta, z, Bm, Cm, y)],
                    None, None, None, None)
     with _learn.on_device(u.device):
         _abi.check(_learn.load().lqg_selective_scan_step(p, state.data_ptr(), _learn.stream(u.device)), "lqg_selective_scan_step")
