@@ -239,11 +239,15 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False):
 
 # ------------------------------------------------------------------------------------------------ selective scan
 
-def _scan_desc(u, A, G, D, delta_bias, softplus, B, T, seqs, state, last, lengths, checkpoints, chunks=0):
+def _scan_desc(u, A, G, D, delta_bias, softplus, B, T, seqs, state, last, lengths, checkpoints, cut=(0, 0)):
     u_, delta, z, Bm, Cm, y = seqs
     return _learn.SELSCAN.pack(_learn.TYPES[u.dtype], softplus, B, T, u.shape[-1], A.shape[1], G, *u_, *delta, *z, *Bm, *Cm, *y,
                                *_learn.param(A), *_learn.param(D), *_learn.param(delta_bias), _learn.ptr(state), _learn.ptr(last),
-                               _learn.ptr(lengths), _learn.ptr(checkpoints), chunks, 0)
+                               _learn.ptr(lengths), _learn.ptr(checkpoints), *cut)
+
+
+def _cut():
+    return options.get("SELSCAN_CHUNKS"), options.get("SELSCAN_CHANNELS")
 
 
 def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
@@ -253,8 +257,8 @@ def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplu
     y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
     last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
     lib = _learn.load()
-    seqs, chunks = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], options.get("SELSCAN_CHUNKS")
-    desc = lambda ck: _scan_desc(u, A, G, D, delta_bias, softplus, nB, T, seqs, state, last, lengths, ck, chunks)  # noqa: E731
+    seqs, cut = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], _cut()
+    desc = lambda ck: _scan_desc(u, A, G, D, delta_bias, softplus, nB, T, seqs, state, last, lengths, ck, cut)  # noqa: E731
     p, ck = desc(None), None
     with _learn.on_device(dev):
         if keep:
@@ -294,7 +298,7 @@ class _Scan(torch.autograd.Function):
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
         seqs = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, None)]
-        p = _scan_desc(u, A, G, D, delta_bias, ctx.softplus, nB, T, seqs, None, None, lengths, ck, options.get("SELSCAN_CHUNKS"))
+        p = _scan_desc(u, A, G, D, delta_bias, ctx.softplus, nB, T, seqs, None, None, lengths, ck, _cut())
         g = _learn.SELSCAN_BARS.pack(*_learn.seq(dy), *(_learn.ptr(t) for t in (dlast, du, ddelta, dz, dBm, dCm, dA, dD, dbias, dstate)))
         with _learn.on_device(dev):
             n = lib.lqg_selscan_grad_workspace(p)

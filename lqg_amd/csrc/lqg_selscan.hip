@@ -36,7 +36,7 @@ int check(const lqg_selscan* p) {
   if (!p) return LQG_ERR_NULL;
   if (p->type != LQG_T_F32 && p->type != LQG_T_BF16 && p->type != LQG_T_F16) return LQG_ERR_ARG;
   if (p->B < 1 || p->T < 1 || p->D < 1 || p->D > MAX_STRIDE || p->N < 1 || p->N > 64 || p->G < 1 || p->D % p->G) return LQG_ERR_ARG;
-  if (p->chunks < 0 || p->chunks > 64) return LQG_ERR_ARG;
+  if (p->chunks < 0 || p->chunks > 64 || (p->channels != 0 && p->channels != 16 && p->channels != 32)) return LQG_ERR_ARG;
   for (const lqg_seq* q : {&p->u, &p->delta, &p->z, &p->Bm, &p->Cm, &p->y})
     if (q->st < 0 || q->st > MAX_STRIDE) return LQG_ERR_ARG;
   for (const lqg_param* q : {&p->A, &p->Dskip, &p->delta_bias})
@@ -48,34 +48,59 @@ int check(const lqg_selscan* p) {
 long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
 int tile_of(long N) { return N > 32 ? 8 : 16; }
 
-// Time of a pass of w waves over the whole axis, in units of one that half fills the 1024 SIMDs: as many rounds as fill them, and a tenth
-// more when every SIMD is taken.  Forward with 5 to 8 states workgroups of two waves share SIMDs early, and backward with 9 to 16 states
-// registers let two waves share one, so that one alone, which waits by itself, leaves time unused (in both 1.3).
-double pass_time(long N, bool grad, long w) {
+// How a scan is laid over the card: channels of a workgroup, and pieces that the time axis is cut into.
+//
+// Time of a pass of w waves over the whole axis, in units of a pass that half fills the 1024 SIMDs: forward two waves of a SIMD overlap, and
+// beyond that time grows with their number; backward a SIMD takes one wave at a time (with 9 to 16 states two, so that one alone, which waits
+// by itself, leaves time unused).
+double pass_time(long N, bool grad, bool narrow, long w) {
   const double q = w / 1024.0;
-  const bool shared = grad ? N > 8 && N <= 16 : N > 4 && N <= 8;
   if (q <= 0.5) return 1.0;
-  if (q <= 1.0) return shared ? 1.3 : 1.1;
-  if (shared && !grad) return q <= 2.0 ? 1.6 : 0.96 * q;
-  return std::ceil(q);
+  if (grad) return q > 1.0 ? std::ceil(q) : N > 8 && N <= 16 ? 1.3 : 1.0;
+  if (narrow) return q <= 1.0 ? (N > 4 ? 1.0 : 1.2) : q <= 2.0 ? (N > 4 ? 1.3 : 1.6) : (N > 4 ? 0.6 : 1.0) * q;
+  return q <= 1.0 ? 1.1 : q <= 2.0 ? 1.35 : 0.68 * q;
 }
 
-// Pieces of the time axis.  A cut into c adds the pass that leaves the carries of c - 1 of them (0.55 of the main pass's time forward, 0.2
-// backward), 3 tiles a piece before its loads are under way, and a launch (6 tiles): the c with the least sum.  Measured, bfloat16 with
-// gate, us uncut / in 2 / 4 / 8 at 2048 steps:  forward N = 16: 126 / 115 / 88 / 88 (512 waves uncut), 128 / 138 / 135 / 143 (1024);
-// N = 8: 149 / 151 / 98 / 107 (512), 192 / 179 / 170 / 198 (1024).  Backward N = 16: 366 / 258 / 188 / 198 (512), 379 / 325 / 333 / 367
-// (1024), 516 / 598 / 630 / 700 (2048); N = 24: 572 / 393 / 392 / 439 (512), 592 / 689 / 734 / 841 (1024), 1144 / 1026 / 934 / 979 (1100).
-// Over 164 such rows (N = 4 .. 64, 512 to 6000 steps, 64 to 2048 waves) the choice is 1.3 % slower than the best cut (geometric mean, 25 %
-// at most); filling the SIMDs up to a threshold of waves was 6.8 % (54 %).
-long pieces(long N, bool grad, long waves, long tiles) {
-  long best = 1;
-  double least = pass_time(N, grad, waves);
-  for (long c = 2; c <= std::min(64L, tiles / 8); ++c) {
-    const double t = (pass_time(N, grad, waves * c) + (grad ? 0.2 : 0.55) * pass_time(N, grad, waves * (c - 1))) * (1.0 / c + 3.0 / tiles) +
-                     6.0 / tiles;
-    if (t < least) least = t, best = c;
+// A cut into c pieces adds the pass that leaves the carries of c - 1 of them (0.55 to 0.6 of the main pass's time forward, 0.2 backward), 3 tiles
+// a piece before its loads are under way, a launch (8 tiles) and the reading of the carries: the c with the least sum; forward a power of two,
+// which leaves whole rounds of workgroups.  Measured, bfloat16 with gate, us at 2048 steps uncut / in 2 / 4 / 8:  forward, 16 channels, N = 16:
+// 90 / 82 / 48 / 41 (256 waves uncut), 91 / 103 / 91 / 93 (1024); N = 4: 110 / 100 / 61 / 50 (256), 121 / 126 / 143 / 146 (1024).  Backward
+// N = 16: 366 / 258 / 188 / 198 (512), 379 / 325 / 333 / 367 (1024), 516 / 598 / 630 / 700 (2048); N = 24: 572 / 393 / 392 / 439 (512), 592 /
+// 689 / 734 / 841 (1024), 1144 / 1026 / 934 / 979 (1100).
+struct Cut { double time; long pieces; };
+Cut cut(long N, bool grad, bool narrow, long waves, long tiles) {
+  Cut best{pass_time(N, grad, narrow, waves), 1};
+  const double carry = grad ? 0.2 : narrow ? 0.55 : 0.6;
+  for (long c = 2; c <= std::min(64L, tiles / 8); c += grad ? 1 : c) {
+    const double main = pass_time(N, grad, narrow, waves * c), before = pass_time(N, grad, narrow, waves * (c - 1));
+    const double t = (main + carry * before) * (1.0 / c + 3.0 / tiles) + (8.0 + 0.35 * c) / tiles;
+    if (t < best.time) best = {t, c};
   }
   return best;
+}
+
+// Forward and up to 32 states a workgroup may have 16 channels instead of 32: twice the waves, each with half the states, in 0.58 to 0.72 of
+// the time while they fill the card.  Measured, us with 32 / 16 channels, uncut, 2048 steps x 2048 channels (trials):  N = 4: 179 / 121 (4),
+// 192 / 121 (8), 198 / 210 (16), 440 / 386 (32); N = 8: 148 / 119 (4), 190 / 133 (8), 209 / 275 (16); N = 16: 126 / 91 (2), 128 / 126 (4), 177 /
+// 204 (8); N = 32: 181 / 119 (2), 186 / 163 (4), 274 / 275 (8).  Over 132 sizes (N = 3 .. 32, 512 to 16384 steps, 32 channels to 32 trials of
+// 2048) width and cut chosen so are 2.3 % slower than the best pair in the geometric mean, 24 % at most.
+void lay_out(ScanArgs& a, bool grad) {
+  const long N = a.p.N, waves = N > 8 ? 4 : N > 4 ? 2 : 1;
+  Cut best{};
+  auto with = [&](int channels) {
+    const long bpg = (a.Dg + channels - 1) / channels;
+    const Cut c = cut(N, grad, channels == 16, bpg * a.p.G * a.p.B * waves, a.tiles);
+    const double time = c.time * (channels == 32 ? 1.0 : N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58);
+    if (best.pieces && time >= best.time) return;
+    best = {time, c.pieces};
+    a.narrow = channels == 16;
+    a.bpg = bpg;
+  };
+  const int asked = grad || N > 32 ? 32 : a.p.channels ? a.p.channels : N <= 4 ? 16 : 0;
+  if (asked != 16) with(32);
+  if (asked != 32) with(16);
+  a.blocks = a.bpg * a.p.G;
+  a.chunks = a.p.chunks ? std::min((long)a.p.chunks, a.tiles) : best.pieces;
 }
 
 ScanArgs describe(const lqg_selscan* p, bool grad) {
@@ -83,11 +108,8 @@ ScanArgs describe(const lqg_selscan* p, bool grad) {
   a.p = *p;
   const long TT = tile_of(p->N);
   a.Dg = p->D / p->G;
-  a.bpg = (a.Dg + CHANNELS - 1) / CHANNELS;
-  a.blocks = a.bpg * p->G;
   a.tiles = (p->T + TT - 1) / TT;
-  const long waves = a.blocks * p->B * (p->N > 8 ? 4 : p->N > 4 ? 2 : 1);
-  a.chunks = p->chunks ? std::min((long)p->chunks, a.tiles) : pieces(p->N, grad, waves, a.tiles);
+  lay_out(a, grad);
   const long per = (a.tiles + a.chunks - 1) / a.chunks;
   a.chunk = per * TT;
   a.chunks = (a.tiles + per - 1) / per;               // no empty chunk

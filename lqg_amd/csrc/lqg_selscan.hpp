@@ -5,9 +5,9 @@
 // B x D x N scalar recurrences; per step of one of them one exponential and four float operations, and B_t, C_t are shared by all
 // channels of a group: bound by the vector units (and their exponential) from N = 8 or so on, by memory below.  Mapping: a workgroup is 32
 // channels with all their states; a wave is those 32 channels twice, each half with NS of the N states in registers, so NW waves hold
-// 2 NS NW states.  The time axis is walked in tiles of TT steps: the threads prepare the tile's TT x 32 elements (softplus, dl u, silu)
-// once for all states through LDS, every wave runs the TT steps on its states and leaves its part of sum_n C h in LDS, and the threads
-// finish the elements they prepared.  B_t and C_t of a tile sit one value per lane in rows of 16 and reach the arithmetic as DPP row
+// 2 NS NW states (or 16 channels four times, where waves would be few).  The time axis is walked in tiles of TT steps: the threads prepare
+// the tile's elements (softplus, dl u, silu) once for all states through LDS, every wave runs the TT steps on its states and leaves its part
+// of sum_n C h in LDS, and the threads finish the elements they prepared.  B_t and C_t of a tile sit one value per lane in rows of 16 and reach the arithmetic as DPP row
 // broadcasts: an operand modifier, no load and no instruction.  Whole tiles (all but the last) run without bounds checks, their loads two
 // tiles ahead.  Few channels: the time axis is cut into chunks; one pass leaves each chunk's end state from zero and its sum of dl, the
 // second enters with exp(A sum dl) h + end state over the chunks before it.
@@ -18,14 +18,14 @@ namespace lqg {
 namespace learn {
 
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int CHANNELS = 32;     // of a workgroup
 
 struct ScanArgs {
   lqg_selscan p;
   lqg_selscan_bars g;
-  long Dg, bpg, blocks;          // channels of a group, blocks of CHANNELS of them, blocks in all
+  long Dg, bpg, blocks;          // channels of a group, blocks of a workgroup's of them, blocks in all
   long chunks, chunk, tiles;     // chunks of the time axis, their steps (a multiple of TT), tiles of TT steps in T
   long run, first;               // chunks of this launch, the first of them
+  bool narrow;                   // 16 channels a workgroup, else 32
   float *hl, *sd;                // carries [B][chunks][N][D], sums of dl [B][chunks][D]
   float *partBC, *partP;         // gradients: [blocks][B][T][2][N], [B * chunks][N + 2][D]
 };
@@ -35,8 +35,8 @@ template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, lo
 }
 
 // The shape of a workgroup: CH channels x NS NW 64 / CH states, TT steps a tile.
-template <int NS_, int NW_, int TT_> struct Shape {
-  static constexpr int CH = CHANNELS, NS = NS_, NW = NW_, TT = TT_;
+template <int NS_, int NW_, int TT_, int CH_ = 32> struct Shape {
+  static constexpr int CH = CH_, NS = NS_, NW = NW_, TT = TT_;
   static constexpr int GRAD_WAVES = NS == 2 && NW > 2 ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
   static constexpr int LS = 64 / CH;          // groups of NS states in a wave
   static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
@@ -182,12 +182,14 @@ template <class S, int T, int J> __device__ inline float bc(const float (&r)[S::
 // products only (it would copy first: one more instruction for each of N).  Two wait states keep a write of C before the block apart
 // from the broadcasts' reads; several steps in a block share them.  SWAP: y goes into a swap of lanes, which must not read it in the
 // two wait states after its write; the compiler keeps its own instructions apart, and does not see these.
-template <class S> struct Group { static constexpr int GS = S::NS == 2 ? 4 : S::NS == 4 ? 2 : 1; };
+template <class S> struct Group { static constexpr int GS = S::NS <= 2 ? 4 : S::NS == 4 ? 2 : 1; };
 #define LQG_FMAC_BCAST(Y, C, K, X) "v_fmac_f32_dpp " Y ", " C ", " X " row_newbcast:" K " row_mask:0xf bank_mask:0xf\n\t"
 template <class S, int T, bool SWAP> __device__ __forceinline__ void dot_bcast(const float (&C)[S::Q], const float (&h)[Group<S>::GS][S::NS], float (&y)[Group<S>::GS]) {
   constexpr int f = T * S::NS, k = f % 16;
   const float c = C[f / 16];
-  if constexpr (S::NS == 2) {
+  if constexpr (S::NS == 1) {
+    y[0] = row_bcast<k>(c) * h[0][0], y[1] = row_bcast<k + 1>(c) * h[1][0], y[2] = row_bcast<k + 2>(c) * h[2][0], y[3] = row_bcast<k + 3>(c) * h[3][0];
+  } else if constexpr (S::NS == 2) {
     y[0] = row_bcast<k>(c) * h[0][0], y[1] = row_bcast<k + 2>(c) * h[1][0], y[2] = row_bcast<k + 4>(c) * h[2][0], y[3] = row_bcast<k + 6>(c) * h[3][0];
     asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%4", "%c9", "%5") LQG_FMAC_BCAST("%1", "%4", "%c10", "%6")
         LQG_FMAC_BCAST("%2", "%4", "%c11", "%7") LQG_FMAC_BCAST("%3", "%4", "%c12", "%8")
@@ -973,7 +975,7 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
     }
     const dim3 g = grid(a.chunks, 0);
     hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
-  } else {
+  } else if constexpr (S::CH == 32) {                     // (backward has no other)
     if (a.chunks > 1) {
       const dim3 g = grid(a.chunks - 1, 1);
       hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
@@ -986,6 +988,12 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
 
 template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
   const long N = a.p.N;
+  if (a.narrow) {
+    if (N > 16) return launch<IT, Shape<2, 4, 16, 16>>(what, a, st);
+    if (N > 8) return launch<IT, Shape<1, 4, 16, 16>>(what, a, st);
+    if (N > 4) return launch<IT, Shape<1, 2, 16, 16>>(what, a, st);
+    return launch<IT, Shape<1, 1, 16, 16>>(what, a, st);
+  }
   if (N > 32) return launch<IT, Shape<8, 4, 8>>(what, a, st);
   if (N > 16) return launch<IT, Shape<4, 4, 16>>(what, a, st);
   if (N > 8) return launch<IT, Shape<2, 4, 16>>(what, a, st);

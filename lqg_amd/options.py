@@ -44,6 +44,7 @@ GRAPH             1         0: inference loops launch eagerly instead of replayi
 GRAPH_AFFINE      1         0: captured constructors are not collapsed into their measured affine map
 SETUP_KERNEL      1         0: PointMassBoundedActor is discretised by torch.linalg instead of lqg_point_mass_setup
 SELSCAN_CHUNKS    0         pieces (at most 64) the selective scan's time axis is cut into (0: the rule of lqg_selscan.hip)  -> lqg_selscan.chunks
+SELSCAN_CHANNELS  0         channels of a workgroup of the selective scan, forward with up to 32 states: 16 or 32 (0: the rule)  -> lqg_selscan.channels
 JIT               1         0: never compile an auxiliary lane-kernel library for an unlisted shape on demand
 
 Build / location variables (read once where the files are located, not behaviour switches): LQG_HIP_LIB, LQG_PAT_DIR,
@@ -57,7 +58,7 @@ DEFAULTS = {
     "COOP": "", "COOP_SPARSE": 1, "COOP_TRIAL_ROWS": 1, "COOP_TRIAL_TPB": 0, "COOP_TRIAL_WIDE": "", "COOP_TRIAL_CHUNKS": "", "COOP_ADJOINT": 0, "ADJOINT_SP": 1, "TRIAL_CHUNKS": "", "TRIAL_LDS": "", "TRIAL_CHUNK_WAVES": 0,
     "TRIAL_CHUNK_MAX_WAVES": 0, "TRIAL_CHUNK_TPL": 0, "FUSE_TRIALS_MAX": 2048, "MIXED": 1, "MIXED_MIN_TRIALS": 3, "HILO": 1,
     "F32_WIDE": 1, "F32_MAX_COND": 1e7, "X4_LAYOUT": 0, "TV_JIT_MIN_WORK": 1 << 20, "NO_SPECIALIZE": 0, "NO_DECOUPLE": 0, "NO_MERGE": 0, "GRAPH": 1, "GRAPH_AFFINE": 1,
-    "SETUP_KERNEL": 1, "JIT": 1, "SELSCAN_CHUNKS": 0,
+    "SETUP_KERNEL": 1, "JIT": 1, "SELSCAN_CHUNKS": 0, "SELSCAN_CHANNELS": 0,
 }
 _overrides = {}
 

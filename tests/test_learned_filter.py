@@ -693,3 +693,14 @@ def test_scan_cut_by_the_rule(case):
     assert min(selscan_spaces(*case[:4])) > 0
     test_scan_forward_and_state(case, 0)
     test_scan_gradients(case, 0)
+
+
+@gpu
+@pytest.mark.parametrize("channels", (16, 32))
+@pytest.mark.parametrize("case", SCAN + LONG, ids=str)
+def test_scan_workgroups_of_either_width(case, channels):
+    """Both widths of a workgroup, uncut and cut, whichever the rule would take."""
+    with options.override(SELSCAN_CHANNELS=channels):
+        for chunks in (1, 3):
+            test_scan_forward_and_state(case, chunks)
+        test_scan_gradients(case, 0)
