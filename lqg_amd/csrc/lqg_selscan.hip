@@ -48,55 +48,57 @@ int check(const lqg_selscan* p) {
 long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
 int tile_of(long N) { return N > 32 ? 8 : 16; }
 
-// How a scan is laid over the card: channels of a workgroup, and pieces that the time axis is cut into.
+// How a scan is laid over the card: channels of a workgroup (16 or, with half the waves, 32), and pieces that the time axis is cut into.
 //
-// Time of a pass of w waves over the whole axis, in units of a pass that half fills the 1024 SIMDs: forward two waves of a SIMD overlap, and
-// beyond that time grows with their number; backward a SIMD takes one wave at a time (with 9 to 16 states two, so that one alone, which waits
-// by itself, leaves time unused).
-double pass_time(long N, bool grad, bool narrow, long w) {
+// Time of a pass of w waves over the whole axis, in units of a pass that half fills the 1024 SIMDs: `one` while no SIMD has two waves, `two`
+// while none has three, then growing with the waves (more 0: by whole rounds, of one wave a SIMD, which is all that registers allow).
+struct Passes { double one, two, more, unit; };   // unit: time of such a pass over that of one with 32 channels
+Passes passes(long N, bool grad, bool narrow) {
+  if (!grad) return !narrow ? Passes{1.1, 1.35, 0.68, 1.0} : N <= 4 ? Passes{1.2, 1.6, 1.0, 0.6} : Passes{1.0, 1.3, 0.6, N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58};
+  if (!narrow) return N > 8 && N <= 16 ? Passes{1.05, 1.4, 0.66, 1.0} : Passes{1.05, 2.0, 0.0, 1.0};
+  return N <= 4 ? Passes{1.05, 1.87, 1.0, 0.66} : N <= 8 ? Passes{1.15, 1.33, 0.73, 0.7} : Passes{1.0, 1.3, 0.63, N <= 16 ? 0.71 : 0.64};
+}
+double pass_time(const Passes& p, long w) {
   const double q = w / 1024.0;
-  if (q <= 0.5) return 1.0;
-  if (grad) return q > 1.0 ? std::ceil(q) : N > 8 && N <= 16 ? 1.3 : 1.0;
-  if (narrow) return q <= 1.0 ? (N > 4 ? 1.0 : 1.2) : q <= 2.0 ? (N > 4 ? 1.3 : 1.6) : (N > 4 ? 0.6 : 1.0) * q;
-  return q <= 1.0 ? 1.1 : q <= 2.0 ? 1.35 : 0.68 * q;
+  return q <= 0.5 ? 1.0 : q <= 1.0 ? p.one : q <= 2.0 ? p.two : p.more > 0.0 ? p.more * q : std::ceil(q);
 }
 
-// A cut into c pieces adds the pass that leaves the carries of c - 1 of them (0.55 to 0.6 of the main pass's time forward, 0.2 backward), 3 tiles
-// a piece before its loads are under way, a launch (8 tiles) and the reading of the carries: the c with the least sum; forward a power of two,
-// which leaves whole rounds of workgroups.  Measured, bfloat16 with gate, us at 2048 steps uncut / in 2 / 4 / 8:  forward, 16 channels, N = 16:
-// 90 / 82 / 48 / 41 (256 waves uncut), 91 / 103 / 91 / 93 (1024); N = 4: 110 / 100 / 61 / 50 (256), 121 / 126 / 143 / 146 (1024).  Backward
-// N = 16: 366 / 258 / 188 / 198 (512), 379 / 325 / 333 / 367 (1024), 516 / 598 / 630 / 700 (2048); N = 24: 572 / 393 / 392 / 439 (512), 592 /
-// 689 / 734 / 841 (1024), 1144 / 1026 / 934 / 979 (1100).
+// A cut into c pieces adds the pass that leaves the carries of c - 1 of them (0.55 to 0.6 of the main pass's time forward, 0.15 to 0.2 backward),
+// 3 tiles a piece before its loads are under way, a launch (8 tiles) and the reading of the carries: the c with the least sum, a power of
+// two, which leaves whole rounds of workgroups.  Measured, bfloat16 with gate, us at 2048 steps uncut / in 2 / 4 / 8:  forward, 16 channels, N =
+// 16: 90 / 82 / 48 / 41 (256 waves uncut), 91 / 103 / 91 / 93 (1024); N = 4: 110 / 100 / 61 / 50 (256), 121 / 126 / 143 / 146 (1024).  Backward, 32
+// channels, N = 16: 380 / 279 / 207 / 212 (512), 395 / 338 / 351 / 379 (1024), 531 / 610 / 640 / 709 (2048).
 struct Cut { double time; long pieces; };
-Cut cut(long N, bool grad, bool narrow, long waves, long tiles) {
-  Cut best{pass_time(N, grad, narrow, waves), 1};
-  const double carry = grad ? 0.2 : narrow ? 0.55 : 0.6;
-  for (long c = 2; c <= std::min(64L, tiles / 8); c += grad ? 1 : c) {
-    const double main = pass_time(N, grad, narrow, waves * c), before = pass_time(N, grad, narrow, waves * (c - 1));
-    const double t = (main + carry * before) * (1.0 / c + 3.0 / tiles) + (8.0 + 0.35 * c) / tiles;
+Cut cut(const Passes& p, double carry, long waves, long tiles) {
+  Cut best{pass_time(p, waves), 1};
+  for (long c = 2; c <= std::min(64L, tiles / 8); c *= 2) {
+    const double t = (pass_time(p, waves * c) + carry * pass_time(p, waves * (c - 1))) * (1.0 / c + 3.0 / tiles) + (8.0 + 0.35 * c) / tiles;
     if (t < best.time) best = {t, c};
   }
   return best;
 }
 
-// Forward and up to 32 states a workgroup may have 16 channels instead of 32: twice the waves, each with half the states, in 0.58 to 0.72 of
-// the time while they fill the card.  Measured, us with 32 / 16 channels, uncut, 2048 steps x 2048 channels (trials):  N = 4: 179 / 121 (4),
-// 192 / 121 (8), 198 / 210 (16), 440 / 386 (32); N = 8: 148 / 119 (4), 190 / 133 (8), 209 / 275 (16); N = 16: 126 / 91 (2), 128 / 126 (4), 177 /
-// 204 (8); N = 32: 181 / 119 (2), 186 / 163 (4), 274 / 275 (8).  Over 132 sizes (N = 3 .. 32, 512 to 16384 steps, 32 channels to 32 trials of
-// 2048) width and cut chosen so are 2.3 % slower than the best pair in the geometric mean, 24 % at most.
+// 16 channels: up to 32 states (forward always with up to 4, whose waves of 32 channels are few and long).  Measured, us with 32 / 16 channels,
+// uncut, 2048 steps x 2048 channels (trials):  forward N = 4: 179 / 121 (4), 192 / 121 (8), 198 / 210 (16), 440 / 386 (32); N = 8: 148 / 119 (4),
+// 190 / 133 (8), 209 / 275 (16); N = 16: 126 / 91 (2), 128 / 126 (4), 177 / 204 (8); N = 32: 181 / 119 (2), 186 / 163 (4), 274 / 275 (8).  Backward
+// N = 3: 512 / 359 (4), 541 / 362 (8), 551 / 634 (16); N = 6: 426 / 354 (4), 441 / 388 (8), 855 / 872 (16); N = 16: 380 / 274 (2), 395 / 351 (4),
+// 531 / 683 (8); N = 24: 599 / 499 (4), 1168 / 969 (8).  Over 132 sizes forward and 112 backward (N = 3 .. 32, 512 to 16384 steps, 256 channels
+// to 32 trials of 2048) width and cut chosen so are 2.3 % and 2.8 % slower than the best pair in the geometric mean, 24 % at most.
 void lay_out(ScanArgs& a, bool grad) {
   const long N = a.p.N, waves = N > 8 ? 4 : N > 4 ? 2 : 1;
   Cut best{};
   auto with = [&](int channels) {
+    const bool narrow = channels == 16;
+    const Passes p = passes(N, grad, narrow);
     const long bpg = (a.Dg + channels - 1) / channels;
-    const Cut c = cut(N, grad, channels == 16, bpg * a.p.G * a.p.B * waves, a.tiles);
-    const double time = c.time * (channels == 32 ? 1.0 : N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58);
-    if (best.pieces && time >= best.time) return;
-    best = {time, c.pieces};
-    a.narrow = channels == 16;
+    Cut c = cut(p, grad ? (narrow ? 0.15 : 0.2) : narrow ? 0.55 : 0.6, bpg * a.p.G * a.p.B * waves, a.tiles);
+    c.time *= p.unit;
+    if (best.pieces && c.time >= best.time) return;
+    best = c;
+    a.narrow = narrow;
     a.bpg = bpg;
   };
-  const int asked = grad || N > 32 ? 32 : a.p.channels ? a.p.channels : N <= 4 ? 16 : 0;
+  const int asked = N > 32 ? 32 : a.p.channels ? a.p.channels : !grad && N <= 4 ? 16 : 0;
   if (asked != 16) with(32);
   if (asked != 32) with(16);
   a.blocks = a.bpg * a.p.G;

@@ -37,7 +37,7 @@ template <class IT> __device__ inline const IT* seq(const lqg_seq& s, long b, lo
 // The shape of a workgroup: CH channels x NS NW 64 / CH states, TT steps a tile.
 template <int NS_, int NW_, int TT_, int CH_ = 32> struct Shape {
   static constexpr int CH = CH_, NS = NS_, NW = NW_, TT = TT_;
-  static constexpr int GRAD_WAVES = NS == 2 && NW > 2 ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
+  static constexpr int GRAD_WAVES = NS == 1 || (NS == 2 && NW > 2) ? 2 : 1;   // waves of the gradient kernel that a SIMD's registers are shared by
   static constexpr int LS = 64 / CH;          // groups of NS states in a wave
   static constexpr int PS = NW * LS;          // groups of NS states in all = partial sums over the states
   static constexpr int NP = NS * PS;          // states it has room for
@@ -215,14 +215,16 @@ template <class S, int T, bool SWAP> __device__ __forceinline__ void dot_bcast(c
   if constexpr (SWAP) {
     if constexpr (S::NS == 2) asm("s_nop 1" : "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3]));
     else if constexpr (S::NS == 4) asm("s_nop 1" : "+v"(y[0]), "+v"(y[1]));
-    else asm("s_nop 1" : "+v"(y[0]));
+    else if constexpr (S::NS == 8) asm("s_nop 1" : "+v"(y[0]));
   }
 }
 // x[j] += bc(C)(T, j) f
 template <class S, int T> __device__ __forceinline__ void add_bcast(float (&x)[S::NS], const float (&C)[S::Q], float f) {
   constexpr int at = T * S::NS, k = at % 16;
   const float c = C[at / 16];
-  if constexpr (S::NS == 2) {
+  if constexpr (S::NS == 1) {
+    asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%1", "%c3", "%2") : "+v"(x[0]) : "v"(c), "v"(f), "n"(k));
+  } else if constexpr (S::NS == 2) {
     asm("s_nop 1\n\t" LQG_FMAC_BCAST("%0", "%2", "%c4", "%3") LQG_FMAC_BCAST("%1", "%2", "%c5", "%3")
         : "+v"(x[0]), "+v"(x[1]) : "v"(c), "v"(f), "n"(k), "n"(k + 1));
   } else {
@@ -473,9 +475,20 @@ template <int BIT, int M> __device__ __forceinline__ void merge_all(float* x, co
 #pragma unroll
     for (int k = 0; k < M; ++k) x[k] = merge<BIT>(x[k], y[k], lane);
   } else {
-    static_assert(M % 4 == 0, "");
+    static_assert(M == 2 || M % 4 == 0, "");
+    if constexpr (M == 2) {
+      float o0, o1;
+      if constexpr (BIT == 3)
+        asm("s_nop 1\n\t" LQG_MERGE("%0", "%2", "%4", "row_ror:8", "0xc") LQG_MERGE("%1", "%3", "%5", "row_ror:8", "0xc")
+            : "=&v"(o0), "=&v"(o1) : "v"(x[0]), "v"(x[1]), "v"(y[0]), "v"(y[1]));
+      else
+        asm("s_nop 1\n\t" LQG_MERGE("%0", "%2", "%4", "row_half_mirror", "0xa") LQG_MERGE("%1", "%3", "%5", "row_half_mirror", "0xa")
+            : "=&v"(o0), "=&v"(o1) : "v"(x[0]), "v"(x[1]), "v"(y[0]), "v"(y[1]));
+      x[0] = o0, x[1] = o1;
+      return;
+    }
 #pragma unroll
-    for (int k = 0; k < M; k += 4) {
+    for (int k = 0; k + 4 <= M; k += 4) {
       float o0, o1, o2, o3;
       if constexpr (BIT == 3)
         asm("s_nop 1\n\t" LQG_MERGE("%0", "%4", "%8", "row_ror:8", "0xc") LQG_MERGE("%1", "%5", "%9", "row_ror:8", "0xc")
@@ -542,7 +555,7 @@ template <class S> struct ChannelSum {
 
 // CARRY: leave each chunk's carry (lambda at its start from 0 at its end) and its sum of dl.
 // Iteration i (downwards): finish tile i+1, prepare tile i-1, request tile i-3's rows and tile i-2's maps, walk tile i up and down; one
-// barrier.  The halves of a wave add their sums before they go to LDS, each for every other step.
+// barrier.  The halves of a wave (16 channels: its rows) add their sums before they go to LDS, each for every second (fourth) step.
 template <class IT, class S, bool CARRY>
 __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const ScanArgs a) {
   constexpr int CH = S::CH, NS = S::NS, NW = S::NW, TT = S::TT, PS = S::PS, R = S::R, Q = S::Q;
@@ -554,7 +567,9 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
   const Place<S> at(a);
   const long D = a.p.D, N = a.p.N, T = a.p.T, b = at.b;
   const unsigned d = at.d;
-  const int ch = at.ch, w = at.row / S::LS, half = at.row % S::LS;
+  const int ch = at.ch, w = at.row / S::LS;
+  // which of the steps that the lane groups' sums are merged for (2 halves, or 4 rows) a lane ends with
+  const int mine = S::LS == 2 ? at.lane >> 5 : (at.lane >> 5) + 2 * (at.lane >> 4 & 1);
   float A2[NS], lam[NS], dA[NS], sum = 0.0f, dDk = 0.0f, dbias = 0.0f;
   load_A2<S>(a, at, A2);
 #pragma unroll
@@ -742,16 +757,20 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
         });
       });
       constexpr int GS = Group<S>::GS;
-      // steps come singly (GS = 1) or in even groups; the halves' sums of a pair of steps: the lower half takes the even step
+      // steps come singly (GS = 1) or in even groups; the halves' sums of a pair of steps, or the rows' of four
+      auto merged = [&](const float* v) __attribute__((always_inline)) {
+        if constexpr (S::LS == 2) return merge<5>(v[0], v[1], at.lane);
+        else return merge<4>(merge<5>(v[0], v[1], at.lane), merge<5>(v[2], v[3], at.lane), at.lane);
+      };
       float ky = 0.0f, k1 = 0.0f, k2 = 0.0f;
       auto put_y = [&](auto tc, const float (&v)[GS]) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::v;
         if constexpr (GS == 1) {
-          if constexpr (t & 1) s_y[P][t - 1 + half][w][ch] = merge<5>(ky, v[0], at.lane);
+          if constexpr (t & 1) s_y[P][t - 1 + mine][w][ch] = merge<5>(ky, v[0], at.lane);
           else ky = v[0];
         } else {
 #pragma unroll
-          for (int k = 0; k < GS; k += 2) s_y[P][t + k + half][w][ch] = merge<5>(v[k], v[k + 1], at.lane);
+          for (int k = 0; k < GS; k += S::LS) s_y[P][t + k + mine][w][ch] = merged(v + k);
         }
       };
       if (gate)
@@ -788,11 +807,10 @@ __global__ __launch_bounds__(64 * S::NW, S::GRAD_WAVES) void k_scan_grad(const S
           dot_bcast<S, t, true>(B, gg, s1);
           if constexpr (GS == 1) {
             if constexpr (t & 1) k1 = s1[0], k2 = s2[0];
-            else s_sum[P][t + half][w][ch] = make_float2(merge<5>(s1[0], k1, at.lane), merge<5>(s2[0], k2, at.lane));
+            else s_sum[P][t + mine][w][ch] = make_float2(merge<5>(s1[0], k1, at.lane), merge<5>(s2[0], k2, at.lane));
           } else {
 #pragma unroll
-            for (int o = 0; o < GS; o += 2)
-              s_sum[P][t + o + half][w][ch] = make_float2(merge<5>(s1[o], s1[o + 1], at.lane), merge<5>(s2[o], s2[o + 1], at.lane));
+            for (int o = 0; o < GS; o += S::LS) s_sum[P][t + o + mine][w][ch] = make_float2(merged(s1 + o), merged(s2 + o));
           }
         }
         using CS = ChannelSum<S>;
@@ -975,7 +993,7 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
     }
     const dim3 g = grid(a.chunks, 0);
     hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
-  } else if constexpr (S::CH == 32) {                     // (backward has no other)
+  } else {
     if (a.chunks > 1) {
       const dim3 g = grid(a.chunks - 1, 1);
       hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);

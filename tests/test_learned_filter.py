@@ -704,3 +704,12 @@ def test_scan_workgroups_of_either_width(case, channels):
         for chunks in (1, 3):
             test_scan_forward_and_state(case, chunks)
         test_scan_gradients(case, 0)
+
+
+@gpu
+@pytest.mark.parametrize("channels", (16, 32))
+@pytest.mark.parametrize("case", SCAN + LONG, ids=str)
+def test_gradients_of_workgroups_of_either_width(case, channels):
+    with options.override(SELSCAN_CHANNELS=channels):
+        for chunks in (1, 3):
+            test_scan_gradients(case, chunks)
