@@ -250,32 +250,33 @@ def _cut():
     return options.get("SELSCAN_CHUNKS"), options.get("SELSCAN_CHANNELS")
 
 
-def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, keep):
-    """y, the last state, the checkpoints (keep)."""
+def _checkpoint_bytes(B, T, D, N):
+    """lqg_selscan_checkpoint_bytes: the states at the start of every 16 steps (8 for N > 32), rows of N rounded up to a power of two."""
+    return 4 * B * -(-T // (8 if N > 32 else 16)) * max(4, 1 << (N - 1).bit_length()) * D
+
+
+def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, cut, ck=None):
     nB, T, nD = u.shape
-    N, G, dev = A.shape[1], _groups(Bm, 2), u.device
+    N, dev = A.shape[1], u.device
     y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
     last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
     lib = _learn.load()
-    seqs, cut = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], _cut()
-    desc = lambda ck: _scan_desc(u, A, G, D, delta_bias, softplus, nB, T, seqs, state, last, lengths, ck, cut)  # noqa: E731
-    p, ck = desc(None), None
+    p = _scan_desc(u, A, _groups(Bm, 2), D, delta_bias, softplus, nB, T, [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], state, last,
+                   lengths, ck, cut)
     with _learn.on_device(dev):
-        if keep:
-            ck = _learn.scratch(lib.lqg_selscan_checkpoint_bytes(p), dev)
-            p = desc(ck)
         n = lib.lqg_selscan_workspace(p)
         ws = _learn.scratch(n, dev)
         _abi.check(lib.lqg_selective_scan(p, _learn.ptr(ws), n, _learn.stream(dev)), "lqg_selective_scan")
-    return y, last, ck
+    return y, last
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state):
-        y, last, ck = _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, True)
+        ctx.softplus, ctx.cut = softplus, _cut()
+        ck = _learn.scratch(_checkpoint_bytes(*u.shape, A.shape[1]), u.device)
+        y, last = _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, ctx.cut, ck)
         ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, ck)
-        ctx.softplus = softplus
         ctx.set_materialize_grads(False)
         return y, last
 
@@ -287,7 +288,7 @@ class _Scan(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 12
         nB, T, nD = u.shape
-        N, G, dev = A.shape[1], _groups(Bm, 2), u.device
+        G, dev = _groups(Bm, 2), u.device
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
         dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
@@ -298,7 +299,7 @@ class _Scan(torch.autograd.Function):
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
         seqs = [_learn.seq(t) for t in (u, delta, z, Bm, Cm, None)]
-        p = _scan_desc(u, A, G, D, delta_bias, ctx.softplus, nB, T, seqs, None, None, lengths, ck, _cut())
+        p = _scan_desc(u, A, G, D, delta_bias, ctx.softplus, nB, T, seqs, None, None, lengths, ck, ctx.cut)
         g = _learn.SELSCAN_BARS.pack(*_learn.seq(dy), *(_learn.ptr(t) for t in (dlast, du, ddelta, dz, dBm, dCm, dA, dD, dbias, dstate)))
         with _learn.on_device(dev):
             n = lib.lqg_selscan_grad_workspace(p)
@@ -361,7 +362,7 @@ def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softpl
         y, last = _Scan.apply(*inputs, lengths, int(bool(softplus)), bool(return_state))
         _note_leaves(y.grad_fn, u.device)
     else:
-        y, last, _ = _scan_forward(*inputs, lengths, int(bool(softplus)), bool(return_state), False)
+        y, last = _scan_forward(*inputs, lengths, int(bool(softplus)), bool(return_state), _cut())
     return (y, last) if return_state else y
 
 

@@ -713,3 +713,12 @@ def test_gradients_of_workgroups_of_either_width(case, channels):
     with options.override(SELSCAN_CHANNELS=channels):
         for chunks in (1, 3):
             test_scan_gradients(case, chunks)
+
+
+def test_bytes_of_checkpoints():
+    from lqg_amd import _learn
+    lib = _learn.load()
+    for N in range(1, 65):
+        for B, T, D in ((1, 1, 1), (3, 16, 5), (2, 17, 7), (5, 1067, 771)):
+            p = _learn.SELSCAN.pack(_learn.T_F32, 1, B, T, D, N, 1, *(6 * _learn.NO_SEQ), *(3 * _learn.NO_PARAM), 0, 0, 0, 0, 0, 0)
+            assert ssm._checkpoint_bytes(B, T, D, N) == lib.lqg_selscan_checkpoint_bytes(p)
