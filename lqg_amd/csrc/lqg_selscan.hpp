@@ -261,7 +261,8 @@ __device__ inline float step_size(const ScanArgs& a, float raw) { return a.p.sof
 
 // ------------------------------------------------------------------------------------------------ forward
 // 8 x 2048 x 2048 x 16 bfloat16 with gate: 180 us on vector units that are issued to 78 % of the time, two waves a SIMD (their 24 cycles for
-// 64 states would take 85 us, the elements' softplus, silu and sums 40, the bytes 53); half of it, one wave a SIMD: 128.
+// 64 states would take 85 us, the elements' softplus, silu and sums 40, the bytes 53); half of it, one wave a SIMD: 128 (16
+// channels, two waves: 126).
 // CARRY: leave each chunk's end state from zero and its sum of dl instead of y.
 // Iteration i: finish tile i-1, prepare tile i+1, request tile i+3's rows and tile i+2's maps, walk tile i; one barrier.
 template <class IT, class S, bool CARRY>
