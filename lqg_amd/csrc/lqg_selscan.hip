@@ -46,7 +46,7 @@ int check(const lqg_selscan* p) {
 
 // states that the workgroups' shapes have room for (Shape::NP)
 long room_of(long N) { return N > 32 ? 64 : N > 16 ? 32 : N > 8 ? 16 : N > 4 ? 8 : 4; }
-int tile_of(long N) { return N > 32 ? 8 : 16; }
+int tile_of(long N, bool narrow) { return N > 32 && !narrow ? 8 : 16; }
 
 // How a scan is laid over the card: channels of a workgroup (16 or, with half the waves, 32), and pieces that the time axis is cut into.
 //
@@ -54,7 +54,7 @@ int tile_of(long N) { return N > 32 ? 8 : 16; }
 // while none has three, then growing with the waves (more 0: by whole rounds, of one wave a SIMD, which is all that registers allow).
 struct Passes { double one, two, more, unit; };   // unit: time of such a pass over that of one with 32 channels
 Passes passes(long N, bool grad, bool narrow) {
-  if (!grad) return !narrow ? Passes{1.1, 1.35, 0.68, 1.0} : N <= 4 ? Passes{1.2, 1.6, 1.0, 0.6} : Passes{1.0, 1.3, 0.6, N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58};
+  if (!grad) return !narrow ? Passes{1.03, 1.45, 0.68, 1.0} : N <= 4 ? Passes{1.2, 1.6, 1.0, 0.6} : Passes{1.0, 1.3, 0.6, N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58};
   if (!narrow) return N > 8 && N <= 16 ? Passes{1.05, 1.4, 0.66, 1.0} : Passes{1.05, 2.0, 0.0, 1.0};
   return N <= 4 ? Passes{1.05, 1.87, 1.0, 0.66} : N <= 8 ? Passes{1.15, 1.33, 0.73, 0.7} : Passes{1.0, 1.3, 0.63, N <= 16 ? 0.71 : 0.64};
 }
@@ -78,9 +78,11 @@ Cut cut(const Passes& p, double carry, long waves, long tiles) {
   return best;
 }
 
-// 16 channels: up to 32 states (forward always with up to 4, whose waves of 32 channels are few and long).  Measured, us with 32 / 16 channels,
+// 16 channels: up to 32 states, and beyond them forward without checkpoints, whose tiles of 16 steps backward has no registers for (always
+// with up to 4 states forward, whose waves of 32 channels are few and long).  Measured, us with 32 / 16 channels,
 // uncut, 2048 steps x 2048 channels (trials):  forward N = 4: 179 / 121 (4), 192 / 121 (8), 198 / 210 (16), 440 / 386 (32); N = 8: 148 / 119 (4),
-// 190 / 133 (8), 209 / 275 (16); N = 16: 126 / 91 (2), 128 / 126 (4), 177 / 204 (8); N = 32: 181 / 119 (2), 186 / 163 (4), 274 / 275 (8).  Backward
+// 190 / 133 (8), 209 / 275 (16); N = 16: 126 / 91 (2), 128 / 126 (4), 177 / 204 (8); N = 32: 181 / 119 (2), 186 / 163 (4), 274 / 275 (8);
+// N = 64: 307 / 175 (2), 311 / 260 (4), 457 / 450 (8).  Backward
 // N = 3: 512 / 359 (4), 541 / 362 (8), 551 / 634 (16); N = 6: 426 / 354 (4), 441 / 388 (8), 855 / 872 (16); N = 16: 380 / 274 (2), 395 / 351 (4),
 // 531 / 683 (8); N = 24: 599 / 499 (4), 1168 / 969 (8).  Over 132 sizes forward and 112 backward (N = 3 .. 32, 512 to 16384 steps, 256 channels
 // to 32 trials of 2048) width and cut chosen so are 2.3 % and 2.8 % slower than the best pair in the geometric mean, 24 % at most.
@@ -90,15 +92,16 @@ void lay_out(ScanArgs& a, bool grad) {
   auto with = [&](int channels) {
     const bool narrow = channels == 16;
     const Passes p = passes(N, grad, narrow);
-    const long bpg = (a.Dg + channels - 1) / channels;
-    Cut c = cut(p, grad ? (narrow ? 0.15 : 0.2) : narrow ? 0.55 : 0.6, bpg * a.p.G * a.p.B * waves, a.tiles);
+    const long bpg = (a.Dg + channels - 1) / channels, TT = tile_of(N, narrow), tiles = (a.p.T + TT - 1) / TT;
+    Cut c = cut(p, grad ? (narrow ? 0.15 : 0.2) : narrow ? 0.55 : 0.6, bpg * a.p.G * a.p.B * waves, tiles);
     c.time *= p.unit;
     if (best.pieces && c.time >= best.time) return;
     best = c;
     a.narrow = narrow;
     a.bpg = bpg;
+    a.tiles = tiles;
   };
-  const int asked = N > 32 ? 32 : a.p.channels ? a.p.channels : !grad && N <= 4 ? 16 : 0;
+  const int asked = N > 32 && (grad || a.p.checkpoints) ? 32 : a.p.channels ? a.p.channels : !grad && N <= 4 ? 16 : 0;
   if (asked != 16) with(32);
   if (asked != 32) with(16);
   a.blocks = a.bpg * a.p.G;
@@ -108,12 +111,10 @@ void lay_out(ScanArgs& a, bool grad) {
 ScanArgs describe(const lqg_selscan* p, bool grad) {
   ScanArgs a{};
   a.p = *p;
-  const long TT = tile_of(p->N);
   a.Dg = p->D / p->G;
-  a.tiles = (p->T + TT - 1) / TT;
   lay_out(a, grad);
   const long per = (a.tiles + a.chunks - 1) / a.chunks;
-  a.chunk = per * TT;
+  a.chunk = per * tile_of(p->N, a.narrow);
   a.chunks = (a.tiles + per - 1) / per;               // no empty chunk
   return a;
 }
@@ -146,7 +147,9 @@ extern "C" size_t lqg_selscan_workspace(const lqg_selscan* p) {
   return check(p) ? 0 : (size_t)carry_floats(describe(p, false)) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p) {
-  return check(p) ? 0 : (size_t)(p->B * describe(p, false).tiles * room_of(p->N) * p->D) * sizeof(float);
+  if (check(p)) return 0;
+  const long TT = tile_of(p->N, p->N <= 32);
+  return (size_t)(p->B * ((p->T + TT - 1) / TT) * room_of(p->N) * p->D) * sizeof(float);
 }
 extern "C" size_t lqg_selscan_grad_workspace(const lqg_selscan* p) {
   return check(p) ? 0 : (size_t)grad_space(describe(p, true)).total * sizeof(float);

@@ -994,7 +994,7 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
     }
     const dim3 g = grid(a.chunks, 0);
     hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
-  } else {
+  } else if constexpr (S::NS * S::CH < 64 || S::CH == 32) {              // (beyond 32 states: 32 channels only)
     if (a.chunks > 1) {
       const dim3 g = grid(a.chunks - 1, 1);
       hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
@@ -1008,6 +1008,7 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
 template <class IT> int by_states(int what, const ScanArgs& a, hipStream_t st) {
   const long N = a.p.N;
   if (a.narrow) {
+    if (N > 32) return launch<IT, Shape<4, 4, 16, 16>>(what, a, st);
     if (N > 16) return launch<IT, Shape<2, 4, 16, 16>>(what, a, st);
     if (N > 8) return launch<IT, Shape<1, 4, 16, 16>>(what, a, st);
     if (N > 4) return launch<IT, Shape<1, 2, 16, 16>>(what, a, st);

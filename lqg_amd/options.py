@@ -44,7 +44,7 @@ GRAPH             1         0: inference loops launch eagerly instead of replayi
 GRAPH_AFFINE      1         0: captured constructors are not collapsed into their measured affine map
 SETUP_KERNEL      1         0: PointMassBoundedActor is discretised by torch.linalg instead of lqg_point_mass_setup
 SELSCAN_CHUNKS    0         pieces (at most 64) the selective scan's time axis is cut into (0: the rule of lqg_selscan.hip)  -> lqg_selscan.chunks
-SELSCAN_CHANNELS  0         channels of a workgroup of the selective scan with up to 32 states: 16 or 32 (0: the rule)  -> lqg_selscan.channels
+SELSCAN_CHANNELS  0         channels of a workgroup of the selective scan, where both are there: 16 or 32 (0: the rule)  -> lqg_selscan.channels
 JIT               1         0: never compile an auxiliary lane-kernel library for an unlisted shape on demand
 
 Build / location variables (read once where the files are located, not behaviour switches): LQG_HIP_LIB, LQG_PAT_DIR,

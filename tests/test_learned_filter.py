@@ -722,3 +722,19 @@ def test_bytes_of_checkpoints():
         for B, T, D in ((1, 1, 1), (3, 16, 5), (2, 17, 7), (5, 1067, 771)):
             p = _learn.SELSCAN.pack(_learn.T_F32, 1, B, T, D, N, 1, *(6 * _learn.NO_SEQ), *(3 * _learn.NO_PARAM), 0, 0, 0, 0, 0, 0)
             assert ssm._checkpoint_bytes(B, T, D, N) == lib.lqg_selscan_checkpoint_bytes(p)
+
+
+@gpu
+@pytest.mark.parametrize("N", (33, 50, 64))
+def test_wide_states_with_and_without_checkpoints(N):
+    """Beyond 32 states a call that needs no gradient may use other workgroups than one that does: both within the bounds."""
+    case = (2, 300, 40, N, 1, F32, True, True, True, True, True, (300, 171))
+    i, kw = scan_case(*case[:6], **dict(zip(KEYS, case[6:])))
+    y, h, by, bh = scan_bounds(i, kw, F32)
+    for channels in (0, 16, 32):
+        for chunks in (0, 1, 3):
+            with options.override(SELSCAN_CHANNELS=channels, SELSCAN_CHUNKS=chunks):
+                for grads in (False, True):
+                    got, last = ssm.selective_scan(**{**i, "u": i["u"].detach().requires_grad_(grads)}, **kw, return_state=True)
+                    within(got.detach(), y, by, "y")
+                    within(last.detach(), h, bh, "state")
