@@ -54,7 +54,8 @@ int tile_of(long N, bool narrow) { return N > 32 && !narrow ? 8 : 16; }
 // while none has three, then growing with the waves (more 0: by whole rounds, of one wave a SIMD, which is all that registers allow).
 struct Passes { double one, two, more, unit; };   // unit: time of such a pass over that of one with 32 channels
 Passes passes(long N, bool grad, bool narrow) {
-  if (!grad) return !narrow ? Passes{1.03, 1.45, 0.68, 1.0} : N <= 4 ? Passes{1.2, 1.6, 1.0, 0.6} : Passes{1.0, 1.3, 0.6, N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58};
+  if (!grad && !narrow) return N <= 8 ? Passes{1.1, 1.35, 0.68, 1.0} : Passes{1.03, 1.45, 0.68, 1.0};
+  if (!grad) return N <= 4 ? Passes{1.2, 1.6, 1.0, 0.6} : Passes{1.0, 1.3, 0.6, N <= 8 ? 0.68 : N <= 16 ? 0.72 : 0.58};
   if (!narrow) return N > 8 && N <= 16 ? Passes{1.05, 1.4, 0.66, 1.0} : Passes{1.05, 2.0, 0.0, 1.0};
   return N <= 4 ? Passes{1.05, 1.87, 1.0, 0.66} : N <= 8 ? Passes{1.15, 1.33, 0.73, 0.7} : Passes{1.0, 1.3, 0.63, N <= 16 ? 0.71 : 0.64};
 }
@@ -85,7 +86,7 @@ Cut cut(const Passes& p, double carry, long waves, long tiles) {
 // N = 64: 307 / 175 (2), 311 / 260 (4), 457 / 450 (8).  Backward
 // N = 3: 512 / 359 (4), 541 / 362 (8), 551 / 634 (16); N = 6: 426 / 354 (4), 441 / 388 (8), 855 / 872 (16); N = 16: 380 / 274 (2), 395 / 351 (4),
 // 531 / 683 (8); N = 24: 599 / 499 (4), 1168 / 969 (8).  Over 132 sizes forward and 112 backward (N = 3 .. 32, 512 to 16384 steps, 256 channels
-// to 32 trials of 2048) width and cut chosen so are 2.3 % and 2.8 % slower than the best pair in the geometric mean, 24 % at most.
+// to 32 trials of 2048) width and cut chosen so are 2.0 % and 2.8 % slower than the best pair in the geometric mean, 24 % at most.
 void lay_out(ScanArgs& a, bool grad) {
   const long N = a.p.N, waves = N > 8 ? 4 : N > 4 ? 2 : 1;
   Cut best{};
