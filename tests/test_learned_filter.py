@@ -738,3 +738,31 @@ def test_wide_states_with_and_without_checkpoints(N):
                     got, last = ssm.selective_scan(**{**i, "u": i["u"].detach().requires_grad_(grads)}, **kw, return_state=True)
                     within(got.detach(), y, by, "y")
                     within(last.detach(), h, bh, "state")
+
+
+@gpu
+def test_gradients_beyond_32_bits():
+    """More than 2^31 elements: the gradients of the last channels are those of the same channels alone."""
+    T, D = 70000, 32768
+    u = torch.randn(1, T, D, dtype=BF16, device="cuda")
+    few = slice(D - 40, D)
+    A, m = -torch.rand(D, 1, device="cuda"), torch.randn(1, T, 1, dtype=BF16, device="cuda")
+    w = torch.randn(D, 3, dtype=BF16, device="cuda")
+    last = torch.tensor([T - 3], device="cuda", dtype=torch.int32)
+
+    def scan(x, a):
+        leaves = [t.detach().requires_grad_() for t in (x, x, a)]
+        y = ssm.selective_scan(*leaves, m, m, softplus=True, lengths=last)
+        return torch.autograd.grad(y, leaves, x)
+
+    v = u[..., few].contiguous()
+    for channels in (16, 32):
+        with options.override(SELSCAN_CHUNKS=1, SELSCAN_CHANNELS=channels):
+            whole, part = scan(u, A), scan(v, A[few].contiguous())
+        assert torch.equal(whole[0][..., few], part[0]) and torch.equal(whole[1][..., few], part[1]) and torch.equal(whole[2][few], part[2])
+        del whole
+    dx = []
+    for x, k in ((u, w), (v, w[few].contiguous())):
+        x = x.detach().requires_grad_()
+        dx.append(torch.autograd.grad(ssm.causal_conv(x, k, silu=True, lengths=last), x, x.detach())[0])
+    assert torch.equal(dx[0][..., few], dx[1])
