@@ -64,7 +64,7 @@ typedef struct lqg_selscan {
   const int32_t* lengths;
   void* checkpoints;
   int32_t chunks;                      /* pieces the time axis is cut into: 0 = the rule, else 1 .. 64 */
-  int32_t channels;                    /* of a workgroup: 0 = the rule, else 16 or 32 (32 in any case: N > 32 with checkpoints) */
+  int32_t channels;                    /* of a workgroup, where both are there: 0 = the rule, else 16 or 32 */
 } lqg_selscan;
 size_t lqg_selscan_workspace(const lqg_selscan* p);                  /* of p as it will be run, checkpoints included */
 size_t lqg_selscan_checkpoint_bytes(const lqg_selscan* p);

@@ -102,7 +102,7 @@ void lay_out(ScanArgs& a, bool grad) {
     a.bpg = bpg;
     a.tiles = tiles;
   };
-  const int asked = N > 32 && (grad || a.p.checkpoints) ? 32 : a.p.channels ? a.p.channels : !grad && N <= 4 ? 16 : 0;
+  const int asked = N > 32 && (grad || a.p.checkpoints) ? 32 : !grad && N <= 4 ? 16 : a.p.channels;
   if (asked != 16) with(32);
   if (asked != 32) with(16);
   a.blocks = a.bpg * a.p.G;

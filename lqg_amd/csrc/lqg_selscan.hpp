@@ -43,6 +43,7 @@ template <int NS_, int NW_, int TT_, int CH_ = 32> struct Shape {
   static constexpr int NP = NS * PS;          // states it has room for
   static constexpr int R = TT / PS;           // elements of a tile (TT x CH) that a thread prepares and finishes: rows PS apart
   static constexpr int Q = TT * NS / 16;      // registers of a tile's B (or C)
+  static constexpr bool FORWARD = CH == 16 || NP > 4, BACKWARD = CH == 32 || NP <= 32;    // the passes it serves
   static_assert(TT % PS == 0 && TT * NS % 16 == 0 && CH % 16 == 0, "");
 };
 
@@ -987,21 +988,24 @@ template <class IT, class S> int launch(int what, ScanArgs a, hipStream_t st) {
     return dim3((unsigned)(a.blocks * run * a.p.B));
   };
   // (nothing enters from the last chunk forward, nor from the first backward: their carries are not asked for)
-  if (what == 0) {
-    if (a.chunks > 1) {
-      const dim3 g = grid(a.chunks - 1, 0);
-      hipLaunchKernelGGL((k_scan<IT, S, true>), g, t, 0, st, a);
+  if constexpr (S::FORWARD)
+    if (what == 0) {
+      if (a.chunks > 1) {
+        const dim3 g = grid(a.chunks - 1, 0);
+        hipLaunchKernelGGL((k_scan<IT, S, true>), g, t, 0, st, a);
+      }
+      const dim3 g = grid(a.chunks, 0);
+      hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
     }
-    const dim3 g = grid(a.chunks, 0);
-    hipLaunchKernelGGL((k_scan<IT, S, false>), g, t, 0, st, a);
-  } else if constexpr (S::NS * S::CH < 64 || S::CH == 32) {              // (beyond 32 states: 32 channels only)
-    if (a.chunks > 1) {
-      const dim3 g = grid(a.chunks - 1, 1);
-      hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
+  if constexpr (S::BACKWARD)
+    if (what == 1) {
+      if (a.chunks > 1) {
+        const dim3 g = grid(a.chunks - 1, 1);
+        hipLaunchKernelGGL((k_scan_grad<IT, S, true>), g, t, 0, st, a);
+      }
+      const dim3 g = grid(a.chunks, 0);
+      hipLaunchKernelGGL((k_scan_grad<IT, S, false>), g, t, 0, st, a);
     }
-    const dim3 g = grid(a.chunks, 0);
-    hipLaunchKernelGGL((k_scan_grad<IT, S, false>), g, t, 0, st, a);
-  }
   return (int)last();
 }
 
