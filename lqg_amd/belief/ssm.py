@@ -102,6 +102,11 @@ def _separate(state, name, *others):
                 raise LqgHipError(f"{name}: it shares memory with another argument")
 
 
+def _like(t):
+    """A dense tensor of the same shape, type and device, not written (half the time of torch.empty with these as arguments)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 # Autograd adds up a leaf's gradient in a node that lives as long as any graph which holds it, on the stream it was made on.  A backward
 # pass under capture must not meet one of the default stream: the wait between the two streams breaks the capture and ends the process.
 _LEAF = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
@@ -130,7 +135,7 @@ def _conv_desc(x, w, bias, silu, B, T, D, xv, yv, state, state_out, lengths):
 
 def _conv_forward(x, w, bias, state, lengths, silu, want_state):
     B, T, D = x.shape
-    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    y = _like(x)
     last = torch.empty((B, w.shape[1] - 1, D), dtype=x.dtype, device=x.device) if want_state else None
     p = _conv_desc(x, w, bias, silu, B, T, D, _learn.seq(x), _learn.seq(y), state, last, lengths)
     with _learn.on_device(x.device):
@@ -160,7 +165,7 @@ class _Conv(torch.autograd.Function):
         dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
         dev = x.device
-        dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        dx = _like(x)
         dw, dbias = torch.empty_like(w), None if bias is None else torch.empty_like(bias)
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
@@ -227,7 +232,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False):
     _no_gradient("causal_conv_step", "use causal_conv", x, state, w, bias)
     _separate(state, "state", x, w, bias)
     _on_gpu(x)
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    y = _like(x)
     if not y.numel():
         return y
     p = _conv_desc(x, w, bias, int(bool(silu)), B, 1, D, _learn.row(x), _learn.row(y), state, None, None)
@@ -258,7 +263,7 @@ def _checkpoint_bytes(B, T, D, N):
 def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths, softplus, want_state, cut, ck=None):
     nB, T, nD = u.shape
     N, dev = A.shape[1], u.device
-    y = torch.empty((nB, T, nD), dtype=u.dtype, device=dev)
+    y = _like(u)
     last = torch.empty((nB, nD, N), dtype=torch.float32, device=dev) if want_state else None
     lib = _learn.load()
     p = _scan_desc(u, A, _groups(Bm, 2), D, delta_bias, softplus, nB, T, [_learn.seq(t) for t in (u, delta, z, Bm, Cm, y)], state, last,
@@ -292,9 +297,8 @@ class _Scan(torch.autograd.Function):
         dy = torch.zeros((nB, T, nD), dtype=u.dtype, device=dev) if dy is None else dy
         dy = _as_it_is(dy)
         dlast = None if dlast is None else dlast.contiguous()
-        new = lambda *shape: torch.empty(shape, dtype=u.dtype, device=dev)  # noqa: E731
-        du, ddelta, dz = new(nB, T, nD), new(nB, T, nD), None if z is None else new(nB, T, nD)
-        dBm, dCm, dA = new(*Bm.shape), new(*Cm.shape), torch.empty_like(A)
+        du, ddelta, dz = _like(u), _like(u), None if z is None else _like(u)
+        dBm, dCm, dA = _like(Bm), _like(Cm), torch.empty_like(A)
         dD, dbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
         dstate = None if state is None else torch.empty_like(state)
         lib = _learn.load()
@@ -375,7 +379,7 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, *, z=None, delta_bias=
     _no_gradient("selective_scan_step", "use selective_scan", u, delta, state, A, Bm, Cm, D, z, delta_bias)
     _separate(state, "state", u, delta, A, Bm, Cm, D, z, delta_bias)
     _on_gpu(u)
-    y = torch.empty((nB, nD), dtype=u.dtype, device=u.device)
+    y = _like(u)
     if not y.numel():
         return y
     p = _scan_desc(u, A, _groups(Bm, 1), D, delta_bias, int(bool(softplus)), nB, 1, [_learn.row(t) for t in (u, delta, z, Bm, Cm, y)],
